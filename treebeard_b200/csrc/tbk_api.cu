@@ -19,6 +19,7 @@
 #include "walk_rank_tiles.cuh"
 #include "walk_lanes.cuh"
 #include "packed_image.h"
+#include "last_error.h"
 
 #ifdef __SSE2__
 #include <emmintrin.h>
@@ -36,11 +37,9 @@
 #include <thread>
 #include <vector>
 
-namespace {
+static thread_local std::string g_last_error;
 
-thread_local std::string g_last_error;
-
-int fail(int code, const char *fmt, ...) {
+int tb::fail(int code, const char *fmt, ...) {
   char buf[1024];
   va_list ap;
   va_start(ap, fmt);
@@ -49,6 +48,10 @@ int fail(int code, const char *fmt, ...) {
   g_last_error = buf;
   return code;
 }
+
+namespace {
+
+using tb::fail;
 
 #define CUDA_TRY(expr)                                                                     \
   do {                                                                                     \
