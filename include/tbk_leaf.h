@@ -12,6 +12,8 @@
  * allocated and no state is kept between calls.  A call that asks for a workspace takes device memory of
  * the size that its *_workspace function states, 256-byte aligned, for its own use until its work on the
  * stream is done: calls that may run at the same time need workspaces of their own.
+ * `aligned` of these functions: 1 if x and weight begin at 16-byte boundaries and have row strides that are
+ * multiples of 8 elements; otherwise a call copies them first, and its workspace has room for that.
  * Inputs and outputs of one call must not overlap, except that `out` may be `residual`.
  *
  * Sums are held in fp32 and every output is rounded once from there; the order of all sums is fixed, so
@@ -58,8 +60,8 @@ TBK_EXPORT int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *lea
 /* out = activation(z) + residual, z = x weight^T + bias, and, where pre is given, pre = z.
  * x [n_rows, inputs], weight [outputs, inputs], bias [outputs] or NULL, residual [n_rows, outputs] or NULL.
  * type: TBK_TYPE_F16 or TBK_TYPE_BF16, of all of them. */
-TBK_EXPORT int tbk_linear_workspace(int64_t n_rows, int64_t inputs, int64_t outputs, int32_t type, int32_t device,
-                                    uint64_t *bytes);
+TBK_EXPORT int tbk_linear_workspace(int64_t n_rows, int64_t inputs, int64_t outputs, int32_t type, int32_t aligned,
+                                    int32_t device, uint64_t *bytes);
 TBK_EXPORT int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64_t ld_weight, const void *bias,
                           int32_t activation, const void *residual, int64_t ld_residual, void *out, int64_t ld_out,
                           void *pre, int64_t ld_pre, int64_t n_rows, int64_t inputs, int64_t outputs, int32_t type,
@@ -72,7 +74,7 @@ TBK_EXPORT int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64
  * pre may be NULL with TBK_ACT_IDENTITY; grad_x, grad_weight, grad_bias may each be NULL (not wanted).
  * dz is rounded to `type` before the two products (grad_bias is summed before that). */
 TBK_EXPORT int tbk_linear_backward_workspace(int64_t n_rows, int64_t inputs, int64_t outputs, int32_t type,
-                                             int32_t device, uint64_t *bytes);
+                                               int32_t aligned, int32_t device, uint64_t *bytes);
 TBK_EXPORT int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_t ld_x, const void *weight,
                                    int64_t ld_weight, const void *pre, int64_t ld_pre, int32_t activation,
                                    const void *skip, int64_t ld_skip, void *grad_x, int64_t ld_grad_x, void *grad_weight, int64_t ld_grad_weight,
@@ -83,8 +85,8 @@ TBK_EXPORT int tbk_linear_backward(const void *grad, int64_t ld_grad, const void
  * lse[n] = log sum_v exp(z[n, v]), loss[n] = lse[n] - z[n, labels[n]], both fp32.  A label outside
  * 0 .. classes-1 leaves its row out: loss 0.  labels: int64 (label_bytes 8) or int32 (4).  A class whose
  * bias is -inf has probability 0; a row of such classes only has lse = -inf. */
-TBK_EXPORT int tbk_class_loss_workspace(int64_t n_rows, int64_t width, int64_t classes, int32_t type, int32_t device,
-                                        uint64_t *bytes);
+TBK_EXPORT int tbk_class_loss_workspace(int64_t n_rows, int64_t width, int64_t classes, int32_t type,
+                                               int32_t aligned, int32_t device, uint64_t *bytes);
 TBK_EXPORT int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_weight, const void *bias,
                               const void *labels, int32_t label_bytes, float *loss, float *lse, int64_t n_rows,
                               int64_t width, int64_t classes, int32_t type, void *workspace, uint64_t workspace_bytes,
@@ -96,13 +98,17 @@ TBK_EXPORT int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, i
  * `type`, scaled by a power of two so that the largest |grad_loss| lies near the middle of the type's range
  * (grad_bias is summed before that). */
 TBK_EXPORT int tbk_class_loss_backward_workspace(int64_t n_rows, int64_t width, int64_t classes, int32_t type,
-                                                 int32_t device, uint64_t *bytes);
+                                               int32_t aligned, int32_t device, uint64_t *bytes);
 TBK_EXPORT int tbk_class_loss_backward(const float *grad_loss, const void *x, int64_t ld_x, const void *weight,
                                        int64_t ld_weight, const void *bias, const void *labels, int32_t label_bytes,
                                        const float *lse, void *grad_x, int64_t ld_grad_x, void *grad_weight,
                                        int64_t ld_grad_weight, void *grad_bias, int64_t n_rows, int64_t width,
                                        int64_t classes, int32_t type, void *workspace, uint64_t workspace_bytes,
                                        int32_t device, void *stream);
+
+/* Reads the status word of the matrix products on a device (synchronises with it): TBK_ERR_DEVICE_WAIT if a
+ * bounded wait inside one gave up since the last check, else TBK_OK. */
+TBK_EXPORT int tbk_leaf_check_status(int32_t device);
 
 #ifdef __cplusplus
 }

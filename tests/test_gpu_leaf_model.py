@@ -16,6 +16,12 @@ HALVES = [torch.bfloat16, torch.float16]
 STEP = 2.0 ** -23
 
 
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    lm.check_status(0)
+
+
 def rounding(want, dtype):
     return torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -25 if dtype is torch.float16 else 0.0)
 
@@ -194,6 +200,28 @@ def test_linear_backward(n, inputs, outputs, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n,inputs,outputs", [(2500, 1030, 3000), (300, 4000, 300), (1500, 30000, 1500), (30000, 1500, 1500)])
+def test_linear_of_many_tiles(n, inputs, outputs, dtype):
+    """Tiles of two blocks, sums cut into parts with either kind of tile, ragged edges of both."""
+    x, w = normal(n, inputs, dtype=dtype), normal(outputs, inputs, dtype=dtype, scale=inputs ** -0.5, seed=1)
+    b, r = normal(outputs, dtype=dtype, seed=2), normal(n, outputs, dtype=dtype, seed=3)
+    z, mass = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t()
+    off = (inputs + 2) * STEP * (mass + z.abs())
+    got, pre = lm.linear(x, w, b, "gelu", r, keep_pre=True)
+    near(pre, z, off)
+    want = ACT["gelu"][0](z) + r.double()
+    near(got, want, SLOPE * off + EVAL * (z.abs() + want.abs()))
+    del z, mass, off, want
+    dx, dw, db = lm.linear_backward(r, x, w, pre, "identity", skip=x)
+    g = r.double()                      # (no slope: dz is grad itself)
+    want = g @ w.double() + x.double()
+    near(dx, want, (outputs + 2) * STEP * (g.abs() @ w.double().abs() + want.abs()))
+    near(dw, g.t() @ x.double(), (n + 2) * STEP * (g.abs().t() @ x.double().abs()))
+    near(db, g.sum(0), (n + 2) * STEP * g.abs().sum(0))
+    assert torch.equal(dw, lm.linear_backward(r, x, w)[1])
+
+
+@pytest.mark.parametrize("dtype", HALVES)
 def test_linear_gradient_is_the_slope_of_linear(dtype):
     """Differences of the plain form in 64 bits, along random directions, against the kernels' gradients."""
     n, inputs, outputs = 40, 24, 56
@@ -262,7 +290,7 @@ def plain_loss(x, w, b, labels):
 
 
 CLASSES = [(1, 8, 2), (1, 512, 4000), (3, 5, 1), (4, 17, 7), (31, 64, 26), (64, 33, 64), (65, 96, 65), (128, 128, 256),
-           (200, 72, 255), (129, 250, 1030), (300, 16, 5003), (513, 40, 777), (1100, 24, 300)]
+           (200, 72, 255), (129, 250, 1030), (300, 16, 5003), (513, 40, 777), (1100, 24, 300), (3000, 136, 5000)]
 
 
 @pytest.mark.parametrize("dtype", HALVES)

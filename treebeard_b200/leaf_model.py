@@ -40,7 +40,8 @@ def lib():
         L.tbk_leaf_sum_backward_workspace.argtypes = [vp, i64, i64, i32, size]
         L.tbk_leaf_sum_backward.argtypes = [vp, vp, i64, i64, vp, i64, i64, i32, vp, i64, vp, u64, vp]
         for name in ("tbk_linear", "tbk_linear_backward", "tbk_class_loss", "tbk_class_loss_backward"):
-            getattr(L, name + "_workspace").argtypes = [i64, i64, i64, i32, i32, size]
+            getattr(L, name + "_workspace").argtypes = [i64, i64, i64, i32, i32, i32, size]
+        L.tbk_leaf_check_status.argtypes = [i32]
         L.tbk_linear.argtypes = [vp, i64, vp, i64, vp, i32, vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, vp, u64, i32, vp]
         L.tbk_linear_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, vp, i64, vp, i64, i64,
                                           i64, i32, vp, u64, i32, vp]
@@ -127,6 +128,16 @@ def _workspace(name, device, *sizes):
     torch = _torch()
     ws = torch.empty(need.value, dtype=torch.uint8, device=device)
     return ws, ws.data_ptr(), need.value
+
+
+def _readable(x, ld_x, weight, ld_w):
+    """Whether the kernels read x and weight where they are: rows that begin at multiples of 16 bytes."""
+    return int(not (x.data_ptr() | weight.data_ptr()) & 15 and (ld_x % 8 == 0 or x.shape[0] <= 1) and (ld_w % 8 == 0 or weight.shape[0] <= 1))
+
+
+def check_status(device: int = 0):
+    """Waits for the device; raises TbkError if a bounded wait inside a matrix product gave up since the last check."""
+    _check(lib().tbk_leaf_check_status(device))
 
 
 def _ptr(t):
@@ -239,7 +250,7 @@ def linear(x, weight, bias=None, activation: str = "identity", residual=None, ke
             same = residual is not None and out.data_ptr() == residual.data_ptr() and ld_o == ld_r
             _apart("out", out, x, weight, bias, None if same else residual)
         pre = torch.empty((n, outputs), dtype=x.dtype, device=device) if keep_pre else None
-        keep, ws, size = _workspace("tbk_linear", device, n, inputs, outputs, kind, device.index)
+        keep, ws, size = _workspace("tbk_linear", device, n, inputs, outputs, kind, _readable(x, ld_x, weight, ld_w), device.index)
         _check(lib().tbk_linear(x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), ACTIVATIONS[activation],
                                 _ptr(residual), ld_r, out.data_ptr(), ld_o, _ptr(pre), outputs, n, inputs, outputs, kind,
                                 ws, size, device.index, _stream_ptr(stream, device.index)))
@@ -268,7 +279,7 @@ def linear_backward(grad, x, weight, pre=None, activation: str = "identity", bia
     with _on(stream):
         grad_x, grad_w = torch.empty((n, inputs), dtype=x.dtype, device=device), torch.empty((outputs, inputs), dtype=x.dtype, device=device)
         grad_b = torch.empty(outputs, dtype=x.dtype, device=device) if bias else None
-        keep, ws, size = _workspace("tbk_linear_backward", device, n, inputs, outputs, kind, device.index)
+        keep, ws, size = _workspace("tbk_linear_backward", device, n, inputs, outputs, kind, _readable(x, ld_x, weight, ld_w), device.index)
         _check(lib().tbk_linear_backward(grad.data_ptr(), ld_g, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(pre), ld_p,
                                          ACTIVATIONS[activation], _ptr(skip), ld_s, grad_x.data_ptr(), inputs, grad_w.data_ptr(), inputs,
                                          _ptr(grad_b), n, inputs, outputs, kind, ws, size, device.index,
@@ -301,7 +312,7 @@ def class_loss(x, weight, labels, bias=None, stream=None):
     device = _device(x, weight, labels, bias)
     with _on(stream):
         loss, lse = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
-        keep, ws, size = _workspace("tbk_class_loss", device, n, width, classes, kind, device.index)
+        keep, ws, size = _workspace("tbk_class_loss", device, n, width, classes, kind, _readable(x, ld_x, weight, ld_w), device.index)
         _check(lib().tbk_class_loss(x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), labels.data_ptr(),
                                     labels.element_size(), loss.data_ptr(), lse.data_ptr(), n, width, classes, kind, ws, size,
                                     device.index, _stream_ptr(stream, device.index)))
@@ -319,7 +330,7 @@ def class_loss_backward(grad_loss, x, weight, labels, lse, bias=None, stream=Non
     with _on(stream):
         grad_x, grad_w = torch.empty((n, width), dtype=x.dtype, device=device), torch.empty((classes, width), dtype=x.dtype, device=device)
         grad_b = torch.empty(classes, dtype=x.dtype, device=device) if bias is not None else None
-        keep, ws, size = _workspace("tbk_class_loss_backward", device, n, width, classes, kind, device.index)
+        keep, ws, size = _workspace("tbk_class_loss_backward", device, n, width, classes, kind, _readable(x, ld_x, weight, ld_w), device.index)
         _check(lib().tbk_class_loss_backward(grad_loss.data_ptr(), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias),
                                              labels.data_ptr(), labels.element_size(), lse.data_ptr(), grad_x.data_ptr(), width,
                                              grad_w.data_ptr(), width, _ptr(grad_b), n, width, classes, kind, ws, size,
