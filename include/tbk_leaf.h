@@ -45,9 +45,10 @@ TBK_EXPORT int64_t tbk_leaf_map_rows(const tbk_leaf_map *map); /* leaves of all 
 /* out[n, :] = sum over trees t of table[row(t, leaf_ids[n, t]), :].  An id that is no leaf of its tree
  * (negative, an inner node, beyond the tree) adds nothing; a row without any leaf gets zeros.
  * type: any TBK_TYPE_*, of table and out. */
+TBK_EXPORT int tbk_leaf_sum_workspace(const tbk_leaf_map *map, int64_t n_rows, int64_t width, int32_t type, uint64_t *bytes);
 TBK_EXPORT int tbk_leaf_sum(const tbk_leaf_map *map, const int32_t *leaf_ids, int64_t n_rows, int64_t ld_ids,
                             const void *table, int64_t ld_table, int64_t width, int32_t type, void *out,
-                            int64_t ld_out, void *stream);
+                            int64_t ld_out, void *workspace, uint64_t workspace_bytes, void *stream);
 
 /* The gradient of tbk_leaf_sum with respect to the table: out[r, :] = sum of grad[n, :] over the (n, t)
  * with row(t, leaf_ids[n, t]) = r, zeros for leaves that no row reached. */

@@ -28,7 +28,7 @@ def refused(status, text=None):
 
 def test_every_declared_symbol_is_exported_and_bound():
     names = declared("tbk_leaf.h", "TBK_EXPORT")
-    assert len(names) == 15 and len(set(names)) == 15
+    assert len(names) == 16 and len(set(names)) == 16
     for name in names:
         assert getattr(lm.lib(), name).argtypes is not None
 
@@ -52,7 +52,7 @@ def test_the_library_checks_its_own_arguments():
     """No device is touched before the arguments hold: made-up addresses are never followed."""
     L, p = lm.lib(), 1 << 20
     err = lambda: L.tbk_last_error().decode()
-    assert L.tbk_leaf_sum(None, p, 1, 1, p, 1, 1, 0, p, 1, None) == INVALID
+    assert L.tbk_leaf_sum(None, p, 1, 1, p, 1, 1, 0, p, 1, None, 0, None) == INVALID
     assert L.tbk_leaf_sum_backward(None, p, 1, 1, p, 1, 1, 0, p, 1, p, 4, None) == INVALID
 
     def linear(x=p, ld_x=8, w=p, act=0, out=p, n=4, inputs=8, outputs=4, kind=2):

@@ -7,8 +7,10 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstring>
 #include <memory>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #define CUDA_TRY(expr)                                                                                            \
@@ -90,12 +92,19 @@ int check_workspace(const void *p, uint64_t have, uint64_t need) {
     if (rc__) return rc__;      \
   } while (0)
 
-template <class F> int with_type(int32_t type, F f) {
-  switch (type) {
-  case TBK_TYPE_F32: return f(float());
-  case TBK_TYPE_F16: return f(__half());
-  default: return f(__nv_bfloat16());
-  }
+// f(element type, bytes that are moved at a time)
+template <class F> int with_piece(int32_t type, int bytes, F f) {
+  auto sized = [&](auto t) {
+    switch (bytes) {
+    case 16: return f(t, std::integral_constant<int, 16>());
+    case 8: return f(t, std::integral_constant<int, 8>());
+    case 4: return f(t, std::integral_constant<int, 4>());
+    default:
+      if constexpr (sizeof(t) == 2) return f(t, std::integral_constant<int, 2>());
+      else return f(t, std::integral_constant<int, 4>());
+    }
+  };
+  return type == TBK_TYPE_F32 ? sized(float()) : type == TBK_TYPE_F16 ? sized(__half()) : sized(__nv_bfloat16());
 }
 template <class F> int with_half(int32_t type, F f) { return type == TBK_TYPE_F16 ? f(__half()) : f(__nv_bfloat16()); }
 
@@ -292,6 +301,64 @@ struct LossGradParts {
   }
 };
 
+// The largest power of two, 16 at most, that divides the addresses and lengths of all rows of two matrices.
+int piece_bytes(int32_t type, int64_t width, const void *p, int64_t ld_p, int64_t rows_p, const void *q, int64_t ld_q, int64_t rows_q) {
+  const uint64_t size = type == TBK_TYPE_F32 ? 4 : 2;
+  const uint64_t all = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | width * size | (rows_p > 1 ? ld_p * size : 0) |
+                       (rows_q > 1 ? ld_q * size : 0) | 16;
+  return (int)(all & (~all + 1));
+}
+// Lanes (as a power of two) that share a row, 16 bytes each.
+int lanes_of(int64_t width, int32_t type) {
+  const int64_t wanted = tiles_of(width, type == TBK_TYPE_F32 ? 4 : 8);
+  int log2 = 0;
+  while (log2 < 5 && (1 << log2) < wanted) ++log2;
+  return log2;
+}
+
+// How a leaf sum is cut.  Up to two rows per multiprocessor: a block per row, trees over its lane groups.
+// Above that: blocks of 64 rows per lane group and warp, and ranges of trees (joined afterwards) so that the
+// multiprocessors are evenly filled; a range costs a round trip of its fp32 sums.
+struct LeafSumPlan {
+  bool by_row;
+  int lanes_log2, threads, trees_per_part;
+  unsigned columns, blocks, parts = 1;
+  int64_t ld_parts;
+  LeafSumPlan(int64_t n, int64_t width, int32_t type, int64_t trees, int sms) {
+    const int elems = type == TBK_TYPE_F32 ? 4 : 8;
+    lanes_log2 = lanes_of(width, type);
+    const int lanes = 1 << lanes_log2;
+    columns = (unsigned)tiles_of(width, (int64_t)elems << lanes_log2);
+    ld_parts = tiles_of(width, elems) * elems;
+    by_row = n <= 2 * sms;
+    trees_per_part = (int)trees;
+    if (by_row) {
+      threads = (int)std::clamp<int64_t>(tiles_of(tiles_of(trees, 8) * lanes, 32) * 32, 32, 1024);
+      blocks = (unsigned)n;
+      return;
+    }
+    const int64_t rows_per_warp = (32 / lanes) * tb::kLeafRows;
+    threads = (int)std::min<int64_t>(512, tiles_of(n, rows_per_warp) * 32);
+    blocks = (unsigned)tiles_of(n, threads / 32 * rows_per_warp);
+    const double gather = (double)n * trees * width * (32 / elems) / 8 / 15e6, trip = (double)n * ld_parts * 8 / 4e6; // us
+    double least = 1e300;
+    for (int64_t p = 1; p <= std::min<int64_t>(64, tiles_of(trees, 2 * lanes)); ++p) {
+      const double units = (double)blocks * columns * p, cost = gather * std::ceil(units / sms) * sms / units + (p > 1 ? trip * p + 4 : 0);
+      if (cost < least) least = cost, parts = (unsigned)p;
+    }
+    trees_per_part = (int)tiles_of(tiles_of(trees, parts), lanes) * lanes;
+    parts = (unsigned)tiles_of(trees, trees_per_part);
+  }
+};
+
+struct LeafGradParts {
+  int64_t ld;
+  uint32_t *numbers;
+  float *sums;
+  LeafGradParts(Parts &w, int64_t n, int64_t width, int64_t trees, int64_t rows)
+      : ld(up8(n)), numbers(w.take<uint32_t>(trees * ld)), sums(w.take<float>(n > tb::kLeafChunk ? rows * width : 0)) {}
+};
+
 } // namespace
 
 extern "C" {
@@ -300,34 +367,47 @@ int tbk_leaf_map_create(const tbk_forest_arrays *fa, int32_t device, tbk_leaf_ma
   if (!out) return fail(TBK_ERR_INVALID, "null argument");
   *out = nullptr;
   if (!fa || !fa->tree_off || !fa->left) return fail(TBK_ERR_INVALID, "null forest array");
-  if (fa->num_trees < 1 || fa->num_trees > kMost) return fail(TBK_ERR_INVALID, "a leaf map needs a tree at least");
+  if (fa->num_trees < 1) return fail(TBK_ERR_INVALID, "a leaf map needs a tree at least");
+  if (fa->num_trees > 1 << 21) return fail(TBK_ERR_UNSUPPORTED, "more than %d trees", 1 << 21);
   if (fa->tree_off[0] != 0) return fail(TBK_ERR_INVALID, "tree_off does not begin with 0");
   for (int64_t t = 0; t < fa->num_trees; ++t)
     if (fa->tree_off[t + 1] <= fa->tree_off[t] || fa->tree_off[t + 1] - fa->tree_off[t] > kMost) return fail(TBK_ERR_INVALID, "tree %lld has no nodes, or too many", (long long)t);
   try {
     std::unique_ptr<tbk_leaf_map> map(new tbk_leaf_map);
-    const int64_t trees = fa->num_trees, nodes = fa->tree_off[trees];
-    std::vector<long long> tree_off(fa->tree_off, fa->tree_off + trees + 1);
-    std::vector<int32_t> node_row((size_t)nodes), row_off((size_t)trees + 1);
+    const int64_t trees = fa->num_trees;
+    std::vector<uint2> words;
+    std::vector<int2> tree((size_t)trees + 1);
+    std::vector<int32_t> row_off((size_t)trees + 1);
     int64_t rows = 0;
     for (int64_t t = 0; t < trees; ++t) {
+      const int64_t nodes = fa->tree_off[t + 1] - fa->tree_off[t];
+      const int32_t *left = fa->left + fa->tree_off[t];
+      tree[t] = make_int2((int)words.size(), (int)nodes);
       row_off[t] = (int32_t)rows;
-      for (int64_t i = tree_off[t]; i < tree_off[t + 1]; ++i) node_row[i] = fa->left[i] < 0 ? (int32_t)rows++ : -1;
-      if (rows > kMost) return fail(TBK_ERR_UNSUPPORTED, "more than %lld leaves", (long long)kMost);
+      for (int64_t i = 0; i < nodes; i += 32) {
+        uint2 w = make_uint2(0, (uint32_t)rows);
+        for (int64_t k = i; k < std::min(nodes, i + 32); ++k)
+          if (left[k] < 0) w.x |= 1u << (k - i), ++rows;
+        words.push_back(w);
+      }
+      if (rows > kMost || words.size() > (size_t)kMost) return fail(TBK_ERR_UNSUPPORTED, "more than %lld leaves", (long long)kMost);
       map->max_rows = std::max<int64_t>(map->max_rows, rows - row_off[t]);
     }
+    tree[trees] = make_int2((int)words.size(), 0);
     row_off[trees] = (int32_t)rows;
     map->device = device;
     map->rows = rows;
-    const size_t a = tree_off.size() * 8, b = (node_row.size() * 4 + 15) / 16 * 16, c = row_off.size() * 4;
+    const size_t a = words.size() * 8, b = tree.size() * 8, c = row_off.size() * 4;
+    std::vector<unsigned char> image(a + b + c);
+    std::memcpy(image.data(), words.data(), a);
+    std::memcpy(image.data() + a, tree.data(), b);
+    std::memcpy(image.data() + a + b, row_off.data(), c);
     OnDevice on(device);
     CUDA_TRY(on.error);
-    CUDA_TRY(cudaMalloc(&map->mem, a + 16 + b + c));
-    unsigned char *p = static_cast<unsigned char *>(map->mem), *pb = p + (a + 15) / 16 * 16, *pc = pb + b;
-    map->view = {reinterpret_cast<long long *>(p), reinterpret_cast<int32_t *>(pb), reinterpret_cast<int32_t *>(pc), trees};
-    cudaError_t e = cudaMemcpy(p, tree_off.data(), a, cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMemcpy(pb, node_row.data(), node_row.size() * 4, cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMemcpy(pc, row_off.data(), c, cudaMemcpyHostToDevice);
+    CUDA_TRY(cudaMalloc(&map->mem, image.size()));
+    unsigned char *p = static_cast<unsigned char *>(map->mem);
+    map->view = {reinterpret_cast<uint2 *>(p), reinterpret_cast<int2 *>(p + a), reinterpret_cast<int32_t *>(p + a + b), trees};
+    const cudaError_t e = cudaMemcpy(p, image.data(), image.size(), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
       cudaFree(map->mem);
       return fail(TBK_ERR_CUDA, "upload of the leaf map failed: %s", cudaGetErrorString(e));
@@ -356,19 +436,45 @@ static int check_leaf_call(const tbk_leaf_map *map, const int32_t *ids, int64_t 
   return check_matrix("leaf_ids", ids, ld_ids, n, map->view.num_trees);
 }
 
+int tbk_leaf_sum_workspace(const tbk_leaf_map *map, int64_t n, int64_t width, int32_t type, uint64_t *bytes) {
+  if (!map || !bytes) return fail(TBK_ERR_INVALID, "null argument");
+  TRY(check_sizes("leaf sum", n, width, 1));
+  const LeafSumPlan plan(n, width, type, map->view.num_trees, multiprocessors(map->device));
+  *bytes = plan.parts > 1 ? (uint64_t)plan.parts * n * plan.ld_parts * 4 : 0;
+  return TBK_OK;
+}
+
 int tbk_leaf_sum(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, const void *table, int64_t ld_table,
-                 int64_t width, int32_t type, void *out, int64_t ld_out, void *stream) {
+                 int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream_) {
   TRY(check_leaf_call(map, ids, n, ld_ids, width, type));
   TRY(check_matrix("table", table, ld_table, map->rows, width));
   TRY(check_matrix("out", out, ld_out, n, width));
   if (n == 0) return TBK_OK;
+  uint64_t need = 0;
+  TRY(tbk_leaf_sum_workspace(map, n, width, type, &need));
+  TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(map->device);
   CUDA_TRY(on.error);
-  return with_type(type, [&](auto t) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  const LeafSumPlan plan(n, width, type, map->view.num_trees, multiprocessors(map->device));
+  return with_piece(type, piece_bytes(type, width, table, ld_table, map->rows, out, ld_out, n), [&](auto t, auto v) {
     using T = decltype(t);
-    tb::tb_leaf_sum_kernel<T><<<(unsigned)n, (unsigned)std::min<int64_t>(256, (width + 31) / 32 * 32), 0, (cudaStream_t)stream>>>(
-        map->view, ids, ld_ids, (const T *)table, ld_table, width, (T *)out, ld_out, n);
+    constexpr int V = decltype(v)::value;
+    if (plan.by_row) {
+      tb::tb_leaf_sum_row_kernel<T, V><<<dim3((unsigned)n, plan.columns), plan.threads, 0, stream>>>(map->view, ids, ld_ids, (const T *)table, ld_table,
+                                                                                                     width, plan.lanes_log2, (T *)out, ld_out);
+      CUDA_TRY(cudaGetLastError());
+      return (int)TBK_OK;
+    }
+    float *parts = plan.parts > 1 ? (float *)ws : nullptr;
+    tb::tb_leaf_sum_kernel<T, V><<<dim3(plan.blocks, plan.columns, plan.parts), plan.threads, 0, stream>>>(
+        map->view, ids, ld_ids, (const T *)table, ld_table, width, plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, n, plan.trees_per_part);
     CUDA_TRY(cudaGetLastError());
+    if (parts) {
+      const int64_t threads = n * plan.ld_parts / tb::Share<T, V>::kElems;
+      tb::tb_leaf_sum_join_kernel<T, V><<<(unsigned)tiles_of(threads, 256), 256, 0, stream>>>(parts, plan.ld_parts, plan.parts, (T *)out, ld_out, width, n);
+      CUDA_TRY(cudaGetLastError());
+    }
     return (int)TBK_OK;
   });
 }
@@ -377,24 +483,44 @@ int tbk_leaf_sum_backward_workspace(const tbk_leaf_map *map, int64_t n, int64_t 
   if (!map || !bytes) return fail(TBK_ERR_INVALID, "null argument");
   (void)type;
   TRY(check_sizes("leaf sum", n, width, 1));
-  *bytes = (uint64_t)map->rows * width * 4;
+  Parts w{nullptr};
+  LeafGradParts parts(w, n, width, map->view.num_trees, map->rows);
+  *bytes = w.used;
   return TBK_OK;
 }
 
 int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, const void *grad, int64_t ld_grad,
-                          int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream) {
+                          int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream_) {
   TRY(check_leaf_call(map, ids, n, ld_ids, width, type));
   TRY(check_matrix("grad", grad, ld_grad, n, width));
   TRY(check_matrix("out", out, ld_out, map->rows, width));
   uint64_t need = 0;
   TRY(tbk_leaf_sum_backward_workspace(map, n, width, type, &need));
-  TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(map->device);
   CUDA_TRY(on.error);
-  return with_type(type, [&](auto t) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  const size_t size = type == TBK_TYPE_F32 ? 4 : 2;
+  if (n == 0) {
+    CUDA_TRY(cudaMemset2DAsync(out, (size_t)ld_out * size, 0, (size_t)width * size, (size_t)map->rows, stream));
+    return TBK_OK;
+  }
+  TRY(check_workspace(ws, ws_bytes, need));
+  Parts w{(unsigned char *)ws};
+  const int64_t trees = map->view.num_trees;
+  LeafGradParts parts(w, n, width, trees, map->rows);
+  tb::tb_leaf_numbers_kernel<<<dim3((unsigned)std::min<int64_t>(tiles_of(n, 32), 4096), (unsigned)tiles_of(trees, 32)), 256, 0, stream>>>(map->view, ids, ld_ids, parts.numbers, parts.ld, n);
+  CUDA_TRY(cudaGetLastError());
+  return with_piece(type, piece_bytes(type, width, grad, ld_grad, n, out, ld_out, map->rows), [&](auto t, auto v) {
     using T = decltype(t);
-    tb::tb_leaf_grad_kernel<T><<<dim3((unsigned)map->view.num_trees, (unsigned)tiles_of(width, 32)), 32, 0, (cudaStream_t)stream>>>(
-        map->view, ids, ld_ids, (const T *)grad, ld_grad, width, (float *)ws, (T *)out, ld_out, n);
+    constexpr int V = decltype(v)::value;
+    const auto kernel = tb::tb_leaf_grad_kernel<T, V>;
+    const int lanes_log2 = lanes_of(width, type), range = (int)std::min<int64_t>(map->max_rows, tb::kLeafRange);
+    const int chunk = (int)std::min<int64_t>(n, tb::kLeafChunk), smem = tb::leaf_grad_smem(chunk, range);
+    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tb::leaf_grad_smem(tb::kLeafChunk, tb::kLeafRange)));
+    const dim3 grid((unsigned)trees, (unsigned)tiles_of(width, (16 / size) << lanes_log2), (unsigned)tiles_of(map->max_rows, range));
+    if (grid.y > 65535 || grid.z > 65535) return fail(TBK_ERR_UNSUPPORTED, "leaf_sum_backward: too many columns or leaves of a tree");
+    kernel<<<grid, 32 * tb::kLeafGradWarps, smem, stream>>>(map->view, parts.numbers, parts.ld, (const T *)grad, ld_grad, width, lanes_log2, parts.sums,
+                                                            (T *)out, ld_out, n, chunk, range);
     CUDA_TRY(cudaGetLastError());
     return (int)TBK_OK;
   });

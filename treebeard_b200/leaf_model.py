@@ -36,7 +36,8 @@ def lib():
         L.tbk_leaf_map_free.argtypes = [vp]
         L.tbk_leaf_map_rows.argtypes = [vp]
         L.tbk_leaf_map_rows.restype = i64
-        L.tbk_leaf_sum.argtypes = [vp, vp, i64, i64, vp, i64, i64, i32, vp, i64, vp]
+        L.tbk_leaf_sum_workspace.argtypes = [vp, i64, i64, i32, size]
+        L.tbk_leaf_sum.argtypes = [vp, vp, i64, i64, vp, i64, i64, i32, vp, i64, vp, u64, vp]
         L.tbk_leaf_sum_backward_workspace.argtypes = [vp, i64, i64, i32, size]
         L.tbk_leaf_sum_backward.argtypes = [vp, vp, i64, i64, vp, i64, i64, i32, vp, i64, vp, u64, vp]
         for name in ("tbk_linear", "tbk_linear_backward", "tbk_class_loss", "tbk_class_loss_backward"):
@@ -188,16 +189,17 @@ def leaf_sum(leaves: LeafMap, ids, table, out=None, stream=None):
     torch = _torch()
     ld_table = _matrix("table", table, table.dtype, leaves.num_rows)
     ld_ids, device = _leaf_call(leaves, ids, table, "leaf_sum")
-    n, width = ids.shape[0], table.shape[1]
+    n, width, kind = ids.shape[0], table.shape[1], _types[table.dtype]
     with _on(stream):
         if out is None:
             out = torch.empty((n, width), dtype=table.dtype, device=device)
         else:
             _device(ids, out)
             _apart("out", out, ids, table)
-        _check(lib().tbk_leaf_sum(leaves._h, ids.data_ptr(), n, ld_ids, table.data_ptr(), ld_table, width,
-                                  _types[table.dtype], out.data_ptr(), _matrix("out", out, table.dtype, n, width),
-                                  _stream_ptr(stream, device.index)))
+        ld_out = _matrix("out", out, table.dtype, n, width)
+        keep, ws, size = _workspace("tbk_leaf_sum", device, leaves._h, n, width, kind)
+        _check(lib().tbk_leaf_sum(leaves._h, ids.data_ptr(), n, ld_ids, table.data_ptr(), ld_table, width, kind,
+                                  out.data_ptr(), ld_out, ws, size, _stream_ptr(stream, device.index)))
     return out
 
 
