@@ -15,7 +15,8 @@
 // All waits are bounded: one that gives up ends the launch with a word in tb_dense_status.
 #pragma once
 #include <cuda.h>
-#include "leaf_sum.cuh"
+#include <cstdint>
+#include "element.cuh"
 
 namespace tb {
 
@@ -308,18 +309,54 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kDenseThr
 
 // ---- what becomes of a tile ---------------------------------------------------------------------
 
+__device__ __forceinline__ float exp2_fast(float x) { // within 2 steps of 2^-23; below 2^-126: 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float inverse_fast(float x) { // within a step of 2^-23
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
+
+// Phi(z), the integral of the normal distribution, and exp(-z^2 / 2).  erfc's shape after Hastings
+// (Approximations for Digital Computers, 1955): Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.33 |z|);
+// P was fitted here, by reweighted least squares, for the relative error: below 1e-6 for all z.  Without
+// branches, since a warp's values need both sides of any (the library's erff took most of a layer's time).
+__device__ __forceinline__ float normal_integral(float z, float *bell) {
+  const float a = fabsf(z), t = inverse_fast(fmaf(a, 0.33f, 1.f));
+  float p = fmaf(0.0332859295f, t, -0.105665717f);
+  p = fmaf(p, t, 0.067432403f);
+  p = fmaf(p, t, 0.0334278586f);
+  p = fmaf(p, t, 0.0910052722f);
+  p = fmaf(p, t, 0.117216671f);
+  p = fmaf(p, t, 0.13164699f);
+  p = fmaf(p, t, 0.131651081f);
+  *bell = exp2_fast(z * z * (-0.5f * kLog2e));
+  const float tail = *bell * t * p;
+  return z >= 0.f ? 1.f - tail : tail;
+}
 __device__ __forceinline__ float act_value(float z, int act) {
   if (act == 1) return z < 0.f ? 0.f : z; // (NaN stays)
-  if (act == 2) return 0.5f * z * (1.f + erff(z * 0.70710678f));
-  if (act == 3) return z / (1.f + expf(-z));
+  if (act == 2) {
+    float bell;
+    return z * normal_integral(z, &bell);
+  }
+  if (act == 3) return z * inverse_fast(1.f + exp2_fast(-kLog2e * z));
   return z;
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
   if (act == 1) return z > 0.f ? 1.f : 0.f;
-  if (act == 2) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+  if (act == 2) {
+    float bell;
+    const float w = normal_integral(z, &bell);
+    return fmaf(z * 0.39894228f, bell, w);
+  }
   if (act == 3) {
-    const float s = 1.f / (1.f + expf(-z));
-    return s * (1.f + z * (1.f - s));
+    const float s = inverse_fast(1.f + exp2_fast(-kLog2e * z));
+    return s * fmaf(z, 1.f - s, 1.f);
   }
   return 1.f;
 }
@@ -374,6 +411,20 @@ template <class F> __device__ __forceinline__ void turned(const float (&v)[32], 
   __syncwarp();
 }
 
+// The same with a lane per column: f(row, value), for results whose rows begin anywhere: a warp then writes 32
+// neighbouring elements at a time instead of every eighth.
+template <class F> __device__ __forceinline__ void turned_columns(const float (&v)[32], unsigned char *mine, F f) {
+  const int lane = threadIdx.x % 32;
+  float4 *s = reinterpret_cast<float4 *>(mine);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[lane * 8 + (i ^ (lane & 7))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  const float *w = reinterpret_cast<const float *>(mine) + lane % 4;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) f(r, w[(r * 8 + ((lane / 4) ^ (r & 7))) * 4]);
+  __syncwarp();
+}
+
 // y = activation(z + bias) + residual, and z + bias
 template <class T> struct LinearEnd {
   const T *bias, *residual;
@@ -381,6 +432,12 @@ template <class T> struct LinearEnd {
   long long ld_residual, ld_out, ld_pre;
   int act;
   bool vec_residual, vec_out, vec_pre, vec_bias;
+  __device__ __forceinline__ void finish1(float c, long long m, long long n) const {
+    const float z = bias ? c + to_float(bias[n]) : c;
+    if (pre) pre[m * ld_pre + n] = from_float<T>(z);
+    const float y = act_value(z, act);
+    out[m * ld_out + n] = from_float<T>(residual ? y + to_float(residual[m * ld_residual + n]) : y);
+  }
   __device__ __forceinline__ void finish8(const float (&c)[8], long long m, long long n, long long N) const {
     const int have = (int)min(8ll, N - n);
     float z[8], b[8];
@@ -413,6 +470,16 @@ template <class T> struct SumEnd {
   long long ld_out, ld_skip;
   const float *scale; // divides the result; null: 1
   bool first, last, vec_out, vec_skip;
+  __device__ __forceinline__ void finish1(float c, long long m, long long n) const {
+    float *s = sums + m * ld + n;
+    if (!first) c += *s;
+    if (!last) {
+      *s = c;
+      return;
+    }
+    if (scale) c *= 1.f / *scale;
+    out[m * ld_out + n] = from_float<T>(skip ? c + to_float(skip[m * ld_skip + n]) : c);
+  }
   __device__ __forceinline__ void finish8(const float (&c)[8], long long m, long long n, long long N) const {
     const int have = (int)min(8ll, N - n);
     float v[8];
@@ -452,9 +519,14 @@ template <class F> struct WholeEnd {
   __device__ __forceinline__ void chunk(State &, const DenseProblem &p, const float (&v)[32], long long row, long long n, const DenseUnit &,
                                         unsigned char *mine) const {
     const long long m0 = row - threadIdx.x % 32;
-    turned(v, mine, [&](int r, int c, const float (&w)[8]) {
-      if (m0 + r < p.M && n + c < p.N) f.finish8(w, m0 + r, n + c, p.N);
-    });
+    if (f.vec_out)
+      turned(v, mine, [&](int r, int c, const float (&w)[8]) {
+        if (m0 + r < p.M && n + c < p.N) f.finish8(w, m0 + r, n + c, p.N);
+      });
+    else
+      turned_columns(v, mine, [&](int r, float w) {
+        if (m0 + r < p.M && n + threadIdx.x % 32 < p.N) f.finish1(w, m0 + r, n + threadIdx.x % 32);
+      });
   }
   __device__ __forceinline__ void stop(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
 };
@@ -495,13 +567,6 @@ __global__ void __launch_bounds__(256) tb_dense_join_kernel(const float *parts, 
 __device__ __forceinline__ long long label_at(const void *labels, int bytes, long long m) {
   return bytes == 8 ? static_cast<const long long *>(labels)[m] : static_cast<const int *>(labels)[m];
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
-
 // The biases of a warp's 128 (or 64) columns of a tile in units of log2, in its shared memory; -inf for
 // columns behind the last class, which thereby have probability 0.
 template <class T, int COLS>
@@ -571,19 +636,29 @@ template <class T, int COLS> struct LseEnd {
     if (row < p.M) parts[(2ll * u.chunk + half) * p.M + row] = make_float2(s.top, s.sum);
   }
 };
-__global__ void __launch_bounds__(128) tb_loss_join_kernel(const float2 *parts, int count, const float *at, const void *labels, int label_bytes,
-                                                           long long classes, float *loss, float *lse, long long rows) {
-  const long long m = (long long)blockIdx.x * 128 + threadIdx.x;
-  if (m >= rows) return;
+// A row's logarithm and loss from its parts: a lane per row, the parts over the block's warps.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const float2 *parts, int count, const float *at, const void *labels, int label_bytes,
+                                                                       long long classes, float *loss, float *lse, long long rows) {
+  __shared__ float2 mine[kJoinWarps][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const long long m = (long long)blockIdx.x * 32 + lane;
   float top = -INFINITY, sum = 0.f;
-  for (int t = 0; t < count; ++t) top = fmaxf(top, parts[t * rows + m].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  for (int t = 0; t < count; ++t) {
-    const float2 q = parts[t * rows + m];
-    sum += q.y * exp2_fast(q.x - ref);
+  auto join = [&](float2 q) {
+    const float most = fmaxf(top, q.x), ref = most == -INFINITY ? 0.f : most;
+    sum = sum * exp2_fast(top - ref) + q.y * exp2_fast(q.x - ref);
+    top = most;
+  };
+  if (m < rows) {
+#pragma unroll 4
+    for (int t = warp; t < count; t += kJoinWarps) join(parts[(long long)t * rows + m]);
   }
-  // ref + log2(sum) may cancel: the two are multiplied out before they are added
-  const float l = fmaf(ref, kLn2, logf(sum));
+  mine[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (warp || m >= rows) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) join(mine[w][lane]);
+  const float l = fmaf(top == -INFINITY ? 0.f : top, kLn2, logf(sum));
   const long long label = label_at(labels, label_bytes, m);
   lse[m] = l;
   loss[m] = label >= 0 && label < classes ? l - at[m] : 0.f;
@@ -671,34 +746,47 @@ template <class T, int COLS> struct ScoreGradEnd {
   __device__ __forceinline__ void stop(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
 };
 
-// dz = grad * activation'(pre), rounded; sums of its columns over 32 rows before that
+// dz = grad * activation'(pre), rounded; sums of its columns over 32 rows before that.  32 rows x 256 columns
+// a block, four rows a warp, whose loads are under way together.
 template <class T>
 __global__ void __launch_bounds__(256) tb_act_grad_kernel(const T *grad, long long ld_grad, bool vec_grad, const T *pre, long long ld_pre,
                                                           bool vec_pre, int act, T *dz, long long ld, float *bias_sums, long long rows,
                                                           long long cols) {
-  const int lane = threadIdx.x % 32;
-  const long long c = ((long long)blockIdx.x * 32 + lane) * 8;
-  if (c >= cols) return;
+  __shared__ float part[8][256];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const long long c = ((long long)blockIdx.y * 32 + lane) * 8, r0 = (long long)blockIdx.x * 32 + warp * 4;
   const int have = (int)min(8ll, cols - c);
-  for (long long r0 = ((long long)blockIdx.y * 8 + threadIdx.x / 32) * 32; r0 < rows; r0 += (long long)gridDim.y * 256) {
-    float sum[8] = {};
-    for (long long r = r0; r < rows && r < r0 + 32; ++r) {
-      float g[8], z[8];
-      load8(grad + r * ld_grad + c, g, have, vec_grad);
-      if (act) {
-        load8(pre + r * ld_pre + c, z, have, vec_pre);
+  float g[4][8], z[4][8], sum[8] = {};
+  if (have > 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] *= act_slope(z[i], act);
-      }
-      store8(dz + r * ld + c, g, 8, true); // (ld a multiple of 8)
+    for (int i = 0; i < 4; ++i) load8(grad + (r0 + i) * ld_grad + c, g[i], r0 + i < rows ? have : 0, vec_grad);
+    if (act) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += g[i];
+      for (int i = 0; i < 4; ++i) load8(pre + (r0 + i) * ld_pre + c, z[i], r0 + i < rows ? have : 0, vec_pre);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[i][k] *= act_slope(z[i][k], act);
     }
-    if (bias_sums) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) bias_sums[r0 / 32 * ld + c + i] = sum[i];
+    for (int i = 0; i < 4; ++i) {
+      if (r0 + i >= rows) break;
+      store8(dz + (r0 + i) * ld + c, g[i], 8, true); // (ld a multiple of 8)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += g[i][k];
     }
   }
+  if (!bias_sums) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = sum[k];
+  __syncthreads();
+  const int k = threadIdx.x % 8, l = threadIdx.x / 8; // (neighbouring threads have neighbouring columns)
+  const long long at = ((long long)blockIdx.y * 32 + l) * 8 + k;
+  if (at >= ld) return;
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += part[w][k * 32 + l];
+  bias_sums[blockIdx.x * ld + at] = s;
 }
 
 // out[c] = sum over `count` rows of sums[., c], times 1 / scale: eight warps take every eighth row each
@@ -733,11 +821,20 @@ __global__ void __launch_bounds__(1024) tb_scale_kernel(const float *v, long lon
   *scale = top > 0.f ? ldexpf(1.f, min(max(13 - e, -100), 100)) : 1.f;
 }
 
-// A matrix whose rows do not begin at multiples of 16 bytes, copied to where they do.
+// A matrix whose rows do not begin at multiples of 16 bytes, copied to where they do: 16 bytes a thread.
 template <class T>
 __global__ void __launch_bounds__(256) tb_align_rows_kernel(const T *src, long long ld_src, T *dst, long long ld, long long rows, long long cols) {
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
-    for (long long c = threadIdx.x; c < cols; c += 256) dst[r * ld + c] = src[r * ld_src + c];
+  const long long per = ld / 8, all = rows * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+    const long long r = i / per, c = i % per * 8;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const unsigned short *p = reinterpret_cast<const unsigned short *>(src + r * ld_src + c + 2 * k);
+      w[k] = (c + 2 * k < cols ? __ldg(p) : 0) | (uint32_t)(c + 2 * k + 1 < cols ? __ldg(p + 1) : 0) << 16;
+    }
+    *reinterpret_cast<uint4 *>(dst + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 } // namespace tb

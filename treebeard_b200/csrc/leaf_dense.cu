@@ -1,64 +1,15 @@
-// C ABI of the operators behind a forest's leaves (include/tbk_leaf.h): checks, plans, launches.
+// C ABI of the linear layers and the class loss (include/tbk_leaf.h): plans, launches.
 #include "../../include/tbk_leaf.h"
 #include "dense.cuh"
-#include "last_error.h"
+#include "leaf_api.h"
 
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstring>
-#include <memory>
-#include <new>
 #include <type_traits>
-#include <vector>
-
-#define CUDA_TRY(expr)                                                                                            \
-  do {                                                                                                            \
-    cudaError_t e__ = (expr);                                                                                     \
-    if (e__ != cudaSuccess)                                                                                       \
-      return fail(TBK_ERR_CUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e__), __FILE__, __LINE__);     \
-  } while (0)
-
-using tb::fail;
-
-struct tbk_leaf_map {
-  int device = 0;
-  int64_t rows = 0, max_rows = 0; // table rows in all, of the largest tree
-  tb::LeafMapView view{};
-  void *mem = nullptr;
-};
 
 namespace {
-
-// Makes a device current for a call's launches and puts the old one back.
-struct OnDevice {
-  int before = -1;
-  cudaError_t error;
-  explicit OnDevice(int device) {
-    error = cudaGetDevice(&before);
-    if (error == cudaSuccess && before != device) error = cudaSetDevice(device);
-    else if (error == cudaSuccess) before = -1;
-  }
-  ~OnDevice() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
-
-constexpr int64_t kMost = 0x7ffff000; // of every size: coordinates of tiles behind the last one fit 32 bits
-
-// A workspace cut into 256-byte aligned parts; with a null base only their sizes are added up.
-struct Parts {
-  unsigned char *base;
-  uint64_t used = 0;
-  template <class P> P *take(uint64_t count) {
-    P *p = base ? reinterpret_cast<P *>(base + used) : nullptr;
-    used += (count * sizeof(P) + 255) / 256 * 256;
-    return p;
-  }
-};
-
-int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 
 int half_type(int32_t type, const char *what) {
   if (type == TBK_TYPE_F16 || type == TBK_TYPE_BF16) return TBK_OK;
@@ -66,59 +17,7 @@ int half_type(int32_t type, const char *what) {
   return fail(TBK_ERR_INVALID, "unknown element type %d", type);
 }
 
-int check_sizes(const char *what, int64_t n, int64_t a, int64_t b) {
-  if (n < 0 || a < 1 || b < 1) return fail(TBK_ERR_INVALID, "%s: sizes %lld, %lld, %lld are not >= 0, >= 1, >= 1", what, (long long)n, (long long)a, (long long)b);
-  if (n > kMost || a > kMost || b > kMost) return fail(TBK_ERR_UNSUPPORTED, "%s: a size is above %lld", what, (long long)kMost);
-  return TBK_OK;
-}
-
-int check_matrix(const char *what, const void *p, int64_t ld, int64_t rows, int64_t cols) {
-  if (!p && rows > 0) return fail(TBK_ERR_INVALID, "%s is null", what);
-  if (ld < cols && rows > 1) return fail(TBK_ERR_INVALID, "%s: %lld elements from row to row are less than its %lld columns", what, (long long)ld, (long long)cols);
-  if (ld > ((int64_t)1 << 38)) return fail(TBK_ERR_UNSUPPORTED, "%s: %lld elements from row to row", what, (long long)ld);
-  return TBK_OK;
-}
-
-int check_workspace(const void *p, uint64_t have, uint64_t need) {
-  if (need == 0) return TBK_OK;
-  if (!p || have < need) return fail(TBK_ERR_INVALID, "the workspace has %llu of %llu bytes", (unsigned long long)(p ? have : 0), (unsigned long long)need);
-  if (reinterpret_cast<uintptr_t>(p) % 256) return fail(TBK_ERR_INVALID, "the workspace is not 256-byte aligned");
-  return TBK_OK;
-}
-
-#define TRY(expr)               \
-  do {                          \
-    const int rc__ = (expr);    \
-    if (rc__) return rc__;      \
-  } while (0)
-
-// f(element type, bytes that are moved at a time)
-template <class F> int with_piece(int32_t type, int bytes, F f) {
-  auto sized = [&](auto t) {
-    switch (bytes) {
-    case 16: return f(t, std::integral_constant<int, 16>());
-    case 8: return f(t, std::integral_constant<int, 8>());
-    case 4: return f(t, std::integral_constant<int, 4>());
-    default:
-      if constexpr (sizeof(t) == 2) return f(t, std::integral_constant<int, 2>());
-      else return f(t, std::integral_constant<int, 4>());
-    }
-  };
-  return type == TBK_TYPE_F32 ? sized(float()) : type == TBK_TYPE_F16 ? sized(__half()) : sized(__nv_bfloat16());
-}
 template <class F> int with_half(int32_t type, F f) { return type == TBK_TYPE_F16 ? f(__half()) : f(__nv_bfloat16()); }
-
-int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
-
-// Multiprocessors of a device; the figure of the architecture where there is none (workspace sizes on a host).
-int multiprocessors(int device) {
-  int n = 0;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 2) {
-    cudaGetLastError();
-    return 148;
-  }
-  return n;
-}
 
 // How a product is cut: 256 x 256 tiles of two blocks or 128 x 128 tiles of one, and, where that leaves
 // multiprocessors without work, the sum into parts that a second kernel joins.  Cycles per 64 k of a tile, around
@@ -229,7 +128,7 @@ bool tma_rows(const void *p, int64_t ld, int64_t rows) {
 // The matrix itself, or a copy that tensor copies can read (in `room`, rows x up8(cols)).
 template <class T> int readable(const void **p, int64_t *ld, int64_t rows, int64_t cols, T *room, cudaStream_t stream) {
   if (tma_rows(*p, *ld, rows)) return TBK_OK;
-  tb::tb_align_rows_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 16), 256, 0, stream>>>((const T *)*p, *ld, room, up8(cols), rows, cols);
+  tb::tb_align_rows_kernel<T><<<(unsigned)std::min<int64_t>(tiles_of(rows * (up8(cols) / 8), 256), 1 << 16), 256, 0, stream>>>((const T *)*p, *ld, room, up8(cols), rows, cols);
   CUDA_TRY(cudaGetLastError());
   *p = room;
   *ld = up8(cols);
@@ -301,230 +200,9 @@ struct LossGradParts {
   }
 };
 
-// The largest power of two, 16 at most, that divides the addresses and lengths of all rows of two matrices.
-int piece_bytes(int32_t type, int64_t width, const void *p, int64_t ld_p, int64_t rows_p, const void *q, int64_t ld_q, int64_t rows_q) {
-  const uint64_t size = type == TBK_TYPE_F32 ? 4 : 2;
-  const uint64_t all = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | width * size | (rows_p > 1 ? ld_p * size : 0) |
-                       (rows_q > 1 ? ld_q * size : 0) | 16;
-  return (int)(all & (~all + 1));
-}
-// Lanes (as a power of two) that share a row, 16 bytes each.
-int lanes_of(int64_t width, int32_t type) {
-  const int64_t wanted = tiles_of(width, type == TBK_TYPE_F32 ? 4 : 8);
-  int log2 = 0;
-  while (log2 < 5 && (1 << log2) < wanted) ++log2;
-  return log2;
-}
-
-// How a leaf sum is cut.  Up to two rows per multiprocessor: a block per row, trees over its lane groups.
-// Above that: blocks of 64 rows per lane group and warp, and ranges of trees (joined afterwards) so that the
-// multiprocessors are evenly filled; a range costs a round trip of its fp32 sums.
-struct LeafSumPlan {
-  bool by_row;
-  int lanes_log2, threads, trees_per_part;
-  unsigned columns, blocks, parts = 1;
-  int64_t ld_parts;
-  LeafSumPlan(int64_t n, int64_t width, int32_t type, int64_t trees, int sms) {
-    const int elems = type == TBK_TYPE_F32 ? 4 : 8;
-    lanes_log2 = lanes_of(width, type);
-    const int lanes = 1 << lanes_log2;
-    columns = (unsigned)tiles_of(width, (int64_t)elems << lanes_log2);
-    ld_parts = tiles_of(width, elems) * elems;
-    by_row = n <= 2 * sms;
-    trees_per_part = (int)trees;
-    if (by_row) {
-      threads = (int)std::clamp<int64_t>(tiles_of(tiles_of(trees, 8) * lanes, 32) * 32, 32, 1024);
-      blocks = (unsigned)n;
-      return;
-    }
-    const int64_t rows_per_warp = (32 / lanes) * tb::kLeafRows;
-    threads = (int)std::min<int64_t>(512, tiles_of(n, rows_per_warp) * 32);
-    blocks = (unsigned)tiles_of(n, threads / 32 * rows_per_warp);
-    const double gather = (double)n * trees * width * (32 / elems) / 8 / 15e6, trip = (double)n * ld_parts * 8 / 4e6; // us
-    double least = 1e300;
-    for (int64_t p = 1; p <= std::min<int64_t>(64, tiles_of(trees, 2 * lanes)); ++p) {
-      const double units = (double)blocks * columns * p, cost = gather * std::ceil(units / sms) * sms / units + (p > 1 ? trip * p + 4 : 0);
-      if (cost < least) least = cost, parts = (unsigned)p;
-    }
-    trees_per_part = (int)tiles_of(tiles_of(trees, parts), lanes) * lanes;
-    parts = (unsigned)tiles_of(trees, trees_per_part);
-  }
-};
-
-struct LeafGradParts {
-  int64_t ld;
-  uint32_t *numbers;
-  float *sums;
-  LeafGradParts(Parts &w, int64_t n, int64_t width, int64_t trees, int64_t rows)
-      : ld(up8(n)), numbers(w.take<uint32_t>(trees * ld)), sums(w.take<float>(n > tb::kLeafChunk ? rows * width : 0)) {}
-};
-
 } // namespace
 
 extern "C" {
-
-int tbk_leaf_map_create(const tbk_forest_arrays *fa, int32_t device, tbk_leaf_map **out) {
-  if (!out) return fail(TBK_ERR_INVALID, "null argument");
-  *out = nullptr;
-  if (!fa || !fa->tree_off || !fa->left) return fail(TBK_ERR_INVALID, "null forest array");
-  if (fa->num_trees < 1) return fail(TBK_ERR_INVALID, "a leaf map needs a tree at least");
-  if (fa->num_trees > 1 << 21) return fail(TBK_ERR_UNSUPPORTED, "more than %d trees", 1 << 21);
-  if (fa->tree_off[0] != 0) return fail(TBK_ERR_INVALID, "tree_off does not begin with 0");
-  for (int64_t t = 0; t < fa->num_trees; ++t)
-    if (fa->tree_off[t + 1] <= fa->tree_off[t] || fa->tree_off[t + 1] - fa->tree_off[t] > kMost) return fail(TBK_ERR_INVALID, "tree %lld has no nodes, or too many", (long long)t);
-  try {
-    std::unique_ptr<tbk_leaf_map> map(new tbk_leaf_map);
-    const int64_t trees = fa->num_trees;
-    std::vector<uint2> words;
-    std::vector<int2> tree((size_t)trees + 1);
-    std::vector<int32_t> row_off((size_t)trees + 1);
-    int64_t rows = 0;
-    for (int64_t t = 0; t < trees; ++t) {
-      const int64_t nodes = fa->tree_off[t + 1] - fa->tree_off[t];
-      const int32_t *left = fa->left + fa->tree_off[t];
-      tree[t] = make_int2((int)words.size(), (int)nodes);
-      row_off[t] = (int32_t)rows;
-      for (int64_t i = 0; i < nodes; i += 32) {
-        uint2 w = make_uint2(0, (uint32_t)rows);
-        for (int64_t k = i; k < std::min(nodes, i + 32); ++k)
-          if (left[k] < 0) w.x |= 1u << (k - i), ++rows;
-        words.push_back(w);
-      }
-      if (rows > kMost || words.size() > (size_t)kMost) return fail(TBK_ERR_UNSUPPORTED, "more than %lld leaves", (long long)kMost);
-      map->max_rows = std::max<int64_t>(map->max_rows, rows - row_off[t]);
-    }
-    tree[trees] = make_int2((int)words.size(), 0);
-    row_off[trees] = (int32_t)rows;
-    map->device = device;
-    map->rows = rows;
-    const size_t a = words.size() * 8, b = tree.size() * 8, c = row_off.size() * 4;
-    std::vector<unsigned char> image(a + b + c);
-    std::memcpy(image.data(), words.data(), a);
-    std::memcpy(image.data() + a, tree.data(), b);
-    std::memcpy(image.data() + a + b, row_off.data(), c);
-    OnDevice on(device);
-    CUDA_TRY(on.error);
-    CUDA_TRY(cudaMalloc(&map->mem, image.size()));
-    unsigned char *p = static_cast<unsigned char *>(map->mem);
-    map->view = {reinterpret_cast<uint2 *>(p), reinterpret_cast<int2 *>(p + a), reinterpret_cast<int32_t *>(p + a + b), trees};
-    const cudaError_t e = cudaMemcpy(p, image.data(), image.size(), cudaMemcpyHostToDevice);
-    if (e != cudaSuccess) {
-      cudaFree(map->mem);
-      return fail(TBK_ERR_CUDA, "upload of the leaf map failed: %s", cudaGetErrorString(e));
-    }
-    *out = map.release();
-    return TBK_OK;
-  } catch (const std::bad_alloc &) {
-    return fail(TBK_ERR_INVALID, "out of host memory");
-  }
-}
-
-int tbk_leaf_map_free(tbk_leaf_map *map) {
-  if (!map) return TBK_OK;
-  OnDevice on(map->device);
-  if (on.error == cudaSuccess) cudaFree(map->mem);
-  delete map;
-  return TBK_OK;
-}
-
-int64_t tbk_leaf_map_rows(const tbk_leaf_map *map) { return map ? map->rows : -1; }
-
-static int check_leaf_call(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, int64_t width, int32_t type) {
-  if (!map) return fail(TBK_ERR_INVALID, "null leaf map");
-  TRY(check_sizes("leaf sum", n, width, 1));
-  if (type != TBK_TYPE_F32 && type != TBK_TYPE_F16 && type != TBK_TYPE_BF16) return fail(TBK_ERR_INVALID, "unknown element type %d", type);
-  return check_matrix("leaf_ids", ids, ld_ids, n, map->view.num_trees);
-}
-
-int tbk_leaf_sum_workspace(const tbk_leaf_map *map, int64_t n, int64_t width, int32_t type, uint64_t *bytes) {
-  if (!map || !bytes) return fail(TBK_ERR_INVALID, "null argument");
-  TRY(check_sizes("leaf sum", n, width, 1));
-  const LeafSumPlan plan(n, width, type, map->view.num_trees, multiprocessors(map->device));
-  *bytes = plan.parts > 1 ? (uint64_t)plan.parts * n * plan.ld_parts * 4 : 0;
-  return TBK_OK;
-}
-
-int tbk_leaf_sum(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, const void *table, int64_t ld_table,
-                 int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream_) {
-  TRY(check_leaf_call(map, ids, n, ld_ids, width, type));
-  TRY(check_matrix("table", table, ld_table, map->rows, width));
-  TRY(check_matrix("out", out, ld_out, n, width));
-  if (n == 0) return TBK_OK;
-  uint64_t need = 0;
-  TRY(tbk_leaf_sum_workspace(map, n, width, type, &need));
-  TRY(check_workspace(ws, ws_bytes, need));
-  OnDevice on(map->device);
-  CUDA_TRY(on.error);
-  cudaStream_t stream = (cudaStream_t)stream_;
-  const LeafSumPlan plan(n, width, type, map->view.num_trees, multiprocessors(map->device));
-  return with_piece(type, piece_bytes(type, width, table, ld_table, map->rows, out, ld_out, n), [&](auto t, auto v) {
-    using T = decltype(t);
-    constexpr int V = decltype(v)::value;
-    if (plan.by_row) {
-      tb::tb_leaf_sum_row_kernel<T, V><<<dim3((unsigned)n, plan.columns), plan.threads, 0, stream>>>(map->view, ids, ld_ids, (const T *)table, ld_table,
-                                                                                                     width, plan.lanes_log2, (T *)out, ld_out);
-      CUDA_TRY(cudaGetLastError());
-      return (int)TBK_OK;
-    }
-    float *parts = plan.parts > 1 ? (float *)ws : nullptr;
-    tb::tb_leaf_sum_kernel<T, V><<<dim3(plan.blocks, plan.columns, plan.parts), plan.threads, 0, stream>>>(
-        map->view, ids, ld_ids, (const T *)table, ld_table, width, plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, n, plan.trees_per_part);
-    CUDA_TRY(cudaGetLastError());
-    if (parts) {
-      const int64_t threads = n * plan.ld_parts / tb::Share<T, V>::kElems;
-      tb::tb_leaf_sum_join_kernel<T, V><<<(unsigned)tiles_of(threads, 256), 256, 0, stream>>>(parts, plan.ld_parts, plan.parts, (T *)out, ld_out, width, n);
-      CUDA_TRY(cudaGetLastError());
-    }
-    return (int)TBK_OK;
-  });
-}
-
-int tbk_leaf_sum_backward_workspace(const tbk_leaf_map *map, int64_t n, int64_t width, int32_t type, uint64_t *bytes) {
-  if (!map || !bytes) return fail(TBK_ERR_INVALID, "null argument");
-  (void)type;
-  TRY(check_sizes("leaf sum", n, width, 1));
-  Parts w{nullptr};
-  LeafGradParts parts(w, n, width, map->view.num_trees, map->rows);
-  *bytes = w.used;
-  return TBK_OK;
-}
-
-int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, const void *grad, int64_t ld_grad,
-                          int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream_) {
-  TRY(check_leaf_call(map, ids, n, ld_ids, width, type));
-  TRY(check_matrix("grad", grad, ld_grad, n, width));
-  TRY(check_matrix("out", out, ld_out, map->rows, width));
-  uint64_t need = 0;
-  TRY(tbk_leaf_sum_backward_workspace(map, n, width, type, &need));
-  OnDevice on(map->device);
-  CUDA_TRY(on.error);
-  cudaStream_t stream = (cudaStream_t)stream_;
-  const size_t size = type == TBK_TYPE_F32 ? 4 : 2;
-  if (n == 0) {
-    CUDA_TRY(cudaMemset2DAsync(out, (size_t)ld_out * size, 0, (size_t)width * size, (size_t)map->rows, stream));
-    return TBK_OK;
-  }
-  TRY(check_workspace(ws, ws_bytes, need));
-  Parts w{(unsigned char *)ws};
-  const int64_t trees = map->view.num_trees;
-  LeafGradParts parts(w, n, width, trees, map->rows);
-  tb::tb_leaf_numbers_kernel<<<dim3((unsigned)std::min<int64_t>(tiles_of(n, 32), 4096), (unsigned)tiles_of(trees, 32)), 256, 0, stream>>>(map->view, ids, ld_ids, parts.numbers, parts.ld, n);
-  CUDA_TRY(cudaGetLastError());
-  return with_piece(type, piece_bytes(type, width, grad, ld_grad, n, out, ld_out, map->rows), [&](auto t, auto v) {
-    using T = decltype(t);
-    constexpr int V = decltype(v)::value;
-    const auto kernel = tb::tb_leaf_grad_kernel<T, V>;
-    const int lanes_log2 = lanes_of(width, type), range = (int)std::min<int64_t>(map->max_rows, tb::kLeafRange);
-    const int chunk = (int)std::min<int64_t>(n, tb::kLeafChunk), smem = tb::leaf_grad_smem(chunk, range);
-    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tb::leaf_grad_smem(tb::kLeafChunk, tb::kLeafRange)));
-    const dim3 grid((unsigned)trees, (unsigned)tiles_of(width, (16 / size) << lanes_log2), (unsigned)tiles_of(map->max_rows, range));
-    if (grid.y > 65535 || grid.z > 65535) return fail(TBK_ERR_UNSUPPORTED, "leaf_sum_backward: too many columns or leaves of a tree");
-    kernel<<<grid, 32 * tb::kLeafGradWarps, smem, stream>>>(map->view, parts.numbers, parts.ld, (const T *)grad, ld_grad, width, lanes_log2, parts.sums,
-                                                            (T *)out, ld_out, n, chunk, range);
-    CUDA_TRY(cudaGetLastError());
-    return (int)TBK_OK;
-  });
-}
 
 int tbk_linear_workspace(int64_t n, int64_t inputs, int64_t outputs, int32_t type, int32_t aligned, int32_t device, uint64_t *bytes) {
   if (!bytes) return fail(TBK_ERR_INVALID, "null argument");
@@ -597,6 +275,7 @@ int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_
   if (skip) TRY(check_matrix("skip", skip, ld_skip, n, inputs));
   if (grad_x) TRY(check_matrix("grad_x", grad_x, ld_gx, n, inputs));
   if (grad_w) TRY(check_matrix("grad_weight", grad_w, ld_gw, outputs, inputs));
+  if (outputs > 1 << 24) return fail(TBK_ERR_UNSUPPORTED, "linear_backward: %lld outputs", (long long)outputs);
   if (n > 0) TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(device);
   CUDA_TRY(on.error);
@@ -613,7 +292,7 @@ int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_
     T *dz = (T *)parts.dz;
     if (grad_w) TRY(readable(&x, &ld_x, n, inputs, (T *)parts.x, stream));
     if (grad_x) TRY(readable(&weight, &ld_w, outputs, inputs, (T *)parts.weight, stream));
-    tb::tb_act_grad_kernel<T><<<dim3((unsigned)tiles_of(outputs, 256), (unsigned)std::min<int64_t>(tiles_of(n, 256), 65535)), 256, 0, stream>>>(
+    tb::tb_act_grad_kernel<T><<<dim3((unsigned)tiles_of(n, 32), (unsigned)tiles_of(outputs, 256)), 256, 0, stream>>>(
         (const T *)grad, ld_grad, vec_rows(grad, ld_grad), (const T *)pre, ld_pre, vec_rows(pre, ld_pre), act, dz, parts.ld,
         grad_b ? parts.bias_sums : nullptr, n, outputs);
     CUDA_TRY(cudaGetLastError());
@@ -679,7 +358,7 @@ int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_w
       const tb::LseEnd<T, 64> end{(const T *)bias, labels, label_bytes, parts.part, parts.at};
       TRY((launch_dense<T, false>(a, b, n, classes, width, 1, parts.cut.run, sms, end, stream)));
     }
-    tb::tb_loss_join_kernel<<<(unsigned)tiles_of(n, 128), 128, 0, stream>>>(parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss, lse, n);
+    tb::tb_loss_join_kernel<<<(unsigned)tiles_of(n, 32), 32 * tb::kJoinWarps, 0, stream>>>(parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss, lse, n);
     CUDA_TRY(cudaGetLastError());
     return (int)TBK_OK;
   });

@@ -7,10 +7,10 @@
 // in registers; nothing of that size goes to memory.  Sums are fp32 in an order that the sizes alone decide,
 // rounded once.
 #pragma once
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
+#include "element.cuh"
+
 #include <cstdint>
+#include <type_traits>
 
 namespace tb {
 
@@ -24,14 +24,6 @@ struct LeafMapView {
   long long num_trees;
 };
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 // Table row of node `id` of a tree; -1: the id is no leaf of it.
 __device__ __forceinline__ int32_t leaf_row(const uint2 *words, int2 tree, int32_t id) {
   if ((uint32_t)id >= (uint32_t)tree.y) return -1;
@@ -41,59 +33,93 @@ __device__ __forceinline__ int32_t leaf_row(const uint2 *words, int2 tree, int32
 }
 
 // A lane's share of a row: 16 bytes' worth of columns, moved V bytes at a time (V divides the rows' addresses
-// and lengths, so that a piece is inside a row or outside of it as a whole).
+// and lengths, so that a piece is inside a row or outside of it as a whole).  Sums are kept as pairs, which the
+// multiprocessor adds two at a time.
 template <class T, int V> struct Share {
-  static constexpr int kElems = 16 / sizeof(T), kPieces = 16 / V, kPer = V / sizeof(T);
-  // columns c .. c + kElems - 1 of the row at p; those from `width` on are zeros
-  static __device__ __forceinline__ uint4 load(const T *p, long long c, long long width) {
+  static constexpr int kElems = 16 / sizeof(T), kPairs = kElems / 2, kPieces = 16 / V, kPer = V / sizeof(T);
+  // the columns of the row at p that begin with column c (p points there); those from `width` on are zeros
+  static __device__ __forceinline__ uint4 load(const unsigned char *p, long long c, long long width) {
     uint4 q = make_uint4(0, 0, 0, 0);
-    unsigned char *to = reinterpret_cast<unsigned char *>(&q);
-    const unsigned char *from = reinterpret_cast<const unsigned char *>(p + c);
+    if constexpr (V == 16) {
+      if (c < width) q = __ldg(reinterpret_cast<const uint4 *>(p));
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      if (c + i * kPer < width) {
-        if constexpr (V == 16) q = __ldg(reinterpret_cast<const uint4 *>(from));
-        else if constexpr (V == 8) *reinterpret_cast<uint2 *>(to + 8 * i) = __ldg(reinterpret_cast<const uint2 *>(from) + i);
-        else if constexpr (V == 4) *reinterpret_cast<uint32_t *>(to + 4 * i) = __ldg(reinterpret_cast<const uint32_t *>(from) + i);
-        else *reinterpret_cast<uint16_t *>(to + 2 * i) = __ldg(reinterpret_cast<const uint16_t *>(from) + i);
-      }
+      for (int i = 0; i < kPieces; ++i)
+        if (c + i * kPer < width) {
+          if constexpr (V == 8) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+            w[2 * i] = x.x, w[2 * i + 1] = x.y;
+          } else if constexpr (V == 4) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
+          else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + i) << (i % 2 * 16);
+        }
+      q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
     return q;
   }
-  static __device__ __forceinline__ void add(float (&acc)[kElems], uint4 q) {
-    const T *v = reinterpret_cast<const T *>(&q);
-#pragma unroll
-    for (int i = 0; i < kElems; ++i) acc[i] += to_float(v[i]);
+  static __device__ __forceinline__ float2 pair(uint32_t w) { // (of a 16-bit type)
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
-  static __device__ __forceinline__ void store(T *p, long long c, long long width, const float (&acc)[kElems]) {
-    uint4 q;
-    T *v = reinterpret_cast<T *>(&q);
+  static __device__ __forceinline__ void add(unsigned long long &acc, float2 v) {
+    asm("{\n .reg .b64 t;\n mov.b64 t, {%1, %2};\n add.rn.f32x2 %0, %0, t;\n}" : "+l"(acc) : "f"(v.x), "f"(v.y));
+  }
+  static __device__ __forceinline__ void add(unsigned long long (&acc)[kPairs], uint4 q) {
+    if constexpr (sizeof(T) == 4) {
+      add(acc[0], make_float2(__uint_as_float(q.x), __uint_as_float(q.y)));
+      add(acc[1], make_float2(__uint_as_float(q.z), __uint_as_float(q.w)));
+    } else {
+      add(acc[0], pair(q.x));
+      add(acc[1], pair(q.y));
+      add(acc[2], pair(q.z));
+      add(acc[3], pair(q.w));
+    }
+  }
+  static __device__ __forceinline__ float2 get(unsigned long long a) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(a));
+    return v;
+  }
+  // p: the row's column c
+  static __device__ __forceinline__ void store(T *p, long long c, long long width, const unsigned long long (&acc)[kPairs]) {
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) v[i] = from_float<T>(acc[i]);
-    const unsigned char *from = reinterpret_cast<const unsigned char *>(&q);
-    unsigned char *to = reinterpret_cast<unsigned char *>(p + c);
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 v = get(acc[i]);
+      if constexpr (sizeof(T) == 4) w[2 * i] = __float_as_uint(v.x), w[2 * i + 1] = __float_as_uint(v.y);
+      else {
+        const T h[2] = {from_float<T>(v.x), from_float<T>(v.y)};
+        w[i] = *reinterpret_cast<const uint32_t *>(h);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
       if (c + i * kPer < width) {
-        if constexpr (V == 16) *reinterpret_cast<uint4 *>(to) = q;
-        else if constexpr (V == 8) reinterpret_cast<uint2 *>(to)[i] = *reinterpret_cast<const uint2 *>(from + 8 * i);
-        else if constexpr (V == 4) reinterpret_cast<uint32_t *>(to)[i] = *reinterpret_cast<const uint32_t *>(from + 4 * i);
-        else reinterpret_cast<uint16_t *>(to)[i] = *reinterpret_cast<const uint16_t *>(from + 2 * i);
+        if constexpr (V == 16) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (V == 8) reinterpret_cast<uint2 *>(p)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+        else if constexpr (V == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+        else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
       }
   }
 };
 
-// ---- few batch rows: a block per row, whose lanes' groups share the trees out ---------------------
-// One chain of three loads (id, words, table row) per 8 trees of a group; latency is all that counts.
+// ---- few batch rows: a cluster of blocks per row, whose lane groups share the trees out ------------
+// One chain of three loads (id, word, table row) per eight trees of a group: latency is all that counts, and
+// as many misses as possible are under way at a time.  The blocks' sums meet in the first one's registers.
+constexpr int kLeafRowThreads = 256;
 template <class T, int V>
-__global__ void __launch_bounds__(1024) tb_leaf_sum_row_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, const T *table, long long ld_table,
-                                                               long long width, int lanes_log2, T *out, long long ld_out) {
+__global__ void __launch_bounds__(kLeafRowThreads) tb_leaf_sum_row_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, const T *table,
+                                                                          uint32_t row_bytes, long long width, int lanes_log2, T *out,
+                                                                          long long ld_out, int blocks) {
   using S = Share<T, V>;
-  constexpr int E = S::kElems;
-  __shared__ float part[32 * 32 * E]; // [warp][lane of a row][element], column lanes_log2 == 5 at most
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2, groups = blockDim.x >> lanes_log2;
-  const long long n = blockIdx.x, c = ((long long)blockIdx.y * lanes + lane) * E;
+  constexpr int P = S::kPairs, kWarps = kLeafRowThreads / 32;
+  __shared__ unsigned long long part[kWarps][32][P]; // [0]: the block's sum in the end
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), rank = blockIdx.x % blocks;
+  const int group = rank * (kLeafRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2), groups = blocks * (kLeafRowThreads >> lanes_log2);
+  const long long n = blockIdx.x / blocks, c = ((long long)blockIdx.y * lanes + lane) * S::kElems;
   const int32_t *id = ids + n * ld_ids;
-  float acc[E] = {};
+  const unsigned char *from = reinterpret_cast<const unsigned char *>(table + c);
+  unsigned long long acc[P] = {};
   for (long long t0 = 0; t0 < m.num_trees; t0 += (long long)groups * 8) {
     int32_t r[8];
 #pragma unroll
@@ -103,123 +129,184 @@ __global__ void __launch_bounds__(1024) tb_leaf_sum_row_kernel(LeafMapView m, co
     }
     uint4 q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = r[i] >= 0 ? S::load(table + r[i] * ld_table, c, width) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 8; ++i) q[i] = r[i] >= 0 ? S::load(from + (unsigned long long)r[i] * row_bytes, c, width) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (r[i] >= 0) S::add(acc, q[i]);
   }
   for (int d = lanes; d < 32; d <<= 1)
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] += __shfl_xor_sync(~0u, acc[i], d);
-  const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    for (int i = 0; i < P; ++i) S::add(acc[i], S::get(__shfl_xor_sync(~0u, acc[i], d)));
+  const int warp = threadIdx.x / 32;
   if ((threadIdx.x & 31) < lanes)
 #pragma unroll
-    for (int i = 0; i < E; ++i) part[(warp * 32 + lane) * E + i] = acc[i];
+    for (int i = 0; i < P; ++i) part[warp][lane][i] = acc[i];
   __syncthreads();
-  if (threadIdx.x >= lanes) return;
-  for (int w = 1; w < warps; ++w)
+  if (threadIdx.x < lanes) {
+    for (int w = 1; w < kWarps; ++w)
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] += part[(w * 32 + lane) * E + i];
-  S::store(out + n * ld_out, c, width, acc);
+      for (int i = 0; i < P; ++i) S::add(acc[i], S::get(part[w][lane][i]));
+#pragma unroll
+    for (int i = 0; i < P; ++i) part[0][lane][i] = acc[i];
+  }
+  if (blocks > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && threadIdx.x < lanes) {
+      const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&part[0][lane][0]);
+      for (int b = 1; b < blocks; ++b) {
+        uint32_t theirs;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(theirs) : "r"(mine), "r"(b));
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          unsigned long long v;
+          asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(theirs + 8 * i) : "memory");
+          S::add(acc[i], S::get(v));
+        }
+      }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // (the others' memory has been read)
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (rank == 0 && threadIdx.x < lanes) S::store(out + n * ld_out + c, c, width, acc);
 }
 
 // ---- many batch rows: a lane group keeps the sums of eight rows -----------------------------------
 // All rows of a block go through the trees side by side, so that the rows of one tree's table, of which most
 // batch rows want the same few, are read from L1 once they have come; eight loads of a lane are in flight.
-// blockIdx.y: columns; blockIdx.z: a range of trees, whose sums are kept in fp32 for tb_leaf_sum_join_kernel.
+// The work -- row tiles times batches of trees, in that order -- is dealt out evenly: a block takes a stretch
+// of it, which may end one tile and begin the next.  A tile that one block has as a whole is finished there,
+// the parts of the others are kept in fp32 for tb_leaf_sum_join_kernel.
 constexpr int kLeafRows = 8;
+struct LeafStretch {
+  long long tiles, batches, blocks; // of the whole; a tile's batches of trees
+  __host__ __device__ long long begin(long long block) const { return block * (tiles * batches) / blocks; }
+  __host__ __device__ long long block_of(long long unit) const { // the block that has this unit
+    long long b = unit * blocks / (tiles * batches);
+    while (b + 1 < blocks && begin(b + 1) <= unit) ++b;
+    while (b > 0 && begin(b) > unit) --b;
+    return b;
+  }
+};
 template <class T, int V>
-__global__ void __launch_bounds__(512) tb_leaf_sum_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, const T *table, long long ld_table,
-                                                          long long width, int lanes_log2, T *out, long long ld_out, float *parts, long long ld_parts,
-                                                          long long n_rows, int trees_per_part) {
+__global__ void __launch_bounds__(512, 1) tb_leaf_sum_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, const T *table, uint32_t row_bytes,
+                                                             long long width, int lanes_log2, T *out, long long ld_out, float *parts, long long ld_parts,
+                                                             long long n_rows, LeafStretch work) {
   using S = Share<T, V>;
-  constexpr int E = S::kElems;
+  constexpr int P = S::kPairs;
   const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), groups = blockDim.x >> lanes_log2;
   const int base = threadIdx.x & 31 & ~(lanes - 1);
-  // (a warp's groups have neighbouring rows, a group's eight rows are `groups` apart)
-  const long long n0 = (long long)blockIdx.x * groups * kLeafRows + (threadIdx.x >> lanes_log2), c = ((long long)blockIdx.y * lanes + lane) * E;
-  const long long t_end = min(m.num_trees, (long long)(blockIdx.z + 1) * trees_per_part);
-  float acc[kLeafRows][E] = {};
-  for (long long t0 = (long long)blockIdx.z * trees_per_part; t0 < t_end; t0 += lanes) {
-    // every lane looks up one tree of the next `lanes`
-    const long long t = t0 + lane;
-    const bool there = t < t_end;
-    const int2 tree = there ? __ldg(m.trees + t) : make_int2(0, 0);
-    int32_t id[kLeafRows], row[kLeafRows];
+  const long long c = ((long long)blockIdx.y * lanes + lane) * S::kElems;
+  const unsigned char *from = reinterpret_cast<const unsigned char *>(table + c);
+  long long u = work.begin(blockIdx.x);
+  const long long u_end = work.begin(blockIdx.x + 1);
+  while (u < u_end) {
+    const long long tile = u / work.batches, b0 = u % work.batches, b1 = min(work.batches, b0 + (u_end - u));
+    // (a warp's groups have neighbouring rows, a group's eight rows are `groups` apart)
+    const long long n0 = tile * groups * kLeafRows + (threadIdx.x >> lanes_log2);
+    const int32_t *id_at[kLeafRows];
+#pragma unroll
+    for (int i = 0; i < kLeafRows; ++i) id_at[i] = ids + min(n0 + (long long)i * groups, n_rows - 1) * ld_ids; // (what is behind the last row is not kept)
+    unsigned long long acc[kLeafRows][P] = {};
+    for (long long b = b0; b < b1; ++b) {
+      // every lane looks up one tree of the batch
+      const long long t = b * lanes + lane;
+      const bool there = t < m.num_trees;
+      const int2 tree = there ? __ldg(m.trees + t) : make_int2(0, 0);
+      int32_t row[kLeafRows];
+#pragma unroll
+      for (int i = 0; i < kLeafRows; ++i) row[i] = there ? __ldg(id_at[i] + t) : -1;
+      bool all = true;
+#pragma unroll
+      for (int i = 0; i < kLeafRows; ++i) {
+        row[i] = leaf_row(m.words, tree, row[i]);
+        all &= row[i] >= 0;
+      }
+      if (__all_sync(~0u, all)) {
+        for (int j = 0; j < lanes; ++j) {
+          uint4 q[kLeafRows];
+#pragma unroll
+          for (int i = 0; i < kLeafRows; ++i) q[i] = S::load(from + (unsigned long long)(uint32_t)__shfl_sync(~0u, row[i], base + j) * row_bytes, c, width);
+#pragma unroll
+          for (int i = 0; i < kLeafRows; ++i) S::add(acc[i], q[i]);
+        }
+      } else { // (some id is no leaf, or the batch ends behind the last tree)
+        for (int j = 0; j < lanes; ++j)
+#pragma unroll
+          for (int i = 0; i < kLeafRows; ++i) {
+            const int32_t r = __shfl_sync(~0u, row[i], base + j);
+            if (r >= 0) S::add(acc[i], S::load(from + (unsigned long long)(uint32_t)r * row_bytes, c, width));
+          }
+      }
+    }
+    const bool whole = b0 == 0 && b1 == work.batches;
+    const long long part = whole ? 0 : blockIdx.x - work.block_of(tile * work.batches);
 #pragma unroll
     for (int i = 0; i < kLeafRows; ++i) {
       const long long n = n0 + (long long)i * groups;
-      id[i] = there && n < n_rows ? __ldg(ids + n * ld_ids + t) : -1;
-    }
+      if (n >= n_rows) break;
+      if (whole) {
+        S::store(out + n * ld_out + c, c, width, acc[i]);
+      } else if (c < ld_parts) {
+        unsigned long long *d = reinterpret_cast<unsigned long long *>(parts + (part * n_rows + n) * ld_parts + c);
 #pragma unroll
-    for (int i = 0; i < kLeafRows; ++i) row[i] = leaf_row(m.words, tree, id[i]);
-    const int now = (int)min((long long)lanes, t_end - t0);
-    for (int j = 0; j < now; ++j) {
-      uint4 q[kLeafRows];
-#pragma unroll
-      for (int i = 0; i < kLeafRows; ++i) {
-        const int32_t r = __shfl_sync(~0u, row[i], base + j);
-        q[i] = r >= 0 ? S::load(table + r * ld_table, c, width) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < P; ++k) d[k] = acc[i][k];
       }
-#pragma unroll
-      for (int i = 0; i < kLeafRows; ++i) S::add(acc[i], q[i]);
     }
-  }
-#pragma unroll
-  for (int i = 0; i < kLeafRows; ++i) {
-    const long long n = n0 + (long long)i * groups;
-    if (n >= n_rows) break;
-    if (!parts) {
-      S::store(out + n * ld_out, c, width, acc[i]);
-    } else if (c < ld_parts) {
-      float4 *d = reinterpret_cast<float4 *>(parts + ((long long)blockIdx.z * n_rows + n) * ld_parts + c);
-#pragma unroll
-      for (int k = 0; k < E / 4; ++k) d[k] = make_float4(acc[i][4 * k], acc[i][4 * k + 1], acc[i][4 * k + 2], acc[i][4 * k + 3]);
-    }
+    u += b1 - b0;
   }
 }
-// Adds the parts of the tree ranges up, in order.
+// Adds the parts of the tiles that several blocks had, in order.
 template <class T, int V>
-__global__ void __launch_bounds__(256) tb_leaf_sum_join_kernel(const float *parts, long long ld_parts, int count, T *out, long long ld_out, long long width, long long n_rows) {
+__global__ void __launch_bounds__(256) tb_leaf_sum_join_kernel(const float *parts, long long ld_parts, int tile_rows, T *out, long long ld_out,
+                                                               long long width, long long n_rows, LeafStretch work) {
   using S = Share<T, V>;
-  constexpr int E = S::kElems;
-  const long long per = ld_parts / E, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  constexpr int P = S::kPairs;
+  const long long per = ld_parts / S::kElems, i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n_rows * per) return;
-  const long long n = i / per, c = i % per * E;
-  float acc[E] = {};
-  for (int s = 0; s < count; ++s) {
-    const float4 *d = reinterpret_cast<const float4 *>(parts + ((long long)s * n_rows + n) * ld_parts + c);
+  const long long n = i / per, c = i % per * S::kElems, tile = n / tile_rows;
+  const long long count = work.block_of((tile + 1) * work.batches - 1) - work.block_of(tile * work.batches) + 1;
+  if (count == 1) return;
+  unsigned long long acc[P] = {};
+  for (long long s = 0; s < count; ++s) {
+    const unsigned long long *d = reinterpret_cast<const unsigned long long *>(parts + (s * n_rows + n) * ld_parts + c);
 #pragma unroll
-    for (int k = 0; k < E / 4; ++k) {
-      const float4 v = d[k];
-      acc[4 * k] += v.x, acc[4 * k + 1] += v.y, acc[4 * k + 2] += v.z, acc[4 * k + 3] += v.w;
-    }
+    for (int k = 0; k < P; ++k) S::add(acc[k], S::get(d[k]));
   }
-  S::store(out + n * ld_out, c, width, acc);
+  S::store(out + n * ld_out + c, c, width, acc);
 }
 
 // ---- gradient -------------------------------------------------------------------------------------
 
-constexpr uint32_t kNoLeaf = 0xffffffffu;
-
-// numbers[t][n] = number of the leaf among its tree's (kNoLeaf: none): the ids the other way around, so that
+// numbers[t][n] = number of the leaf among its tree's (all ones: none): the ids the other way around, so that
 // the rows of one tree lie side by side, and looked up with a tree per warp, which touches few lines.
-__global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, uint32_t *numbers, long long ld,
+constexpr int kNumberRows = 128;
+template <class N>
+__global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, N *numbers, long long ld,
                                                               long long n_rows) {
-  __shared__ int32_t tile[32][33];
+  __shared__ int32_t tile[32][kNumberRows + 1];
   const int x = threadIdx.x % 32, y = threadIdx.x / 32;
   const long long t0 = (long long)blockIdx.y * 32;
-  for (long long n0 = (long long)blockIdx.x * 32; n0 < n_rows; n0 += (long long)gridDim.x * 32) {
+  for (long long n0 = (long long)blockIdx.x * kNumberRows; n0 < n_rows; n0 += (long long)gridDim.x * kNumberRows) {
+    __syncthreads();
+    const int32_t *from = ids + n0 * ld_ids + t0 + x;
+    int32_t v[kNumberRows / 8];
+#pragma unroll
+    for (int i = 0; i < kNumberRows / 8; ++i) v[i] = n0 + y + 8 * i < n_rows && t0 + x < m.num_trees ? __ldg(from + (y + 8 * i) * ld_ids) : -1;
+#pragma unroll
+    for (int i = 0; i < kNumberRows / 8; ++i) tile[x][y + 8 * i] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = y; i < 32; i += 8) tile[i][x] = n0 + i < n_rows && t0 + x < m.num_trees ? ids[(n0 + i) * ld_ids + t0 + x] : -1;
-    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+      const long long t = t0 + y * 4 + i;
+      if (t >= m.num_trees) break;
+      const int2 tree = __ldg(m.trees + t);
+      const int32_t first = __ldg(m.rows + t);
 #pragma unroll
-    for (int i = y; i < 32; i += 8) {
-      const long long t = t0 + i;
-      if (t >= m.num_trees || n0 + x >= n_rows) continue;
-      const int32_t r = leaf_row(m.words, __ldg(m.trees + t), tile[x][i]);
-      numbers[t * ld + n0 + x] = r < 0 ? kNoLeaf : (uint32_t)(r - __ldg(m.rows + t));
+      for (int k = 0; k < kNumberRows / 32; ++k) {
+        const int32_t r = leaf_row(m.words, tree, tile[y * 4 + i][x + 32 * k]);
+        if (n0 + x + 32 * k < n_rows) numbers[t * ld + n0 + x + 32 * k] = r < 0 ? (N)~(N)0 : (N)(r - first);
+      }
     }
   }
 }
@@ -230,30 +317,31 @@ __global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, con
 // which add up runs of equal leaves.  A leaf inside one group's stretch is finished there; the ends of
 // stretches are joined in order afterwards.  Batches above kLeafChunk rows come in pieces, with fp32 sums in
 // `sums` in between.
-constexpr int kLeafRange = 1024, kLeafChunk = 32768, kLeafGradWarps = 16;
+constexpr int kLeafRange = 1024, kLeafChunk = 32768, kLeafGradWarps = 8;
 constexpr int kLeafGradFixed = kLeafRange * 4 + 16;
 __host__ __device__ constexpr int leaf_grad_smem(int chunk, int range) { // counters and, after them, the ends of stretches share their place
-  return kLeafGradFixed + (kLeafGradWarps * range * 4 > 16384 ? kLeafGradWarps * range * 4 : 16384) + (chunk + 7) / 8 * 16; // order: two bytes a row
+  return kLeafGradFixed + (kLeafGradWarps * range * 4 > 8192 ? kLeafGradWarps * range * 4 : 8192) + (chunk + 15) / 8 * 16; // order: two bytes a row
 }
-template <class T, int V>
-__global__ void __launch_bounds__(32 * kLeafGradWarps) tb_leaf_grad_kernel(LeafMapView m, const uint32_t *numbers, long long ld_numbers, const T *grad,
-                                                                           long long ld_grad, long long width, int lanes_log2, float *sums, T *out,
-                                                                           long long ld_out, long long n_rows, int chunk, int range) {
+template <class T, int V, class N>
+__global__ void __launch_bounds__(32 * kLeafGradWarps, 3) tb_leaf_grad_kernel(LeafMapView m, const N *numbers, long long ld_numbers, const T *grad,
+                                                                              uint32_t row_bytes, long long width, int lanes_log2, float *sums, T *out,
+                                                                              long long ld_out, long long n_rows, int chunk, int range) {
   using S = Share<T, V>;
-  constexpr int E = S::kElems;
+  constexpr int P = S::kPairs;
+  constexpr uint32_t kNone = (N)~(N)0;
   extern __shared__ __align__(16) unsigned char raw[];
-  uint32_t *start = reinterpret_cast<uint32_t *>(raw);              // [kLeafRange + 1] first place of a leaf
-  uint32_t *count = reinterpret_cast<uint32_t *>(raw + kLeafGradFixed); // [warp][range]
-  float *ends = reinterpret_cast<float *>(count);                   // [group][lanes * E] sum of a stretch's first run
-  uint16_t *order = reinterpret_cast<uint16_t *>(raw + leaf_grad_smem(0, range));
+  uint32_t *start = reinterpret_cast<uint32_t *>(raw);                  // [leaves + 1] first place of a leaf
+  uint32_t *count = reinterpret_cast<uint32_t *>(raw + kLeafGradFixed); // [warp][leaves]
+  unsigned long long *ends = reinterpret_cast<unsigned long long *>(count); // [thread][P] sum of a stretch's first run
+  uint16_t *order = reinterpret_cast<uint16_t *>(raw + leaf_grad_smem(0, range) - 16);
   const int tid = threadIdx.x, warp = tid / 32, wl = tid % 32;
   const int lanes = 1 << lanes_log2, lane = tid & (lanes - 1), group = tid >> lanes_log2, groups = (32 * kLeafGradWarps) >> lanes_log2;
-  const long long t = blockIdx.x, c = ((long long)blockIdx.y * lanes + lane) * E;
+  const long long t = blockIdx.x, c = ((long long)blockIdx.y * lanes + lane) * S::kElems;
   const int32_t row0 = m.rows[t] + (int)blockIdx.z * range;
   const int leaves = min(range, m.rows[t + 1] - row0);
   if (leaves <= 0) return;
   const uint32_t first_leaf = blockIdx.z * (uint32_t)range;
-  const uint32_t *mine = numbers + t * ld_numbers;
+  const N *mine = numbers + t * ld_numbers;
 
   for (long long b0 = 0; b0 < n_rows; b0 += chunk) {
     const int now = (int)min((long long)chunk, n_rows - b0);
@@ -262,9 +350,15 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps) tb_leaf_grad_kernel(LeafM
     __syncthreads();
     for (int i = tid; i < kLeafGradWarps * leaves; i += 32 * kLeafGradWarps) count[i] = 0;
     __syncthreads();
-    for (int i = from + wl; i < to; i += 32) {
-      const uint32_t l = mine[b0 + i] - first_leaf;
-      if (l < (uint32_t)leaves) atomicAdd(&count[warp * leaves + l], 1u);
+    uint32_t *own = count + warp * leaves;
+    constexpr int kAhead = 8; // numbers of a lane that are loaded at a time
+    for (int i0 = from + wl; i0 < to; i0 += 32 * kAhead) {
+      uint32_t l[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) l[k] = i0 + 32 * k < to ? (uint32_t)__ldg(mine + b0 + i0 + 32 * k) : kNone;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (l[k] != kNone && l[k] - first_leaf < (uint32_t)leaves) atomicAdd(own + (l[k] - first_leaf), 1u);
     }
     __syncthreads();
     // places: leaf by leaf, within a leaf warp by warp
@@ -292,23 +386,36 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps) tb_leaf_grad_kernel(LeafM
         before += __shfl_sync(~0u, s, 31);
       }
       if (wl == 0) start[leaves] = before;
+      if (wl < 8) order[before + wl] = 0; // (read, never added)
     }
     __syncthreads();
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const int i = i0 + wl;
-      const uint32_t l = i < to ? mine[b0 + i] - first_leaf : kNoLeaf;
-      const uint32_t same = __match_any_sync(~0u, l);
-      if (l < (uint32_t)leaves) {
-        const uint32_t at = count[warp * leaves + l], rank = __popc(same & ((1u << wl) - 1));
-        order[start[l] + at + rank] = (uint16_t)i;
-        __syncwarp(same);
-        if (rank == 0) count[warp * leaves + l] = at + __popc(same);
+    for (int l = tid; l < leaves; l += 32 * kLeafGradWarps)
+#pragma unroll
+      for (int w = 0; w < kLeafGradWarps; ++w) count[w * leaves + l] += start[l];
+    __syncthreads();
+    for (int i0 = from; i0 < to; i0 += 32 * kAhead) {
+      uint32_t ls[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) ls[k] = i0 + 32 * k + wl < to ? (uint32_t)__ldg(mine + b0 + i0 + 32 * k + wl) : kNone;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (i0 + 32 * k >= to) break;
+        const uint32_t l = ls[k] == kNone || ls[k] - first_leaf >= (uint32_t)leaves ? kNone : ls[k] - first_leaf;
+        const uint32_t same = __match_any_sync(~0u, l);
+        const uint32_t rank = __popc(same & ((1u << wl) - 1));
+        uint32_t at = 0;
+        if (l != kNone) at = own[l];
+        __syncwarp();
+        if (l != kNone) {
+          order[at + rank] = (uint16_t)(i0 + 32 * k + wl);
+          if (rank == 0) own[l] = at + __popc(same);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     __syncthreads();
 
-    const int total = (int)start[leaves], piece = (total + groups - 1) / groups;
+    const int total = (int)start[leaves], piece = ((total + groups - 1) / groups + 7) & ~7;
     const int a = min(total, group * piece), z = min(total, a + piece);
     // the leaf that the place `a` belongs to: the last one that starts at or before it and is not empty
     int l = 0;
@@ -321,32 +428,41 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps) tb_leaf_grad_kernel(LeafM
       }
       l = lo;
     }
-    auto finish = [&](int leaf, float (&acc)[E]) {
+    auto finish = [&](int leaf, unsigned long long (&acc)[P]) {
       const long long r = row0 + leaf;
       float *s = sums + r * width + c;
       if (!first) {
 #pragma unroll
-        for (int k = 0; k < E; ++k)
-          if (c + k < width) acc[k] += s[k];
+        for (int k = 0; k < P; ++k) S::add(acc[k], make_float2(c + 2 * k < width ? s[2 * k] : 0.f, c + 2 * k + 1 < width ? s[2 * k + 1] : 0.f));
       }
-      if (last) S::store(out + r * ld_out, c, width, acc);
+      if (last) S::store(out + r * ld_out + c, c, width, acc);
       else {
 #pragma unroll
-        for (int k = 0; k < E; ++k)
-          if (c + k < width) s[k] = acc[k];
+        for (int k = 0; k < P; ++k) {
+          const float2 v = S::get(acc[k]);
+          if (c + 2 * k < width) s[2 * k] = v.x;
+          if (c + 2 * k + 1 < width) s[2 * k + 1] = v.y;
+        }
       }
     };
-    float acc[E] = {};
+    unsigned long long acc[P] = {};
     bool whole = a < z && start[l] == (uint32_t)a; // the run at hand began in this stretch
     bool open = false;                            // the stretch's last run goes on in the next one
-    float *end0 = ends + (size_t)tid * E;
+    unsigned long long *end0 = ends + tid * P;
     if (a < z) {
       int stop = (int)start[l + 1];
-      const T *g0 = grad + b0 * ld_grad;
+      const unsigned char *g0 = reinterpret_cast<const unsigned char *>(grad + c) + (unsigned long long)b0 * row_bytes;
       for (int i = a; i < z; i += 8) {
+        const uint4 o = *reinterpret_cast<const uint4 *>(order + i);
+        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
         uint4 q[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = i + k < z ? S::load(g0 + (long long)order[i + k] * ld_grad, c, width) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < 8; ++k) q[k] = S::load(g0 + (unsigned long long)(k % 2 ? ow[k / 2] >> 16 : ow[k / 2] & 0xffffu) * row_bytes, c, width);
+        if (stop >= i + 8 && z >= i + 8) { // (one run)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) S::add(acc, q[k]);
+          continue;
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           if (i + k >= z) break;
@@ -354,9 +470,9 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps) tb_leaf_grad_kernel(LeafM
             if (whole) finish(l, acc);
             else
 #pragma unroll
-              for (int e = 0; e < E; ++e) end0[e] = acc[e];
+              for (int e = 0; e < P; ++e) end0[e] = acc[e];
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = 0.f;
+            for (int e = 0; e < P; ++e) acc[e] = 0;
             whole = true;
             do ++l; while ((int)start[l + 1] <= i + k);
             stop = (int)start[l + 1];
@@ -367,22 +483,22 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps) tb_leaf_grad_kernel(LeafM
       open = stop > z;
       if (!whole)
 #pragma unroll
-        for (int e = 0; e < E; ++e) end0[e] = acc[e];
+        for (int e = 0; e < P; ++e) end0[e] = acc[e];
       else if (!open) finish(l, acc);
     }
     __syncthreads();
     if (a < z && open && whole) { // a leaf that begins here and ends in a later stretch: its parts in order
       const int stop = (int)start[l + 1];
       for (int g = group + 1; g * piece < stop; ++g) {
-        const float *e0 = ends + ((size_t)g * lanes + lane) * E;
+        const unsigned long long *e0 = ends + ((g << lanes_log2) + lane) * P;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += e0[e];
+        for (int e = 0; e < P; ++e) S::add(acc[e], S::get(e0[e]));
       }
       finish(l, acc);
     }
     for (int leaf = group; leaf < leaves; leaf += groups) // leaves without a row
       if (start[leaf + 1] == start[leaf] && (first || last)) {
-        float none[E] = {};
+        unsigned long long none[P] = {};
         finish(leaf, none);
       }
   }
