@@ -4,38 +4,57 @@
 // Either operand may lie with k or with its rows one behind the other in memory (the products of the
 // backward passes sum over rows): the tensor map's box and the shared-memory descriptor differ, nothing is
 // transposed.  A block has one warp that issues the tensor copies, one that issues the matrix instructions
-// and eight that take finished tiles out of tensor memory; two accumulators, so that a tile is taken out
-// while the next one is computed.  Blocks are persistent and walk over units: a row tile, a run of column
-// tiles, a part of the sum.
+// and sixteen that take finished sums out of tensor memory and, through shared memory, on their way (a chunk of
+// theirs is one chain of short steps, so that eight warps took twice as long as sixteen).  Blocks are
+// persistent and walk over units: a row tile, a run of column tiles, a part of the sum.
 //
-//   PAIR: two blocks of a cluster on one 256 x 256 tile; each brings 128 rows of A and 128 of B, so a stage
-//         of 64 k costs an SM 32 KB of L2 traffic for 512 cycles of matrix work (48 KB for one block's 128 x 256).
-//   else: one block, 128 x 128 tiles, for products with few tiles.
+// Three shapes (kernel template SHAPE).  What bounds them is shared memory: 128 bytes a cycle are written by the
+// tensor copies and read by the matrix unit.  With 64 k at a time, bytes written + read per cycle of matrix work:
+//   kDenseTall  two blocks on 512 x 256 results, 256 rows of A and 128 of B each: 48 + 64.  Both accumulators,
+//               128 x 256 a block, belong to one tile; so that one is taken out while the other is still computed,
+//               the first runs ahead of the second by up to three stages at a tile's beginning and two at its end.
+//   kDensePair  two blocks on 256 x 256 results, 128 rows of each operand: 64 + 64, measured at three quarters of
+//               the tall one's rate; two tiles' accumulators, one taken out while the other is computed.
+//   kDenseOne   one block on 128 x 128 results, for products with few tiles: 128 + 128, half the rate.
 //
 // All waits are bounded: one that gives up ends the launch with a word in tb_dense_status.
 #pragma once
 #include <cuda.h>
 #include <cstdint>
+#include <type_traits>
 #include "element.cuh"
 
 namespace tb {
 
-constexpr int kDenseThreads = 384, kDenseEndWarps = 8, kDenseK = 64;
-constexpr int kDenseStageBytes = 32768, kDenseStages = 6; // 128 rows of A and 128 of B, 64 k each
-constexpr int kDenseEndBytes = 4096;                      // a finishing warp's own shared memory
-constexpr int kDenseSmem = 1024 + kDenseStages * kDenseStageBytes + kDenseEndWarps * kDenseEndBytes + 256;
+constexpr int kDenseEndWarps = 16, kDenseThreads = 128 + 32 * kDenseEndWarps, kDenseK = 64;
+enum DenseShape { kDenseOne = 0, kDensePair = 1, kDenseTall = 2 };
+constexpr int kDenseEndBytes = 4096, kDenseBiasBytes = 256; // a finishing warp's own shared memory
+__host__ __device__ constexpr int dense_rows(int shape) { return shape == kDenseTall ? 512 : shape == kDensePair ? 256 : 128; }
+__host__ __device__ constexpr int dense_cols(int shape) { return shape == kDenseOne ? 128 : 256; }
+__host__ __device__ constexpr int dense_stages(int shape) { return shape == kDenseTall ? 3 : 4; }
+__host__ __device__ constexpr int dense_stage_bytes(int shape) { return shape == kDenseTall ? 49152 : 32768; }
+__host__ __device__ constexpr int dense_smem_bytes(int shape) {
+  return 1024 + dense_stages(shape) * dense_stage_bytes(shape) + kDenseEndWarps * (kDenseEndBytes + kDenseBiasBytes) + 512;
+}
 
 __device__ int tb_dense_status; // 0, or 4: a wait gave up
 
 struct DenseProblem {
   CUtensorMap a, b;
-  long long M, N;
+  int M, N;
   int a_rows_inner, b_rows_inner; // 1: rows lie one behind the other, not k
   int m_tiles, n_tiles, k_blocks;
   int chunk, chunks; // column tiles of a unit, units along the columns
   int splits;        // parts of the sum
   int group;         // row tiles that are walked together
-  long long units;
+  int units;
+};
+// Up to two products of one launch: the second one's units follow the first one's, so that the last wave of one
+// and the first of the other share the multiprocessors.
+template <class End, int JOBS> struct DenseJobs {
+  DenseProblem p[JOBS];
+  End end[JOBS];
+  int units; // of all
 };
 
 __device__ __forceinline__ uint32_t dense_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -47,7 +66,7 @@ __device__ __forceinline__ void dense_expect(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ bool dense_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
@@ -91,18 +110,14 @@ __device__ __forceinline__ void dense_mma(uint32_t d, uint64_t a, uint64_t b, ui
     asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
                  " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-__device__ __forceinline__ void dense_take(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-                 "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-                 "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+// 32 columns of a warp's 32 rows out of tensor memory; there after dense_taken, which every use depends on.
+__device__ __forceinline__ void dense_take(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void dense_taken(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
 // Operand in shared memory, 128-byte swizzle: k one behind the other: 8 rows of 64 k per 1 KB; rows one
 // behind the other: 64 rows x 64 k per 8 KB (the leading offset), 8 k per 1 KB.
@@ -121,42 +136,65 @@ template <> __device__ __forceinline__ constexpr uint32_t dense_format<__nv_bflo
 struct DenseUnit {
   int m, n0, n1, k0, k1, split, chunk;
 };
-__device__ __forceinline__ DenseUnit dense_unit(const DenseProblem &p, long long u) {
+__device__ __forceinline__ DenseUnit dense_unit(const DenseProblem &p, int u) {
   DenseUnit w;
-  w.split = (int)(u % p.splits);
-  const long long r = u / p.splits, per = (long long)p.group * p.chunks;
-  const int g = (int)(r / per) * p.group, in = (int)(r % per), rows = min(p.group, p.m_tiles - g);
-  w.m = g + in % rows;
+  int r = u;
+  w.split = 0;
+  if (p.splits > 1) w.split = u % p.splits, r = u / p.splits;
+  const int per = p.group * p.chunks, g = r / per, in = r - g * per, rows = min(p.group, p.m_tiles - g * p.group);
   w.chunk = in / rows;
+  w.m = g * p.group + in - w.chunk * rows;
   w.n0 = w.chunk * p.chunk;
   w.n1 = min(w.n0 + p.chunk, p.n_tiles);
-  w.k0 = (int)((long long)w.split * p.k_blocks / p.splits);
-  w.k1 = (int)((long long)(w.split + 1) * p.k_blocks / p.splits);
+  w.k0 = 0, w.k1 = p.k_blocks;
+  if (p.splits > 1) {
+    w.k0 = (int)((long long)w.split * p.k_blocks / p.splits);
+    w.k1 = (int)((long long)(w.split + 1) * p.k_blocks / p.splits);
+  }
   return w;
 }
 
+// A finishing warp's place: 4 KB and 256 bytes of shared memory, a barrier for copies into it.
+struct DenseWarp {
+  unsigned char *mine;
+  unsigned char *bias;
+  uint32_t bar, phase;
+  uint32_t turn; // which 2 KB the next result goes through
+  bool ok;
+};
+
 // End: what becomes of a tile.  A thread of a finishing warp has one row and 32 columns at a time:
-//   start(state, p, row, unit, half)                  once per unit
-//   tile(state, p, n, smem)                           once per column tile, n the warp's first column
-//   chunk(state, p, v, row, n, smem)                  v[j] = C[row, n + j]; row = the warp's first row + lane
-//   stop(state, p, row, unit, half)                   after the unit's last tile
-// `half` says which half of a tile's columns the warp has.
-template <class T, bool PAIR, class End>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kDenseThreads, 1)
-    tb_dense_kernel(const __grid_constant__ DenseProblem p, const __grid_constant__ End end) {
-  constexpr int BN = PAIR ? 256 : 128, BM = PAIR ? 256 : 128;
+//   start(state, p, row, unit)              once per unit and row
+//   tile(p, n, warp)                        once per column tile, n the warp's first column
+//   ahead(p, row, n, columns, warp)         before the wait for the sums of these columns
+//   chunk(state, p, r, row, n, unit, warp, second, more)   r[j] = C[row, n + j] (bits); row = the warp's first row + lane;
+//                                           second: not the warp's first 32 columns; more: 32 more follow
+//   stop(state, p, row, unit, part)         after the unit's last tile; part: which quarter of the columns the warp had
+template <class T, int SHAPE, class End, int JOBS>
+__global__ void __cluster_dims__(SHAPE == kDenseOne ? 1 : 2, 1, 1) __launch_bounds__(kDenseThreads, 1)
+    tb_dense_kernel(const __grid_constant__ DenseJobs<End, JOBS> jobs) {
+  constexpr bool PAIR = SHAPE != kDenseOne;
+  constexpr int BM = dense_rows(SHAPE), BN = dense_cols(SHAPE), MT = SHAPE == kDenseTall ? 2 : 1;
+  constexpr int kStages = dense_stages(SHAPE), kStageBytes = dense_stage_bytes(SHAPE), kColumns = BN / 4; // of a finishing warp
   extern __shared__ unsigned char raw[];
   const uint32_t base = (dense_smem(raw) + 1023u) & ~1023u;
-  unsigned char *base_p = raw + (base - dense_smem(raw));
-  unsigned char *end_p = base_p + kDenseStages * kDenseStageBytes;
-  const uint32_t bars = base + kDenseStages * kDenseStageBytes + kDenseEndWarps * kDenseEndBytes;
-  const uint32_t full = bars, empty = bars + 64, tfull = bars + 128, tempty = bars + 144, tmem_at = bars + 160;
+  unsigned char *end_p = raw + (base - dense_smem(raw)) + kStages * kStageBytes;
+  const uint32_t bars = base + kStages * kStageBytes + kDenseEndWarps * (kDenseEndBytes + kDenseBiasBytes);
+  const uint32_t full = bars, empty = bars + 48, tfull = bars + 96, tempty = bars + 112, own = bars + 128, tmem_at = bars + 256;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = PAIR ? blockIdx.x & 1 : 0;
-  const long long first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  // f(product, End, unit of it) for the block's u-th unit; the products' fields are constants of each branch
+  // (indexed, they would be loads)
+  auto of_job = [&](int u, auto f) {
+    if constexpr (JOBS == 2) {
+      if (u >= jobs.p[0].units) return f(jobs.p[1], jobs.end[1], u - jobs.p[0].units);
+    }
+    f(jobs.p[0], jobs.end[0], u);
+  };
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < kDenseStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       dense_bar_init(full + 8 * i, 1);
       dense_bar_init(empty + 8 * i, 1);
     }
@@ -164,6 +202,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kDenseThr
       dense_bar_init(tfull + 8 * i, 1);
       dense_bar_init(tempty + 8 * i, kDenseEndWarps * (PAIR ? 2 : 1));
     }
+    for (int i = 0; i < kDenseEndWarps; ++i) dense_bar_init(own + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -190,8 +229,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kDenseThr
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      long long loads = 0;
-      for (long long u = first; ok && u < p.units; u += step) {
+      int loads = 0;
+      for (int unit = first; ok && unit < jobs.units; unit += step) of_job(unit, [&](const DenseProblem &p, const End &, int u) {
         const DenseUnit w = dense_unit(p, u);
         const int row = w.m * BM + (int)rank * 128;
         for (int n = w.n0; ok && n < w.n1; ++n) {
@@ -199,13 +238,16 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kDenseThr
           for (int k = w.k0; k < w.k1; ++k) {
             if (!(ok = dense_wait(empty + 8 * stage, phase ^ 1))) break;
             const uint32_t bar = PAIR ? dense_first(full + 8 * stage) : full + 8 * stage;
-            if (rank == 0) dense_expect(full + 8 * stage, kDenseStageBytes * (PAIR ? 2 : 1));
-            const uint32_t a = base + stage * kDenseStageBytes, b = a + kDenseStageBytes / 2;
-            if (p.a_rows_inner) {
-              dense_load<PAIR>(a, &p.a, row, k * kDenseK, bar);
-              dense_load<PAIR>(a + 8192, &p.a, row + 64, k * kDenseK, bar);
-            } else {
-              dense_load<PAIR>(a, &p.a, k * kDenseK, row, bar);
+            if (rank == 0) dense_expect(full + 8 * stage, kStageBytes * (PAIR ? 2 : 1));
+            const uint32_t a = base + stage * kStageBytes, b = a + MT * 16384;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              if (p.a_rows_inner) {
+                dense_load<PAIR>(a + j * 16384, &p.a, row + j * 256, k * kDenseK, bar);
+                dense_load<PAIR>(a + j * 16384 + 8192, &p.a, row + j * 256 + 64, k * kDenseK, bar);
+              } else {
+                dense_load<PAIR>(a + j * 16384, &p.a, k * kDenseK, row + j * 256, bar);
+              }
             }
             if (p.b_rows_inner) {
               dense_load<PAIR>(b, &p.b, col, k * kDenseK, bar);
@@ -213,84 +255,139 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kDenseThr
             } else {
               dense_load<PAIR>(b, &p.b, k * kDenseK, col, bar);
             }
-            ++loads;
-            if (++stage == kDenseStages) stage = 0, phase ^= 1;
+            loads = min(loads + 1, kStages);
+            if (++stage == kStages) stage = 0, phase ^= 1;
           }
         }
-      }
+      });
       // what was loaded has been used, and every arrival of the matrix unit at this block's barriers is in:
       // the block may end
-      for (int i = 0; i < kDenseStages && i < loads; ++i) {
-        if (stage-- == 0) stage = kDenseStages - 1, phase ^= 1;
+      for (int i = 0; i < kStages && i < loads; ++i) {
+        if (stage-- == 0) stage = kStages - 1, phase ^= 1;
         if (ok) ok = dense_wait(empty + 8 * stage, phase);
         else if (rank == 0) dense_wait(full + 8 * stage, phase); // (copies in flight land before the way out)
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = 1u << 4 | dense_format<T>() << 7 | dense_format<T>() << 10 | (uint32_t)p.a_rows_inner << 15 |
-                             (uint32_t)p.b_rows_inner << 16 | (uint32_t)(BN / 8) << 17 | (uint32_t)(BM / 16) << 24;
-      const uint32_t a_step = p.a_rows_inner ? 2048 >> 4 : 32 >> 4, b_step = p.b_rows_inner ? 2048 >> 4 : 32 >> 4;
       int stage = 0, buf = 0;
       uint32_t phase = 0, tphase = 0;
-      for (long long u = first; ok && u < p.units; u += step) {
+      for (int unit = first; ok && unit < jobs.units; unit += step) of_job(unit, [&](const DenseProblem &p, const End &, int u) {
         const DenseUnit w = dense_unit(p, u);
-        for (int n = w.n0; ok && n < w.n1; ++n) {
-          if (!(ok = dense_wait(tempty + 8 * buf, tphase ^ 1))) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t d = tmem + (uint32_t)(buf * BN);
-          for (int k = w.k0; k < w.k1; ++k) {
-            if (!(ok = dense_wait(full + 8 * stage, phase))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = base + stage * kDenseStageBytes;
-            const uint64_t a = dense_desc(at, p.a_rows_inner), b = dense_desc(at + kDenseStageBytes / 2, p.b_rows_inner);
+        const uint32_t idesc = 1u << 4 | dense_format<T>() << 7 | dense_format<T>() << 10 | (uint32_t)p.a_rows_inner << 15 |
+                               (uint32_t)p.b_rows_inner << 16 | (uint32_t)(BN / 8) << 17 | (uint32_t)((PAIR ? 256 : 128) / 16) << 24;
+        const uint32_t a_step = p.a_rows_inner ? 2048 >> 4 : 32 >> 4, b_step = p.b_rows_inner ? 2048 >> 4 : 32 >> 4;
+        // 64 k of a stage, rows block j, into accumulator `acc`
+        auto multiply = [&](int at_stage, int j, int acc, bool fresh) {
+          const uint32_t at = base + at_stage * kStageBytes;
+          const uint64_t a = dense_desc(at + j * 16384, p.a_rows_inner), b = dense_desc(at + MT * 16384, p.b_rows_inner);
 #pragma unroll
-            for (int i = 0; i < kDenseK / 16; ++i) dense_mma<PAIR>(d, a + i * a_step, b + i * b_step, idesc, k > w.k0 || i > 0);
-            dense_commit<PAIR>(empty + 8 * stage);
-            if (++stage == kDenseStages) stage = 0, phase ^= 1;
+          for (int i = 0; i < kDenseK / 16; ++i)
+            dense_mma<PAIR>(tmem + (uint32_t)(acc * BN), a + i * a_step, b + i * b_step, idesc, !fresh || i > 0);
+        };
+        for (int n = w.n0; ok && n < w.n1; ++n) {
+          if constexpr (SHAPE == kDenseTall) {
+            constexpr int kTail = 2;
+            if (!(ok = dense_wait(tempty, tphase ^ 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            int behind = stage, lag = 0; // the second accumulator's next stage, and how many it is behind
+            bool second = false, fresh = true;
+            for (int k = w.k0; k < w.k1; ++k) {
+              if (!(ok = dense_wait(full + 8 * stage, phase))) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              multiply(stage, 0, 0, k == w.k0);
+              ++lag;
+              if (++stage == kStages) stage = 0, phase ^= 1;
+              const bool end = k == w.k1 - 1;
+              if (end) dense_commit<PAIR>(tfull);
+              if (!second) {
+                if (lag == kStages || end) {
+                  if (!(ok = dense_wait(tempty + 8, tphase ^ 1))) break;
+                  second = true;
+                } else {
+                  second = dense_try(tempty + 8, tphase ^ 1);
+                }
+                if (second) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              }
+              if (second && (end || k < w.k1 - kTail || lag == kStages))
+                for (; lag > 0; --lag) {
+                  multiply(behind, 1, 1, fresh);
+                  fresh = false;
+                  dense_commit<PAIR>(empty + 8 * behind);
+                  if (++behind == kStages) behind = 0;
+                }
+            }
+            if (!ok) break;
+            dense_commit<PAIR>(tfull + 8);
+            tphase ^= 1;
+          } else {
+            if (!(ok = dense_wait(tempty + 8 * buf, tphase ^ 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int k = w.k0; k < w.k1; ++k) {
+              if (!(ok = dense_wait(full + 8 * stage, phase))) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              multiply(stage, 0, buf, k == w.k0);
+              dense_commit<PAIR>(empty + 8 * stage);
+              if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+            if (!ok) break;
+            dense_commit<PAIR>(tfull + 8 * buf);
+            if (++buf == 2) buf = 0, tphase ^= 1;
           }
-          if (!ok) break;
-          dense_commit<PAIR>(tfull + 8 * buf);
-          if (++buf == 2) buf = 0, tphase ^= 1;
         }
-      }
+      });
     }
   } else if (warp >= 4) {
-    const int e = warp - 4, half = e / 4;
-    unsigned char *mine = end_p + e * kDenseEndBytes;
+    const int e = warp - 4, part = e / 4;
+    DenseWarp me{end_p + e * kDenseEndBytes, end_p + kDenseEndWarps * kDenseEndBytes + e * kDenseBiasBytes, own + 8 * e, 0, 0, true};
     const uint32_t free_bar = PAIR ? dense_first(tempty) : tempty;
     int buf = 0;
     uint32_t tphase = 0;
-    for (long long u = first; ok && u < p.units; u += step) {
+    for (int unit = first; ok && unit < jobs.units; unit += step) of_job(unit, [&](const DenseProblem &p, const End &end, int u) {
       const DenseUnit w = dense_unit(p, u);
-      const long long row = (long long)w.m * BM + rank * 128 + (warp % 4) * 32 + lane;
-      typename End::State state;
-      end.start(state, p, row, w, half);
-      for (int n = w.n0; n < w.n1; ++n) {
-        const long long col = (long long)n * BN + half * (BN / 2);
-        end.tile(state, p, col, mine);
-        if (!(ok = __all_sync(~0u, dense_wait(tfull + 8 * buf, tphase)))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t at = tmem + (uint32_t)(buf * BN + half * (BN / 2)) + ((uint32_t)(warp % 4) << 21);
+      const int row = w.m * BM + (int)rank * 128 + (warp % 4) * 32 + lane;
+      typename End::State state[MT];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) end.start(state[j], p, row + j * 256, w);
+      for (int n = w.n0; ok && n < w.n1; ++n) {
+        const int col = n * BN + part * kColumns;
+        end.tile(p, col, me);
+#pragma unroll(sizeof(state) > 2 ? 2 : 1)
+        for (int j = 0; j < MT; ++j) {
+          if (MT == 2) buf = j;
+          if (col < p.N) end.ahead(p, row + j * 256, col, kColumns, me);
+          if (!(ok = __all_sync(~0u, dense_wait(tfull + 8 * buf, tphase)))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t at = tmem + (uint32_t)(buf * BN + part * kColumns) + ((uint32_t)(warp % 4) << 21);
 #pragma unroll 1
-        for (int c = 0; c < BN / 64; ++c) {
-          float v[32];
-          dense_take(at + c * 32, v);
-          if (c == BN / 64 - 1) { // the accumulator is free as soon as the last values are in registers
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) {
-              if constexpr (PAIR)
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(free_bar + 8 * buf) : "memory");
-              else
-                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(free_bar + 8 * buf) : "memory");
+          for (int c = 0; c < kColumns; c += 32) {
+            uint32_t r[32];
+            __syncwarp();
+            dense_take(at + c, r);
+            dense_taken(r);
+            if (c + 32 == kColumns) { // the accumulator is free as soon as its last values are in registers
+              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (PAIR)
+                  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free_bar + 8 * buf) : "memory");
+                else
+                  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(free_bar + 8 * buf) : "memory");
+              }
             }
+            if (col + c < p.N) end.chunk(state[j], p, r, row + j * 256, col + c, w, me, c > 0, c + 32 < kColumns && col + c + 32 < p.N);
           }
-          if (col + c * 32 < p.N) end.chunk(state, p, v, row, col + c * 32, w, mine);
         }
-        if (++buf == 2) buf = 0, tphase ^= 1;
+        if (MT == 2) tphase ^= 1;
+        else if (++buf == 2) buf = 0, tphase ^= 1;
       }
-      if (ok) end.stop(state, p, row, w, half);
-    }
+      if (ok) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) end.stop(state[j], p, row + j * 256, w, part);
+      }
+    });
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); // (stores under way read shared memory)
+    ok = ok && me.ok;
   }
   if (!ok) atomicExch(&tb_dense_status, 4);
   __syncwarp();
@@ -321,44 +418,86 @@ __device__ __forceinline__ float inverse_fast(float x) { // within a step of 2^-
 }
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
 
-// Phi(z), the integral of the normal distribution, and exp(-z^2 / 2).  erfc's shape after Hastings
+// Two fp32 operations in one instruction.
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ explicit Two(float2 a) : Two(a.x, a.y) {}
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Phi(z), the integral of the normal distribution, and exp(-z^2 / 2), of two z.  erfc's shape after Hastings
 // (Approximations for Digital Computers, 1955): Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.33 |z|);
 // P was fitted here, by reweighted least squares, for the relative error: below 1e-6 for all z.  Without
 // branches, since a warp's values need both sides of any (the library's erff took most of a layer's time).
-__device__ __forceinline__ float normal_integral(float z, float *bell) {
-  const float a = fabsf(z), t = inverse_fast(fmaf(a, 0.33f, 1.f));
-  float p = fmaf(0.0332859295f, t, -0.105665717f);
-  p = fmaf(p, t, 0.067432403f);
-  p = fmaf(p, t, 0.0334278586f);
-  p = fmaf(p, t, 0.0910052722f);
-  p = fmaf(p, t, 0.117216671f);
-  p = fmaf(p, t, 0.13164699f);
-  p = fmaf(p, t, 0.131651081f);
-  *bell = exp2_fast(z * z * (-0.5f * kLog2e));
-  const float tail = *bell * t * p;
-  return z >= 0.f ? 1.f - tail : tail;
+__device__ __forceinline__ float2 normal_integral(float2 z, float2 *bell) {
+  const float2 d = fma2(Two(fabsf(z.x), fabsf(z.y)), Two(0.33f), Two(1.f)).get();
+  const Two t(inverse_fast(d.x), inverse_fast(d.y)), zz(z.x, z.y);
+  Two p = fma2(Two(0.0332859295f), t, Two(-0.105665717f));
+  p = fma2(p, t, Two(0.067432403f));
+  p = fma2(p, t, Two(0.0334278586f));
+  p = fma2(p, t, Two(0.0910052722f));
+  p = fma2(p, t, Two(0.117216671f));
+  p = fma2(p, t, Two(0.13164699f));
+  p = fma2(p, t, Two(0.131651081f));
+  const float2 e = (zz * (zz * Two(-0.5f * kLog2e))).get();
+  *bell = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+  const float2 tail = (Two(bell->x, bell->y) * t * p).get();
+  return make_float2(z.x >= 0.f ? 1.f - tail.x : tail.x, z.y >= 0.f ? 1.f - tail.y : tail.y);
 }
-__device__ __forceinline__ float act_value(float z, int act) {
-  if (act == 1) return z < 0.f ? 0.f : z; // (NaN stays)
-  if (act == 2) {
-    float bell;
-    return z * normal_integral(z, &bell);
+enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
+template <int ACT> __device__ __forceinline__ float2 act_value(float2 z) {
+  if constexpr (ACT == kActRelu) return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y); // (NaN stays)
+  if constexpr (ACT == kActGelu) {
+    float2 bell;
+    const float2 w = normal_integral(z, &bell);
+    return make_float2(z.x * w.x, z.y * w.y);
   }
-  if (act == 3) return z * inverse_fast(1.f + exp2_fast(-kLog2e * z));
+  if constexpr (ACT == kActSilu)
+    return make_float2(z.x * inverse_fast(1.f + exp2_fast(-kLog2e * z.x)), z.y * inverse_fast(1.f + exp2_fast(-kLog2e * z.y)));
   return z;
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == 1) return z > 0.f ? 1.f : 0.f;
-  if (act == 2) {
-    float bell;
-    const float w = normal_integral(z, &bell);
-    return fmaf(z * 0.39894228f, bell, w);
+template <int ACT> __device__ __forceinline__ float2 act_slope(float2 z) {
+  if constexpr (ACT == kActRelu) return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+  if constexpr (ACT == kActGelu) {
+    float2 bell;
+    const float2 w = normal_integral(z, &bell);
+    return make_float2(fmaf(z.x * 0.39894228f, bell.x, w.x), fmaf(z.y * 0.39894228f, bell.y, w.y));
   }
-  if (act == 3) {
-    const float s = inverse_fast(1.f + exp2_fast(-kLog2e * z));
-    return s * fmaf(z, 1.f - s, 1.f);
+  if constexpr (ACT == kActSilu) {
+    const float s = inverse_fast(1.f + exp2_fast(-kLog2e * z.x)), t = inverse_fast(1.f + exp2_fast(-kLog2e * z.y));
+    return make_float2(s * fmaf(z.x, 1.f - s, 1.f), t * fmaf(z.y, 1.f - t, 1.f));
   }
-  return 1.f;
+  return make_float2(1.f, 1.f);
+}
+// f(activation as a constant): one test for all of a thread's values
+template <class F> __device__ __forceinline__ void with_act(int act, F f) {
+  switch (act) {
+  case kActRelu: f(std::integral_constant<int, kActRelu>()); break;
+  case kActGelu: f(std::integral_constant<int, kActGelu>()); break;
+  case kActSilu: f(std::integral_constant<int, kActSilu>()); break;
+  }
 }
 
 template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -369,6 +508,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <class T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 // Eight consecutive elements, `n` of them there; `vec`: 16-byte aligned.
 template <class T> __device__ __forceinline__ void store8(T *p, const float (&v)[8], int n, bool vec) {
@@ -392,68 +535,134 @@ template <class T> __device__ __forceinline__ void load8(const T *p, float (&v)[
   }
 }
 
-// Turns 32 rows x 32 columns of a warp around in its shared memory, so that a lane has eight consecutive
-// columns of a row: f(row 0..31, column 0, 8, 16 or 24, values).  16-byte pieces are swapped around by the
-// row's number, which keeps both directions free of bank conflicts.
-template <class F> __device__ __forceinline__ void turned(const float (&v)[32], unsigned char *mine, F f) {
-  const int lane = threadIdx.x % 32;
-  float4 *s = reinterpret_cast<float4 *>(mine);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[lane * 8 + (i ^ (lane & 7))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+// Results on their way out: a warp puts 32 rows x 32 columns (a row is 64 bytes, its 16-byte pieces swapped
+// around by the row's number, as the tensor map says) into its shared memory and one tensor copy takes them to
+// where they belong; what is behind the last row or column the copy leaves out.
+constexpr int kOutBytes = 2048;
+template <int BUT> __device__ __forceinline__ void out_free() { // all copies but the last BUT have read the shared memory
+  if (threadIdx.x % 32 == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUT) : "memory");
   __syncwarp();
+}
+__device__ __forceinline__ uint4 *out_piece(unsigned char *buf, int i) { // the lane's row's columns 8 i ...
+  const int lane = threadIdx.x % 32;
+  return reinterpret_cast<uint4 *>(buf) + lane * 4 + (i ^ (lane >> 1 & 3));
+}
+template <class T> __device__ __forceinline__ void out_put(unsigned char *buf, const Two (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + lane / 4, c = lane % 4;
-    const float4 x = s[r * 8 + ((2 * c) ^ (r & 7))], y = s[r * 8 + ((2 * c + 1) ^ (r & 7))];
-    const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    f(r, c * 8, w);
+    const float2 a = v[4 * i].get(), b = v[4 * i + 1].get(), c = v[4 * i + 2].get(), d = v[4 * i + 3].get();
+    *out_piece(buf, i) = make_uint4(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y), pack2<T>(c.x, c.y), pack2<T>(d.x, d.y));
   }
+}
+__device__ __forceinline__ void out_ready() { // (of all lanes, before one of them sends)
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
+__device__ __forceinline__ void out_send(const CUtensorMap *map, const unsigned char *buf, int m, int n) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+               ::"l"(map), "r"(n), "r"(m), "r"(dense_smem(buf)) : "memory");
+}
+__device__ __forceinline__ void out_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
-// The same with a lane per column: f(row, value), for results whose rows begin anywhere: a warp then writes 32
-// neighbouring elements at a time instead of every eighth.
-template <class F> __device__ __forceinline__ void turned_columns(const float (&v)[32], unsigned char *mine, F f) {
+// 32 rows x 32 fp32 values turned around in shared memory, 16-byte pieces swapped around by the row's number,
+// which keeps both directions free of bank conflicts.  f(row, column 0, 8, 16 or 24, eight values) ...
+__device__ __forceinline__ void turn(const uint32_t (&r)[32], unsigned char *mine) {
   const int lane = threadIdx.x % 32;
-  float4 *s = reinterpret_cast<float4 *>(mine);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[lane * 8 + (i ^ (lane & 7))] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  uint4 *s = reinterpret_cast<uint4 *>(mine);
   __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[lane * 8 + (i ^ (lane & 7))] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+  __syncwarp();
+}
+template <class F> __device__ __forceinline__ void turned(const uint32_t (&r)[32], unsigned char *mine, F f) {
+  turn(r, mine);
+  const int lane = threadIdx.x % 32;
+  const float4 *s = reinterpret_cast<const float4 *>(mine);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + lane / 4, c = lane % 4;
+    const float4 x = s[row * 8 + ((2 * c) ^ (row & 7))], y = s[row * 8 + ((2 * c + 1) ^ (row & 7))];
+    const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    f(row, c * 8, w);
+  }
+}
+// ... or f(row, value of the lane's column), for results whose rows begin anywhere: a warp then writes 32
+// neighbouring elements at a time.
+template <class F> __device__ __forceinline__ void turned_columns(const uint32_t (&r)[32], unsigned char *mine, F f) {
+  turn(r, mine);
+  const int lane = threadIdx.x % 32;
   const float *w = reinterpret_cast<const float *>(mine) + lane % 4;
 #pragma unroll 8
-  for (int r = 0; r < 32; ++r) f(r, w[(r * 8 + ((lane / 4) ^ (r & 7))) * 4]);
-  __syncwarp();
+  for (int row = 0; row < 32; ++row) f(row, w[(row * 8 + ((lane / 4) ^ (row & 7))) * 4]);
 }
 
-// y = activation(z + bias) + residual, and z + bias
-template <class T> struct LinearEnd {
-  const T *bias, *residual;
+// What a whole sum c becomes: z = c / scale + bias; out = activation(z) + addend; pre = z.  Or, with `sums`, one
+// piece of a longer sum, added to the pieces before it.  With `parts` the sum is cut into parts, which are kept:
+// parts[split][row][ld_parts].
+template <class T> struct Result {
+  CUtensorMap out_map, pre_map, addend_map; // where `sends`
+  const T *bias, *addend;
   T *out, *pre;
-  long long ld_residual, ld_out, ld_pre;
+  float *sums; // [rows][ld_sums] or null
+  float *parts; // or null
+  const float *scale; // a power of two, or null
+  long long ld_addend, ld_out, ld_pre, ld_sums, ld_parts;
   int act;
-  bool vec_residual, vec_out, vec_pre, vec_bias;
+  bool first, last;                                   // piece of a sum
+  bool sends, vec_addend, vec_out, vec_pre, vec_bias; // rows lie at multiples of 16 bytes
   __device__ __forceinline__ void finish1(float c, long long m, long long n) const {
+    if (sums) {
+      float *s = sums + m * ld_sums + n;
+      if (!first) c += *s;
+      if (!last) {
+        *s = c;
+        return;
+      }
+    }
+    if (scale) c *= 1.f / *scale;
     const float z = bias ? c + to_float(bias[n]) : c;
     if (pre) pre[m * ld_pre + n] = from_float<T>(z);
-    const float y = act_value(z, act);
-    out[m * ld_out + n] = from_float<T>(residual ? y + to_float(residual[m * ld_residual + n]) : y);
+    float y = z;
+    with_act(act, [&](auto a) { y = act_value<decltype(a)::value>(make_float2(z, z)).x; });
+    out[m * ld_out + n] = from_float<T>(addend ? y + to_float(addend[m * ld_addend + n]) : y);
   }
   __device__ __forceinline__ void finish8(const float (&c)[8], long long m, long long n, long long N) const {
     const int have = (int)min(8ll, N - n);
     float z[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = c[i];
+    if (sums) {
+      float4 *s = reinterpret_cast<float4 *>(sums + m * ld_sums + n); // (ld a multiple of 8: whole pieces of 8 are there)
+      if (!first) {
+        const float4 x = s[0], y = s[1];
+        z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w, z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
+      }
+      if (!last) {
+        s[0] = make_float4(z[0], z[1], z[2], z[3]);
+        s[1] = make_float4(z[4], z[5], z[6], z[7]);
+        return;
+      }
+    }
+    if (scale) {
+      const float d = 1.f / *scale;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] *= d;
+    }
     if (bias) {
       load8(bias + n, b, have, vec_bias);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = c[i] + b[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = c[i];
+      for (int i = 0; i < 8; ++i) z[i] += b[i];
     }
     if (pre) store8(pre + m * ld_pre + n, z, have, vec_pre);
+    with_act(act, [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = act_value(z[i], act);
-    if (residual) {
-      load8(residual + m * ld_residual + n, b, have, vec_residual);
+      for (int i = 0; i < 8; i += 2) {
+        const float2 y = act_value<decltype(a)::value>(make_float2(z[i], z[i + 1]));
+        z[i] = y.x, z[i + 1] = y.y;
+      }
+    });
+    if (addend) {
+      load8(addend + m * ld_addend + n, b, have, vec_addend);
 #pragma unroll
       for (int i = 0; i < 8; ++i) z[i] += b[i];
     }
@@ -461,101 +670,128 @@ template <class T> struct LinearEnd {
   }
 };
 
-// gradient with respect to an operand: a finished sum, or one piece of it
-template <class T> struct SumEnd {
-  float *sums; // [rows][ld]: what came before, where the sum comes in pieces
-  long long ld;
-  T *out;
-  const T *skip; // added at the end, or null
-  long long ld_out, ld_skip;
-  const float *scale; // divides the result; null: 1
-  bool first, last, vec_out, vec_skip;
-  __device__ __forceinline__ void finish1(float c, long long m, long long n) const {
-    float *s = sums + m * ld + n;
-    if (!first) c += *s;
-    if (!last) {
-      *s = c;
+// Finishes sums.  Where all matrices' rows lie at multiples of 16 bytes (`sends`) a lane keeps its row: addends
+// come, and results go, 32 rows x 32 columns at a time by tensor copies.  (Reading them a row per lane took longer
+// than the product.)  A warp has two pieces of 2 KB, which results go through by turns; addends come there, one
+// for each half of the warp's columns, before the sums are done, and the results replace them; where z is kept too,
+// the second is z's.
+template <class T> struct ResultEnd {
+  Result<T> f;
+  struct State {};
+  __device__ __forceinline__ void start(State &, const DenseProblem &, int, const DenseUnit &) const {}
+  __device__ __forceinline__ void tile(const DenseProblem &p, int n, DenseWarp &w) const {
+    if (!f.bias || !f.sends) return;
+    T *b = reinterpret_cast<T *>(w.bias);
+    __syncwarp();
+#pragma unroll
+    for (int i = threadIdx.x % 32; i < 64; i += 32) { // (of the 64 columns that the warp's lie in)
+      const int c = n - n % 64 + i;
+      b[i] = c < p.N ? f.bias[c] : from_float<T>(0.f);
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void fetch(int row, int n, unsigned char *to, DenseWarp &w) const {
+    dense_load<false>(dense_smem(to), &f.addend_map, n, row, w.bar);
+  }
+  // (row: the lane's; the first lane's is the warp's first)
+  __device__ __forceinline__ void ahead(const DenseProblem &p, int row, int n, int columns, DenseWarp &w) const {
+    if (!f.sends || !f.addend || threadIdx.x % 32) return;
+    const bool two = columns > 32 && n + 32 < p.N && !f.pre;
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); // (the last results may still be on their way)
+    dense_expect(w.bar, two ? 2 * kOutBytes : kOutBytes);
+    fetch(row, n, w.mine, w);
+    if (two) fetch(row, n + 32, w.mine + kOutBytes, w);
+  }
+  __device__ __forceinline__ void chunk(State &, const DenseProblem &p, const uint32_t (&r)[32], int row, int n, const DenseUnit &u,
+                                        DenseWarp &w, bool second, bool more) const {
+    const int lane = threadIdx.x % 32;
+    const int m0 = row - lane;
+    if (!f.sends) {
+      if (f.parts)
+        turned(r, w.mine, [&](int k, int c, const float (&x)[8]) {
+          if (m0 + k >= p.M || n + c >= p.N) return;
+          float4 *d = reinterpret_cast<float4 *>(f.parts + ((long long)u.split * p.M + m0 + k) * f.ld_parts + n + c);
+          d[0] = make_float4(x[0], x[1], x[2], x[3]);
+          d[1] = make_float4(x[4], x[5], x[6], x[7]);
+        });
+      else if (f.vec_out)
+        turned(r, w.mine, [&](int k, int c, const float (&x)[8]) {
+          if (m0 + k < p.M && n + c < p.N) f.finish8(x, m0 + k, n + c, p.N);
+        });
+      else
+        turned_columns(r, w.mine, [&](int k, float x) {
+          if (m0 + k < p.M && n + lane < p.N) f.finish1(x, m0 + k, n + lane);
+        });
       return;
     }
-    if (scale) c *= 1.f / *scale;
-    out[m * ld_out + n] = from_float<T>(skip ? c + to_float(skip[m * ld_skip + n]) : c);
-  }
-  __device__ __forceinline__ void finish8(const float (&c)[8], long long m, long long n, long long N) const {
-    const int have = (int)min(8ll, N - n);
-    float v[8];
+    Two z[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c[i];
-    float *s = sums + m * ld + n; // (ld a multiple of 8: whole pieces of 8 are there)
-    if (!first) {
+    for (int i = 0; i < 16; ++i) z[i] = Two(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    if (f.scale) {
+      const Two d(1.f / *f.scale);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += s[i];
+      for (int i = 0; i < 16; ++i) z[i] = z[i] * d;
     }
-    if (!last) {
+    auto add8 = [&](int i, uint4 q) {
+      z[4 * i] = z[4 * i] + Two(unpack2<T>(q.x));
+      z[4 * i + 1] = z[4 * i + 1] + Two(unpack2<T>(q.y));
+      z[4 * i + 2] = z[4 * i + 2] + Two(unpack2<T>(q.z));
+      z[4 * i + 3] = z[4 * i + 3] + Two(unpack2<T>(q.w));
+    };
+    if (f.bias) {
+      const uint4 *b = reinterpret_cast<const uint4 *>(w.bias) + n % 64 / 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = v[i];
-      return;
+      for (int i = 0; i < 4; ++i) add8(i, b[i]);
     }
-    if (scale) {
-      const float d = 1.f / *scale; // (a power of two)
+    unsigned char *to = w.mine + (f.pre ? 0 : f.addend ? (second ? kOutBytes : 0) : w.turn);
+    w.turn ^= kOutBytes;
+    if (f.addend) {
+      if (!second || f.pre) {
+        if (w.ok) w.ok = __all_sync(~0u, dense_wait(w.bar, w.phase));
+        w.phase ^= 1;
+      }
+    } else if (f.pre) {
+      out_free<0>();
+    } else {
+      out_free<1>(); // (the other piece's copy may be under way)
+    }
+    if (f.pre) {
+      if (f.addend) out_free<0>();
+      out_put<T>(w.mine + kOutBytes, z);
+    }
+    with_act(f.act, [&](auto a) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= d;
-    }
-    if (skip) {
-      float b[8];
-      load8(skip + m * ld_skip + n, b, have, vec_skip);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += b[i];
-    }
-    store8(out + m * ld_out + n, v, have, vec_out);
-  }
-};
-
-// Finishes whole sums in place.
-template <class F> struct WholeEnd {
-  F f;
-  struct State {};
-  __device__ __forceinline__ void start(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
-  __device__ __forceinline__ void tile(State &, const DenseProblem &, long long, unsigned char *) const {}
-  __device__ __forceinline__ void chunk(State &, const DenseProblem &p, const float (&v)[32], long long row, long long n, const DenseUnit &,
-                                        unsigned char *mine) const {
-    const long long m0 = row - threadIdx.x % 32;
-    if (f.vec_out)
-      turned(v, mine, [&](int r, int c, const float (&w)[8]) {
-        if (m0 + r < p.M && n + c < p.N) f.finish8(w, m0 + r, n + c, p.N);
-      });
-    else
-      turned_columns(v, mine, [&](int r, float w) {
-        if (m0 + r < p.M && n + threadIdx.x % 32 < p.N) f.finish1(w, m0 + r, n + threadIdx.x % 32);
-      });
-  }
-  __device__ __forceinline__ void stop(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
-};
-// Keeps the parts of sums that are cut into `splits`: parts[split][row][ld]
-struct PartEnd {
-  float *parts;
-  long long ld;
-  struct State {};
-  __device__ __forceinline__ void start(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
-  __device__ __forceinline__ void tile(State &, const DenseProblem &, long long, unsigned char *) const {}
-  __device__ __forceinline__ void chunk(State &, const DenseProblem &p, const float (&v)[32], long long row, long long n, const DenseUnit &u,
-                                        unsigned char *mine) const {
-    const long long m0 = row - threadIdx.x % 32;
-    turned(v, mine, [&](int r, int c, const float (&w)[8]) {
-      if (m0 + r >= p.M || n + c >= p.N) return;
-      float4 *d = reinterpret_cast<float4 *>(parts + ((long long)u.split * p.M + m0 + r) * ld + n + c);
-      d[0] = make_float4(w[0], w[1], w[2], w[3]);
-      d[1] = make_float4(w[4], w[5], w[6], w[7]);
+      for (int i = 0; i < 16; ++i) z[i] = Two(act_value<decltype(a)::value>(z[i].get()));
     });
+    if (f.addend) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) add8(i, *out_piece(to, i));
+    }
+    out_put<T>(to, z);
+    out_ready();
+    if (lane) return;
+    if (m0 < p.M) {
+      out_send(&f.out_map, to, m0, n);
+      if (f.pre) out_send(&f.pre_map, w.mine + kOutBytes, m0, n);
+    }
+    out_commit();
+    if (more && f.addend && f.pre) { // (no room for it before)
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      dense_expect(w.bar, kOutBytes);
+      fetch(m0, n + 32, w.mine, w);
+    }
   }
-  __device__ __forceinline__ void stop(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
+  __device__ __forceinline__ void stop(State &, const DenseProblem &, int, const DenseUnit &, int) const {}
 };
 // Adds the parts up, in order, and finishes them.
-template <class F>
-__global__ void __launch_bounds__(256) tb_dense_join_kernel(const float *parts, int splits, long long ld, long long M, long long N, F f) {
+template <class T>
+__global__ void __launch_bounds__(256) tb_dense_join_kernel(const float *parts, int splits, long long ld, long long M, long long N,
+                                                            const __grid_constant__ Result<T> f) {
   const long long per = ld / 8, i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= M * per) return;
   const long long m = i / per, n = i % per * 8;
   float v[8] = {};
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float4 *d = reinterpret_cast<const float4 *>(parts + ((long long)s * M + m) * ld + n);
     const float4 a = d[0], b = d[1];
@@ -567,10 +803,10 @@ __global__ void __launch_bounds__(256) tb_dense_join_kernel(const float *parts, 
 __device__ __forceinline__ long long label_at(const void *labels, int bytes, long long m) {
   return bytes == 8 ? static_cast<const long long *>(labels)[m] : static_cast<const int *>(labels)[m];
 }
-// The biases of a warp's 128 (or 64) columns of a tile in units of log2, in its shared memory; -inf for
+// The biases of a warp's 64 (or 32) columns of a tile in units of log2, in its shared memory; -inf for
 // columns behind the last class, which thereby have probability 0.
 template <class T, int COLS>
-__device__ __forceinline__ void stage_bias(const T *bias, long long n, long long N, float *dst) {
+__device__ __forceinline__ void stage_bias(const T *bias, int n, int N, float *dst) {
   __syncwarp();
 #pragma unroll
   for (int i = threadIdx.x % 32; i < COLS; i += 32) dst[i] = n + i >= N ? -INFINITY : bias ? to_float(bias[n + i]) * kLog2e : 0.f;
@@ -578,7 +814,7 @@ __device__ __forceinline__ void stage_bias(const T *bias, long long n, long long
 }
 
 // Sum of a row's exponentials over the tiles of a unit, relative to the largest score of them, in one pass:
-// the sum so far is scaled down whenever a larger score comes.  parts[2 * chunk + half][row]
+// the sum so far is scaled down whenever a larger score comes.  parts[4 * chunk + part][row]
 template <class T, int COLS> struct LseEnd {
   const T *bias;
   const void *labels;
@@ -587,57 +823,61 @@ template <class T, int COLS> struct LseEnd {
   float *at; // [rows] the label's score
   struct State {
     float top, sum;
-    long long label, tile;
+    int label;
   };
-  __device__ __forceinline__ void start(State &s, const DenseProblem &p, long long row, const DenseUnit &, int) const {
+  __device__ __forceinline__ void start(State &s, const DenseProblem &p, int row, const DenseUnit &) const {
     s.top = -INFINITY;
     s.sum = 0.f;
-    s.label = row < p.M ? label_at(labels, label_bytes, row) : -1;
+    const long long label = row < p.M ? label_at(labels, label_bytes, row) : -1;
+    s.label = label >= 0 && label < p.N ? (int)label : -1;
   }
-  __device__ __forceinline__ void tile(State &s, const DenseProblem &p, long long n, unsigned char *mine) const {
-    s.tile = n;
-    stage_bias<T, COLS>(bias, n, p.N, reinterpret_cast<float *>(mine));
+  __device__ __forceinline__ void tile(const DenseProblem &p, int n, DenseWarp &w) const {
+    stage_bias<T, COLS>(bias, n, p.N, reinterpret_cast<float *>(w.bias));
   }
-  __device__ __forceinline__ void chunk(State &s, const DenseProblem &p, float (&v)[32], long long row, long long n, const DenseUnit &,
-                                        unsigned char *mine) const {
-    const long long at_label = s.label - n;
-    if (at_label >= 0 && at_label < 32 && s.label < p.N) { // (the score itself, not its multiple)
+  __device__ __forceinline__ void ahead(const DenseProblem &, int, int, int, DenseWarp &) const {}
+  __device__ __forceinline__ void chunk(State &s, const DenseProblem &p, const uint32_t (&r)[32], int row, int n, const DenseUnit &,
+                                        DenseWarp &w, bool, bool) const {
+    const int at_label = s.label - n;
+    if (s.label >= 0 && at_label >= 0 && at_label < 32) { // (the score itself, not its multiple)
       float z = 0.f;
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j == at_label) z = v[j];
+        if (j == at_label) z = __uint_as_float(r[j]);
       at[row] = bias ? z + to_float(bias[s.label]) : z;
     }
-    const float4 *b4 = reinterpret_cast<const float4 *>(mine) + (n - s.tile) / 4;
-    float top = -INFINITY;
+    const ulonglong2 *b2 = reinterpret_cast<const ulonglong2 *>(w.bias) + n % COLS / 4;
+    Two z[16];
+    float top = s.top;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float4 b = b4[j];
-      v[4 * j] = fmaf(v[4 * j], kLog2e, b.x);
-      v[4 * j + 1] = fmaf(v[4 * j + 1], kLog2e, b.y);
-      v[4 * j + 2] = fmaf(v[4 * j + 2], kLog2e, b.z);
-      v[4 * j + 3] = fmaf(v[4 * j + 3], kLog2e, b.w);
-      top = fmaxf(top, fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3])));
+      const ulonglong2 b = b2[j];
+      Two lo, hi;
+      lo.v = b.x, hi.v = b.y;
+      z[2 * j] = fma2(Two(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), Two(kLog2e), lo);
+      z[2 * j + 1] = fma2(Two(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), Two(kLog2e), hi);
+      const float2 x = z[2 * j].get(), y = z[2 * j + 1].get();
+      top = fmaxf(top, fmaxf(x.x, x.y));
+      top = fmaxf(top, fmaxf(y.x, y.y));
     }
-    top = fmaxf(top, s.top);
     const float ref = top == -INFINITY ? 0.f : top; // (all so far forbidden: exponentials are 0)
-    float a = 0.f, b = 0.f, c = 0.f, d = 0.f;
+    const Two less(-ref);
+    Two sum[2] = {Two(0.f), Two(0.f)};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a += exp2_fast(v[4 * j] - ref);
-      b += exp2_fast(v[4 * j + 1] - ref);
-      c += exp2_fast(v[4 * j + 2] - ref);
-      d += exp2_fast(v[4 * j + 3] - ref);
+    for (int j = 0; j < 16; ++j) {
+      const float2 x = (z[j] + less).get();
+      sum[j & 1] = sum[j & 1] + Two(exp2_fast(x.x), exp2_fast(x.y));
     }
-    s.sum = s.sum * exp2_fast(s.top - ref) + ((a + b) + (c + d));
+    const float2 x = (sum[0] + sum[1]).get();
+    s.sum = s.sum * exp2_fast(s.top - ref) + (x.x + x.y);
     s.top = top;
   }
-  __device__ __forceinline__ void stop(State &s, const DenseProblem &p, long long row, const DenseUnit &u, int half) const {
-    if (row < p.M) parts[(2ll * u.chunk + half) * p.M + row] = make_float2(s.top, s.sum);
+  __device__ __forceinline__ void stop(State &s, const DenseProblem &p, int row, const DenseUnit &u, int part) const {
+    if (row < p.M) parts[(4ll * u.chunk + part) * p.M + row] = make_float2(s.top, s.sum);
   }
 };
+
 // A row's logarithm and loss from its parts: a lane per row, the parts over the block's warps.
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 32;
 __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const float2 *parts, int count, const float *at, const void *labels, int label_bytes,
                                                                        long long classes, float *loss, float *lse, long long rows) {
   __shared__ float2 mine[kJoinWarps][32];
@@ -656,7 +896,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const flo
   mine[warp][lane] = make_float2(top, sum);
   __syncthreads();
   if (warp || m >= rows) return;
-#pragma unroll
+#pragma unroll 4
   for (int w = 1; w < kJoinWarps; ++w) join(mine[w][lane]);
   const float l = fmaf(top == -INFINITY ? 0.f : top, kLn2, logf(sum));
   const long long label = label_at(labels, label_bytes, m);
@@ -667,113 +907,133 @@ __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const flo
 // dz = weight * (exp(z - lse) - [label]) * scale, rounded, and the sums of its columns over 32 rows before
 // that: bias_sums[row / 32][ld]
 template <class T, int COLS> struct ScoreGradEnd {
+  CUtensorMap dz_map;
   const T *bias; // of the piece's first class
   const void *labels;
   int label_bytes;
   const float *grad, *lse, *scale;
-  T *dz;
-  long long ld, first, classes; // class of column 0, all classes
+  long long ld, first, classes; // of bias_sums; class of column 0, all classes
   float *bias_sums;
   struct State {
     float weight, lse2;
-    long long label, tile;
+    int label; // column, or behind the last one
   };
-  __device__ __forceinline__ void start(State &s, const DenseProblem &p, long long row, const DenseUnit &, int) const {
+  __device__ __forceinline__ void start(State &s, const DenseProblem &p, int row, const DenseUnit &) const {
     s.weight = s.lse2 = 0.f;
-    s.label = -1;
+    s.label = 0x7fffffff;
     if (row >= p.M) return;
     const long long label = label_at(labels, label_bytes, row);
     if (label < 0 || label >= classes) return; // (its dz are zeros whatever the scores)
-    s.label = label - first;
+    if (label >= first && label < first + p.N) s.label = (int)(label - first);
     s.weight = grad[row] * *scale;
     s.lse2 = lse[row] * kLog2e;
   }
-  __device__ __forceinline__ void tile(State &s, const DenseProblem &p, long long n, unsigned char *mine) const {
-    s.tile = n;
-    stage_bias<T, COLS>(bias, n, p.N, reinterpret_cast<float *>(mine + 2048));
+  __device__ __forceinline__ void tile(const DenseProblem &p, int n, DenseWarp &w) const {
+    stage_bias<T, COLS>(bias, n, p.N, reinterpret_cast<float *>(w.bias));
   }
-  __device__ __forceinline__ void chunk(State &s, const DenseProblem &p, float (&v)[32], long long row, long long n, const DenseUnit &,
-                                        unsigned char *mine) const {
+  __device__ __forceinline__ void ahead(const DenseProblem &, int, int, int, DenseWarp &) const {}
+  __device__ __forceinline__ void chunk(State &s, const DenseProblem &p, const uint32_t (&r)[32], int row, int n, const DenseUnit &,
+                                        DenseWarp &w, bool, bool) const {
     const int lane = threadIdx.x % 32;
-    const float4 *b4 = reinterpret_cast<const float4 *>(mine + 2048) + (n - s.tile) / 4;
-    const bool live = s.weight != 0.f;
-    const float lse2 = s.lse2;
+    unsigned char *mine = w.mine + w.turn;
+    w.turn ^= kOutBytes;
+    const ulonglong2 *b2 = reinterpret_cast<const ulonglong2 *>(w.bias) + n % COLS / 4;
+    const Two less(-s.lse2), weight(s.weight);
+    Two v[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float4 b = b4[j];
-      v[4 * j] = s.weight * exp2_fast(fmaf(v[4 * j], kLog2e, b.x - lse2));
-      v[4 * j + 1] = s.weight * exp2_fast(fmaf(v[4 * j + 1], kLog2e, b.y - lse2));
-      v[4 * j + 2] = s.weight * exp2_fast(fmaf(v[4 * j + 2], kLog2e, b.z - lse2));
-      v[4 * j + 3] = s.weight * exp2_fast(fmaf(v[4 * j + 3], kLog2e, b.w - lse2));
+      const ulonglong2 b = b2[j];
+      Two lo, hi;
+      lo.v = b.x, hi.v = b.y;
+      const float2 x = (fma2(Two(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), Two(kLog2e), lo) + less).get();
+      const float2 y = (fma2(Two(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), Two(kLog2e), hi) + less).get();
+      v[2 * j] = Two(exp2_fast(x.x), exp2_fast(x.y)) * weight;
+      v[2 * j + 1] = Two(exp2_fast(y.x), exp2_fast(y.y)) * weight;
     }
-    if (!live) {
+    if (s.weight == 0.f) { // (a score may be infinite)
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = 0.f;
+      for (int j = 0; j < 16; ++j) v[j] = Two(0.f);
     }
-    const long long at = s.label - n;
-    if (live && at >= 0 && at < 32) {
+    const int at = s.label - n;
+    if (at >= 0 && at < 32) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j == at) v[j] -= s.weight;
+      for (int j = 0; j < 16; ++j) {
+        const float2 x = v[j].get();
+        v[j] = Two(2 * j == at ? x.x - s.weight : x.x, 2 * j + 1 == at ? x.y - s.weight : x.y);
+      }
     }
-    uint4 *q = reinterpret_cast<uint4 *>(mine);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      q[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
-                                                         pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
-    __syncwarp();
-    const long long m0 = row - lane;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + lane / 4, c = lane % 4;
-      if (m0 + r < p.M && n + c * 8 < ld) *reinterpret_cast<uint4 *>(dz + (m0 + r) * ld + n + c * 8) = q[r * 4 + (c ^ ((r >> 1) & 3))];
+    out_free<1>(); // (the other piece's copy may be under way)
+    out_put<T>(mine, v);
+    const int m0 = row - lane;
+    out_ready();
+    if (lane == 0) {
+      if (m0 < p.M) out_send(&dz_map, mine, m0, n);
+      out_commit();
     }
-    __syncwarp();
     if (bias_sums) {
       // sums over the 32 lanes of 32 values each: every step halves the values and doubles the lanes summed
+      float c[32];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 x = v[j].get();
+        c[2 * j] = x.x, c[2 * j + 1] = x.y;
+      }
 #pragma unroll
       for (int d = 16; d; d >>= 1) {
         const bool upper = lane & d;
 #pragma unroll
         for (int j = 0; j < d; ++j) {
-          const float keep = upper ? v[j + d] : v[j], give = upper ? v[j] : v[j + d];
-          v[j] = keep + __shfl_xor_sync(~0u, give, d);
+          const float keep = upper ? c[j + d] : c[j], give = upper ? c[j] : c[j + d];
+          c[j] = keep + __shfl_xor_sync(~0u, give, d);
         }
       }
-      if (m0 < p.M && n + lane < ld) bias_sums[m0 / 32 * ld + n + lane] = v[0];
+      if (m0 < p.M && n + lane < ld) bias_sums[(long long)(m0 / 32) * ld + n + lane] = c[0];
     }
   }
-  __device__ __forceinline__ void stop(State &, const DenseProblem &, long long, const DenseUnit &, int) const {}
+  __device__ __forceinline__ void stop(State &, const DenseProblem &, int, const DenseUnit &, int) const {}
 };
 
 // dz = grad * activation'(pre), rounded; sums of its columns over 32 rows before that.  32 rows x 256 columns
 // a block, four rows a warp, whose loads are under way together.
-template <class T>
-__global__ void __launch_bounds__(256) tb_act_grad_kernel(const T *grad, long long ld_grad, bool vec_grad, const T *pre, long long ld_pre,
-                                                          bool vec_pre, int act, T *dz, long long ld, float *bias_sums, long long rows,
-                                                          long long cols) {
+template <class T> __device__ __forceinline__ uint4 raw8(const T *p, int n, bool vec) { // eight elements, n of them there
+  if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+  uint32_t w[4] = {0, 0, 0, 0};
+  const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) w[i / 2] |= (uint32_t)__ldg(q + i) << (i % 2 * 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class T, int ACT>
+__global__ void __launch_bounds__(256, 4) tb_act_grad_kernel(const T *grad, long long ld_grad, bool vec_grad, const T *pre, long long ld_pre,
+                                                             bool vec_pre, T *dz, long long ld, float *bias_sums, int rows, int cols) {
   __shared__ float part[8][256];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long long c = ((long long)blockIdx.y * 32 + lane) * 8, r0 = (long long)blockIdx.x * 32 + warp * 4;
-  const int have = (int)min(8ll, cols - c);
-  float g[4][8], z[4][8], sum[8] = {};
+  const int c = (blockIdx.y * 32 + lane) * 8, r0 = blockIdx.x * 32 + warp * 4, have = min(8, cols - c);
+  float sum[8] = {};
   if (have > 0) {
+    uint4 g[4], z[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load8(grad + (r0 + i) * ld_grad + c, g[i], r0 + i < rows ? have : 0, vec_grad);
-    if (act) {
+    for (int i = 0; i < 4; ++i) g[i] = raw8(grad + (r0 + i) * ld_grad + c, r0 + i < rows ? have : 0, vec_grad);
+    if constexpr (ACT != kActNone) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load8(pre + (r0 + i) * ld_pre + c, z[i], r0 + i < rows ? have : 0, vec_pre);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) g[i][k] *= act_slope(z[i][k], act);
+      for (int i = 0; i < 4; ++i) z[i] = raw8(pre + (r0 + i) * ld_pre + c, r0 + i < rows ? have : 0, vec_pre);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (r0 + i >= rows) break;
-      store8(dz + (r0 + i) * ld + c, g[i], 8, true); // (ld a multiple of 8)
+      const uint32_t gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w}, zw[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
+      uint32_t o[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum[k] += g[i][k];
+      for (int k = 0; k < 4; ++k) {
+        float2 v = unpack2<T>(gw[k]);
+        if constexpr (ACT != kActNone) {
+          const float2 d = act_slope<ACT>(unpack2<T>(zw[k]));
+          v.x *= d.x, v.y *= d.y;
+        }
+        sum[2 * k] += v.x, sum[2 * k + 1] += v.y;
+        o[k] = pack2<T>(v.x, v.y);
+      }
+      if (r0 + i < rows) *reinterpret_cast<uint4 *>(dz + (r0 + i) * ld + c) = make_uint4(o[0], o[1], o[2], o[3]); // (ld a multiple of 8)
     }
   }
   if (!bias_sums) return;
@@ -781,7 +1041,7 @@ __global__ void __launch_bounds__(256) tb_act_grad_kernel(const T *grad, long lo
   for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = sum[k];
   __syncthreads();
   const int k = threadIdx.x % 8, l = threadIdx.x / 8; // (neighbouring threads have neighbouring columns)
-  const long long at = ((long long)blockIdx.y * 32 + l) * 8 + k;
+  const int at = (blockIdx.y * 32 + l) * 8 + k;
   if (at >= ld) return;
   float s = 0.f;
 #pragma unroll
@@ -789,19 +1049,21 @@ __global__ void __launch_bounds__(256) tb_act_grad_kernel(const T *grad, long lo
   bias_sums[blockIdx.x * ld + at] = s;
 }
 
-// out[c] = sum over `count` rows of sums[., c], times 1 / scale: eight warps take every eighth row each
+// out[c] = sum over `count` rows of sums[., c], times 1 / scale: 32 warps take every 32nd row each
 template <class T>
-__global__ void __launch_bounds__(256) tb_column_sum_kernel(const float *sums, long long count, long long ld, T *out, long long cols, const float *scale) {
-  __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) tb_column_sum_kernel(const float *sums, long long count, long long ld, T *out, long long cols, const float *scale) {
+  __shared__ float part[32][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const long long c = (long long)blockIdx.x * 32 + lane;
   float s = 0.f;
   if (c < cols)
-    for (long long t = warp; t < count; t += 8) s += sums[t * ld + c];
+#pragma unroll 4
+    for (long long t = warp; t < count; t += 32) s += sums[t * ld + c];
   part[warp][lane] = s;
   __syncthreads();
   if (warp || c >= cols) return;
-  for (int i = 1; i < 8; ++i) s += part[i][lane];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) s += part[i][lane];
   out[c] = from_float<T>(scale ? s / *scale : s);
 }
 

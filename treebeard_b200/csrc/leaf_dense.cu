@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 namespace {
@@ -19,30 +20,63 @@ int half_type(int32_t type, const char *what) {
 
 template <class F> int with_half(int32_t type, F f) { return type == TBK_TYPE_F16 ? f(__half()) : f(__nv_bfloat16()); }
 
-// How a product is cut: 256 x 256 tiles of two blocks or 128 x 128 tiles of one, and, where that leaves
-// multiprocessors without work, the sum into parts that a second kernel joins.  Cycles per 64 k of a tile, around
-// a tile and for the second kernel were measured (see tb_dense_kernel); the cheapest cut is taken.
-struct ProductPlan {
-  bool pair = false;
-  int splits = 1;
+// How products are cut: into tiles of one of the three shapes of tb_dense_kernel and, where that leaves
+// multiprocessors without work, the sums into parts that a second kernel joins.  Cycles per 64 k of a tile, around a
+// tile and for the join follow measurements; the cheapest cut of a launch's one or two products is taken.
+struct Size {
+  int64_t m, n, k;
 };
-ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int sms, bool may_split) {
-  ProductPlan best;
+struct Cut {
+  int shape = tb::kDenseOne;
+  int splits[2] = {1, 1};
+};
+Cut plan_products(const Size *sizes, int count, int sms, bool may_split) {
+  static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
+  constexpr double kPer64[] = {700, 750, 1385}, kAround[] = {900, 900, 2900};
+  Cut best;
   double least = 1e300;
-  const int64_t kb = tiles_of(k, 64);
-  for (int pair = 0; pair < 2; ++pair) {
-    const double tiles = (double)tiles_of(m, pair ? 256 : 128) * tiles_of(n, pair ? 256 : 128), slots = pair ? sms / 2 : sms;
-    for (int64_t splits = 1; splits <= (may_split ? std::min<int64_t>(kb, 32) : 1); ++splits) {
-      double cost = std::ceil(tiles * splits / slots) * (tiles_of(kb, splits) * (pair ? 530.0 : 300.0) + (pair ? 1400 : 900)) + 2500;
-      if (splits > 1) cost += 5000 + (double)m * n * 8 * splits / 2500;
-      if (cost < least) least = cost, best.pair = pair, best.splits = (int)splits;
+  for (int shape = 0; shape < 3; ++shape) {
+    const int64_t slots = shape == tb::kDenseOne ? sms : sms / 2;
+    double tiles[2] = {}, kb[2] = {};
+    for (int i = 0; i < count; ++i) {
+      tiles[i] = (double)tiles_of(sizes[i].m, tb::dense_rows(shape)) * tiles_of(sizes[i].n, tb::dense_cols(shape));
+      kb[i] = (double)tiles_of(sizes[i].k, 64);
+    }
+    for (const int s0 : kSplits) {
+      if (s0 > 1 && (!may_split || s0 > kb[0])) break;
+      for (const int s1 : kSplits) {
+        if (s1 > 1 && (!may_split || count < 2 || s1 > kb[1])) break;
+        const int s[2] = {s0, s1};
+        double per[2] = {}, join = 0;
+        int64_t units[2] = {};
+        for (int i = 0; i < count; ++i) {
+          per[i] = std::ceil(kb[i] / s[i]) * kPer64[shape] + kAround[shape];
+          units[i] = (int64_t)tiles[i] * s[i];
+          if (s[i] > 1) join += 5000 + (double)sizes[i].m * sizes[i].n * 8 * s[i] / 2500;
+        }
+        // slot i has units i, i + slots, ... of both products' one after the other: some slots have one more of the
+        // first's, some one more in all
+        const int64_t all = units[0] + units[1], a = units[0] / slots, ra = units[0] % slots, b = all / slots, rb = all % slots;
+        auto load = [&](int64_t of_first, int64_t of_all) { return of_first * per[0] + (of_all - of_first) * per[1]; };
+        double cost = 0;
+        if (ra > 0 && rb > 0) cost = std::max(cost, load(a + 1, b + 1));
+        if (rb > ra) cost = std::max(cost, load(a, b + 1));
+        if (ra > rb) cost = std::max(cost, load(a + 1, b));
+        if (std::max(ra, rb) < slots) cost = std::max(cost, load(a, b));
+        cost += join;
+        if (cost < least) least = cost, best.shape = shape, best.splits[0] = s0, best.splits[1] = s1;
+      }
     }
   }
   return best;
 }
-uint64_t part_floats(int64_t m, int64_t n, int64_t k, int sms) {
-  const ProductPlan plan = plan_product(m, n, k, sms, true);
-  return plan.splits > 1 ? (uint64_t)plan.splits * m * up8(n) : 0;
+// fp32 room for the parts of a launch's products
+uint64_t part_floats(const Size *sizes, int count, int sms) {
+  const Cut cut = plan_products(sizes, count, sms, true);
+  uint64_t sum = 0;
+  for (int i = 0; i < count; ++i)
+    if (cut.splits[i] > 1) sum += (uint64_t)cut.splits[i] * sizes[i].m * up8(sizes[i].n);
+  return sum;
 }
 
 // An operand of a product: rows x sum matrix at p, row-major, or (rows_inner) sum x rows.
@@ -63,61 +97,99 @@ EncodeTiled encode_tiled() {
   }();
   return f;
 }
-template <class T> int tensor_map(CUtensorMap *map, const Side &s, int64_t rows, int64_t k) {
+template <class T> int encode_map(CUtensorMap *map, const void *p, int64_t inner, int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return fail(TBK_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-  const int64_t inner = s.rows_inner ? rows : k, outer = s.rows_inner ? k : rows;
-  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)(outer > 1 ? s.ld : up8(inner)) * 2};
-  const cuuint32_t box[2] = {64, s.rows_inner ? 64u : 128u}, one[2] = {1, 1};
-  const CUresult rc = encode(map, sizeof(T) == 2 && std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                             const_cast<void *>(s.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return rc == CUDA_SUCCESS ? TBK_OK : fail(TBK_ERR_CUDA, "cuTensorMapEncodeTiled: %d (%lld x %lld, %lld)", (int)rc, (long long)outer, (long long)inner, (long long)s.ld);
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer}, strides[1] = {(cuuint64_t)(outer > 1 ? ld : up8(inner)) * 2};
+  const cuuint32_t box[2] = {box_inner, box_outer}, one[2] = {1, 1};
+  const CUresult rc = encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(p),
+                             dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? TBK_OK : fail(TBK_ERR_CUDA, "cuTensorMapEncodeTiled: %d (%lld x %lld, %lld)", (int)rc, (long long)outer, (long long)inner, (long long)ld);
 }
+template <class T> int side_map(CUtensorMap *map, const Side &s, int64_t rows, int64_t k) {
+  return encode_map<T>(map, s.p, s.rows_inner ? rows : k, s.rows_inner ? k : rows, s.ld, 64, s.rows_inner ? 64 : 128);
+}
+// Where a warp's 32 rows and columns of a result go.
+template <class T> int out_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64_t ld) { return encode_map<T>(map, p, cols, rows, ld, 32, 32); }
 
-template <class T, bool PAIR, class End>
-int launch_dense(const Side &a, const Side &b, int64_t m, int64_t n, int64_t k, int splits, int run, int sms, const End &end, cudaStream_t stream) {
-  constexpr int tile = PAIR ? 256 : 128;
-  tb::DenseProblem p;
-  TRY(tensor_map<T>(&p.a, a, m, k));
-  TRY(tensor_map<T>(&p.b, b, n, k));
-  p.M = m, p.N = n;
-  p.a_rows_inner = a.rows_inner, p.b_rows_inner = b.rows_inner;
-  p.m_tiles = (int)tiles_of(m, tile), p.n_tiles = (int)tiles_of(n, tile), p.k_blocks = (int)tiles_of(k, 64);
-  const int64_t slots = PAIR ? sms / 2 : sms;
-  p.chunk = run;
-  p.chunks = (int)tiles_of(p.n_tiles, p.chunk);
-  p.splits = splits;
-  p.group = PAIR ? 8 : 16;
-  p.units = (long long)p.m_tiles * p.chunks * splits;
+template <class T> int set_problem(tb::DenseProblem *p, int shape, const Side &a, const Side &b, const Size &size, int splits, int run) {
+  TRY(side_map<T>(&p->a, a, size.m, size.k));
+  TRY(side_map<T>(&p->b, b, size.n, size.k));
+  p->M = (int)size.m, p->N = (int)size.n;
+  p->a_rows_inner = a.rows_inner, p->b_rows_inner = b.rows_inner;
+  p->m_tiles = (int)tiles_of(size.m, tb::dense_rows(shape)), p->n_tiles = (int)tiles_of(size.n, tb::dense_cols(shape));
+  p->k_blocks = (int)tiles_of(size.k, 64);
+  p->chunk = run;
+  p->chunks = (int)tiles_of(p->n_tiles, run);
+  p->splits = splits;
+  p->group = shape == tb::kDenseOne ? 16 : shape == tb::kDensePair ? 8 : 4;
+  const int64_t units = (int64_t)p->m_tiles * p->chunks * splits;
+  if (units > 1 << 30) return fail(TBK_ERR_UNSUPPORTED, "a product of %lld x %lld", (long long)size.m, (long long)size.n);
+  p->units = (int)units;
+  return TBK_OK;
+}
+// Launches what stands in jobs.p, jobs.end.
+template <class T, int SHAPE, class End, int JOBS> int launch_shape(const tb::DenseJobs<End, JOBS> &jobs, int slots, cudaStream_t stream) {
   static std::atomic<uint64_t> ready{0}; // devices on which the kernel may use its shared memory
+  constexpr int smem = tb::dense_smem_bytes(SHAPE);
+  const auto kernel = tb::tb_dense_kernel<T, SHAPE, End, JOBS>;
   int device = 0;
   CUDA_TRY(cudaGetDevice(&device));
   if (device > 63 || !(ready.load() >> device & 1)) {
-    CUDA_TRY(cudaFuncSetAttribute(tb::tb_dense_kernel<T, PAIR, End>, cudaFuncAttributeMaxDynamicSharedMemorySize, tb::kDenseSmem));
+    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (device <= 63) ready.fetch_or(1ull << device);
   }
-  const unsigned grid = (unsigned)std::min<int64_t>(p.units, slots) * (PAIR ? 2 : 1);
-  tb::tb_dense_kernel<T, PAIR, End><<<grid, tb::kDenseThreads, tb::kDenseSmem, stream>>>(p, end);
+  const unsigned grid = (unsigned)std::min(jobs.units, slots) * (SHAPE == tb::kDenseOne ? 1 : 2);
+  kernel<<<grid, tb::kDenseThreads, smem, stream>>>(jobs);
   CUDA_TRY(cudaGetLastError());
   return TBK_OK;
 }
+template <class T, class End, int JOBS> int launch_jobs(int shape, tb::DenseJobs<End, JOBS> &jobs, int sms, cudaStream_t stream) {
+  jobs.units = jobs.p[0].units + (JOBS > 1 ? jobs.p[JOBS - 1].units : 0);
+  return shape == tb::kDenseOne    ? launch_shape<T, tb::kDenseOne, End, JOBS>(jobs, sms, stream)
+         : shape == tb::kDensePair ? launch_shape<T, tb::kDensePair, End, JOBS>(jobs, sms / 2, stream)
+                                   : launch_shape<T, tb::kDenseTall, End, JOBS>(jobs, sms / 2, stream);
+}
+// The first `count` products of two.
+template <class T, class End> int launch_some(int shape, tb::DenseJobs<End, 2> &jobs, int count, int sms, cudaStream_t stream) {
+  if (count == 2) return launch_jobs<T, End, 2>(shape, jobs, sms, stream);
+  tb::DenseJobs<End, 1> one;
+  one.p[0] = jobs.p[0], one.end[0] = jobs.end[0];
+  return launch_jobs<T, End, 1>(shape, one, sms, stream);
+}
 
-// C[m, n] = sum_k A[m, k] B[n, k], finished by F.  parts: room for what part_floats says.
-template <class T, class F>
-int product(const Side &a, const Side &b, int64_t m, int64_t n, int64_t k, const F &f, float *parts, int sms, cudaStream_t stream) {
-  const ProductPlan plan = plan_product(m, n, k, sms, true);
-  if (plan.splits == 1) {
-    const tb::WholeEnd<F> end{f};
-    return plan.pair ? launch_dense<T, true>(a, b, m, n, k, 1, 1, sms, end, stream)
-                     : launch_dense<T, false>(a, b, m, n, k, 1, 1, sms, end, stream);
+// A launch's product: C[m, n] = sum_k A[m, k] B[n, k], finished by `end`.
+template <class T> struct Product {
+  Side a, b;
+  Size size;
+  tb::Result<T> end;
+};
+// One or two products, which do not depend on one another.  parts: room for what part_floats says.
+template <class T> int products(const Product<T> *list, int count, float *parts, int sms, cudaStream_t stream) {
+  Size sizes[2];
+  for (int i = 0; i < count; ++i) sizes[i] = list[i].size;
+  const Cut cut = plan_products(sizes, count, sms, true);
+  tb::DenseJobs<tb::ResultEnd<T>, 2> jobs;
+  float *room[2] = {};
+  for (int i = 0; i < count; ++i) {
+    const Product<T> &x = list[i];
+    TRY(set_problem<T>(&jobs.p[i], cut.shape, x.a, x.b, x.size, cut.splits[i], 1));
+    jobs.end[i].f = x.end;
+    if (cut.splits[i] == 1) continue;
+    room[i] = parts;
+    jobs.end[i].f.parts = parts, jobs.end[i].f.ld_parts = up8(x.size.n);
+    jobs.end[i].f.sends = false;
+    parts += (uint64_t)cut.splits[i] * x.size.m * up8(x.size.n);
   }
-  const int64_t ld = up8(n);
-  const tb::PartEnd end{parts, ld};
-  if (plan.pair) TRY((launch_dense<T, true>(a, b, m, n, k, plan.splits, 1, sms, end, stream)));
-  else TRY((launch_dense<T, false>(a, b, m, n, k, plan.splits, 1, sms, end, stream)));
-  tb::tb_dense_join_kernel<F><<<(unsigned)tiles_of(m * (ld / 8), 256), 256, 0, stream>>>(parts, plan.splits, ld, m, n, f);
-  CUDA_TRY(cudaGetLastError());
+  TRY((launch_some<T, tb::ResultEnd<T>>(cut.shape, jobs, count, sms, stream)));
+  for (int i = 0; i < count; ++i) {
+    if (cut.splits[i] == 1) continue;
+    const Size &z = list[i].size;
+    const int64_t ld = up8(z.n);
+    tb::tb_dense_join_kernel<T><<<(unsigned)tiles_of(z.m * (ld / 8), 256), 256, 0, stream>>>(room[i], cut.splits[i], ld, z.m, z.n, list[i].end);
+    CUDA_TRY(cudaGetLastError());
+  }
   return TBK_OK;
 }
 
@@ -137,6 +209,22 @@ template <class T> int readable(const void **p, int64_t *ld, int64_t rows, int64
 // Whether 16 bytes at a time can be read or written at every eighth column.
 bool vec_rows(const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 
+// Where a product's whole sums go: out = sum / *scale + addend, before an activation and a bias are set.
+template <class T>
+int set_result(tb::Result<T> *end, void *out, int64_t ld, int64_t rows, int64_t cols, const void *addend, int64_t ld_addend, void *pre, int64_t ld_pre) {
+  std::memset(static_cast<void *>(end), 0, sizeof *end);
+  end->out = (T *)out, end->ld_out = ld, end->vec_out = vec_rows(out, ld);
+  end->addend = (const T *)addend, end->ld_addend = ld_addend, end->vec_addend = vec_rows(addend, ld_addend);
+  end->pre = (T *)pre, end->ld_pre = ld_pre, end->vec_pre = vec_rows(pre, ld_pre);
+  end->first = end->last = true;
+  end->sends = tma_rows(out, ld, rows) && (!addend || tma_rows(addend, ld_addend, rows)) && (!pre || tma_rows(pre, ld_pre, rows));
+  if (!end->sends) return TBK_OK;
+  TRY(out_map<T>(&end->out_map, out, rows, cols, ld));
+  if (addend) TRY(out_map<T>(&end->addend_map, addend, rows, cols, ld_addend));
+  if (pre) TRY(out_map<T>(&end->pre_map, pre, rows, cols, ld_pre));
+  return TBK_OK;
+}
+
 typedef unsigned short Half; // an element of either 16-bit type
 
 struct LinearParts {
@@ -144,7 +232,10 @@ struct LinearParts {
   float *parts;
   LinearParts(Parts &w, int64_t n, int64_t inputs, int64_t outputs, bool aligned, int sms)
       : x(w.take<Half>(aligned ? 0 : n * up8(inputs))), weight(w.take<Half>(aligned ? 0 : outputs * up8(inputs))),
-        parts(w.take<float>(part_floats(n, outputs, inputs, sms))) {}
+        parts(nullptr) {
+    const Size size{n, outputs, inputs};
+    parts = w.take<float>(n > 0 ? part_floats(&size, 1, sms) : 0);
+  }
 };
 struct LinearGradParts {
   int64_t ld;
@@ -153,22 +244,24 @@ struct LinearGradParts {
   LinearGradParts(Parts &w, int64_t n, int64_t inputs, int64_t outputs, bool aligned, int sms)
       : ld(up8(outputs)), x(w.take<Half>(aligned ? 0 : n * up8(inputs))), weight(w.take<Half>(aligned ? 0 : outputs * up8(inputs))),
         dz(w.take<Half>(n * ld)), bias_sums(w.take<float>(tiles_of(n, 32) * ld)),
-        parts(w.take<float>(std::max(part_floats(n, inputs, outputs, sms), part_floats(outputs, inputs, n, sms)))) {}
+        parts(nullptr) {
+    const Size both[2] = {{n, inputs, outputs}, {outputs, inputs, n}};
+    if (n > 0) parts = w.take<float>(std::max({part_floats(both, 2, sms), part_floats(both, 1, sms), part_floats(both + 1, 1, sms)}));
+  }
 };
 
 // How the scores of a loss are cut: a unit goes through a run of column tiles, as long as every slot still gets
 // eight units, so that the last ones end together.
 struct LossCut {
-  bool pair;
-  int run, parts; // column tiles of a unit; partial sums of a row
+  int shape, run, parts; // column tiles of a unit; partial sums of a row
   LossCut(int64_t n, int64_t width, int64_t classes, int sms) {
-    pair = plan_product(n, classes, width, sms, false).pair;
-    const int64_t tile = pair ? 256 : 128, slots = pair ? sms / 2 : sms, cols = tiles_of(classes, tile);
-    run = (int)std::clamp<int64_t>(tiles_of(n, tile) * cols / (8 * slots), 1, 8);
-    parts = 2 * (int)tiles_of(cols, run);
+    const Size size{n, classes, width};
+    shape = plan_products(&size, 1, sms, false).shape;
+    const int64_t slots = shape == tb::kDenseOne ? sms : sms / 2, cols = tiles_of(classes, tb::dense_cols(shape));
+    run = (int)std::clamp<int64_t>(tiles_of(n, tb::dense_rows(shape)) * cols / (8 * slots), 1, 8);
+    parts = 4 * (int)tiles_of(cols, run);
   }
 };
-
 struct LossParts {
   LossCut cut;
   Half *x, *weight;
@@ -179,9 +272,9 @@ struct LossParts {
         part(w.take<float2>((uint64_t)n * cut.parts)), at(w.take<float>(n)) {}
 };
 
-// Classes of a piece of dz: about 64 MB, so that a piece that has just been written is read from L2.
+// Classes of a piece of dz, which is about 256 MB: enough tiles to fill the multiprocessors evenly.
 int64_t piece_classes(int64_t n, int64_t classes) {
-  const int64_t fits = ((int64_t)32 << 20) / std::max<int64_t>(1, n) / 256 * 256;
+  const int64_t fits = ((int64_t)128 << 20) / std::max<int64_t>(1, n) / 256 * 256;
   return std::min(up8(classes), std::max<int64_t>(256, fits));
 }
 struct LossGradParts {
@@ -195,7 +288,10 @@ struct LossGradParts {
         bias_sums(w.take<float>(tiles_of(n, 32) * piece)), sums(w.take<float>(piece < classes ? n * ld_sums : 0)) {
     uint64_t most = 0; // of a full piece's products and the last one's
     for (const int64_t now : {std::min(piece, classes), (classes - 1) % piece + 1})
-      if (n > 0) most = std::max({most, part_floats(n, width, now, sms), part_floats(now, width, n, sms)});
+      if (n > 0) {
+        const Size both[2] = {{n, width, now}, {now, width, n}};
+        most = std::max({most, part_floats(both, 2, sms), part_floats(both, 1, sms), part_floats(both + 1, 1, sms)});
+      }
     parts = w.take<float>(most);
   }
 };
@@ -238,9 +334,11 @@ int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64_t ld_w, co
     LinearParts parts(w, n, inputs, outputs, aligned, sms);
     TRY(readable(&x, &ld_x, n, inputs, (T *)parts.x, stream));
     TRY(readable(&weight, &ld_w, outputs, inputs, (T *)parts.weight, stream));
-    const tb::LinearEnd<T> end{(const T *)bias, (const T *)residual, (T *)out, (T *)pre, ld_res, ld_out, ld_pre, act,
-                               vec_rows(residual, ld_res), vec_rows(out, ld_out), vec_rows(pre, ld_pre), vec_rows(bias, 0)};
-    return product<T>({x, ld_x, false}, {weight, ld_w, false}, n, outputs, inputs, end, parts.parts, sms, stream);
+    Product<T> product{{x, ld_x, false}, {weight, ld_w, false}, {n, outputs, inputs}, {}};
+    TRY(set_result<T>(&product.end, out, ld_out, n, outputs, residual, ld_res, pre, ld_pre));
+    product.end.bias = (const T *)bias, product.end.vec_bias = vec_rows(bias, 0);
+    product.end.act = act;
+    return products<T>(&product, 1, parts.parts, sms, stream);
   });
 }
 
@@ -292,23 +390,35 @@ int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_
     T *dz = (T *)parts.dz;
     if (grad_w) TRY(readable(&x, &ld_x, n, inputs, (T *)parts.x, stream));
     if (grad_x) TRY(readable(&weight, &ld_w, outputs, inputs, (T *)parts.weight, stream));
-    tb::tb_act_grad_kernel<T><<<dim3((unsigned)tiles_of(n, 32), (unsigned)tiles_of(outputs, 256)), 256, 0, stream>>>(
-        (const T *)grad, ld_grad, vec_rows(grad, ld_grad), (const T *)pre, ld_pre, vec_rows(pre, ld_pre), act, dz, parts.ld,
-        grad_b ? parts.bias_sums : nullptr, n, outputs);
+    auto slopes = [&](auto a) {
+      tb::tb_act_grad_kernel<T, decltype(a)::value><<<dim3((unsigned)tiles_of(n, 32), (unsigned)tiles_of(outputs, 256)), 256, 0, stream>>>(
+          (const T *)grad, ld_grad, vec_rows(grad, ld_grad), (const T *)pre, ld_pre, vec_rows(pre, ld_pre), dz, parts.ld,
+          grad_b ? parts.bias_sums : nullptr, (int)n, (int)outputs);
+    };
+    switch (act) {
+    case TBK_ACT_RELU: slopes(std::integral_constant<int, tb::kActRelu>()); break;
+    case TBK_ACT_GELU: slopes(std::integral_constant<int, tb::kActGelu>()); break;
+    case TBK_ACT_SILU: slopes(std::integral_constant<int, tb::kActSilu>()); break;
+    default: slopes(std::integral_constant<int, tb::kActNone>());
+    }
     CUDA_TRY(cudaGetLastError());
     if (grad_b) {
-      tb::tb_column_sum_kernel<T><<<(unsigned)tiles_of(outputs, 32), 256, 0, stream>>>(parts.bias_sums, tiles_of(n, 32), parts.ld, (T *)grad_b, outputs, nullptr);
+      tb::tb_column_sum_kernel<T><<<(unsigned)tiles_of(outputs, 32), 1024, 0, stream>>>(parts.bias_sums, tiles_of(n, 32), parts.ld, (T *)grad_b, outputs, nullptr);
       CUDA_TRY(cudaGetLastError());
     }
+    Product<T> list[2];
+    int count = 0;
     if (grad_x) {
-      const tb::SumEnd<T> end{nullptr, 0, (T *)grad_x, (const T *)skip, ld_gx, ld_skip, nullptr, true, true, vec_rows(grad_x, ld_gx), vec_rows(skip, ld_skip)};
-      TRY((product<T>({dz, parts.ld, false}, {weight, ld_w, true}, n, inputs, outputs, end, parts.parts, sms, stream)));
+      Product<T> &q = list[count++];
+      q.a = {dz, parts.ld, false}, q.b = {weight, ld_w, true}, q.size = {n, inputs, outputs};
+      TRY(set_result<T>(&q.end, grad_x, ld_gx, n, inputs, skip, ld_skip, nullptr, 0));
     }
     if (grad_w) {
-      const tb::SumEnd<T> end{nullptr, 0, (T *)grad_w, nullptr, ld_gw, 0, nullptr, true, true, vec_rows(grad_w, ld_gw), false};
-      TRY((product<T>({dz, parts.ld, true}, {x, ld_x, true}, outputs, inputs, n, end, parts.parts, sms, stream)));
+      Product<T> &q = list[count++];
+      q.a = {dz, parts.ld, true}, q.b = {x, ld_x, true}, q.size = {outputs, inputs, n};
+      TRY(set_result<T>(&q.end, grad_w, ld_gw, outputs, inputs, nullptr, 0, nullptr, 0));
     }
-    return (int)TBK_OK;
+    return count ? products<T>(list, count, parts.parts, sms, stream) : (int)TBK_OK;
   });
 }
 
@@ -351,13 +461,15 @@ int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_w
     TRY(readable(&x, &ld_x, n, width, (T *)parts.x, stream));
     TRY(readable(&weight, &ld_w, classes, width, (T *)parts.weight, stream));
     const Side a{x, ld_x, false}, b{weight, ld_w, false};
-    if (parts.cut.pair) {
-      const tb::LseEnd<T, 128> end{(const T *)bias, labels, label_bytes, parts.part, parts.at};
-      TRY((launch_dense<T, true>(a, b, n, classes, width, 1, parts.cut.run, sms, end, stream)));
-    } else {
-      const tb::LseEnd<T, 64> end{(const T *)bias, labels, label_bytes, parts.part, parts.at};
-      TRY((launch_dense<T, false>(a, b, n, classes, width, 1, parts.cut.run, sms, end, stream)));
-    }
+    auto scores = [&](auto cols) {
+      using End = tb::LseEnd<T, decltype(cols)::value>;
+      tb::DenseJobs<End, 1> jobs;
+      TRY(set_problem<T>(&jobs.p[0], parts.cut.shape, a, b, {n, classes, width}, 1, parts.cut.run));
+      jobs.end[0] = {(const T *)bias, labels, label_bytes, parts.part, parts.at};
+      return launch_jobs<T, End, 1>(parts.cut.shape, jobs, sms, stream);
+    };
+    if (parts.cut.shape == tb::kDenseOne) TRY(scores(std::integral_constant<int, 32>()));
+    else TRY(scores(std::integral_constant<int, 64>()));
     tb::tb_loss_join_kernel<<<(unsigned)tiles_of(n, 32), 32 * tb::kJoinWarps, 0, stream>>>(parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss, lse, n);
     CUDA_TRY(cudaGetLastError());
     return (int)TBK_OK;
@@ -412,26 +524,44 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
       const Side xs{x, ld_x, false}, ws_{W + v * ld_w, ld_w, false};
       const T *b = bias ? (const T *)bias + v : nullptr;
       float *sums = grad_b ? parts.bias_sums : nullptr;
-      if (plan_product(n, now, width, sms, false).pair) {
-        const tb::ScoreGradEnd<T, 128> end{b, labels, label_bytes, grad, lse, parts.scale, dz, ld, v, classes, sums};
-        TRY((launch_dense<T, true>(xs, ws_, n, now, width, 1, 1, sms, end, stream)));
-      } else {
-        const tb::ScoreGradEnd<T, 64> end{b, labels, label_bytes, grad, lse, parts.scale, dz, ld, v, classes, sums};
-        TRY((launch_dense<T, false>(xs, ws_, n, now, width, 1, 1, sms, end, stream)));
-      }
+      CUtensorMap dz_map;
+      TRY(out_map<T>(&dz_map, dz, n, now, ld));
+      const Size size{n, now, width};
+      const int shape = plan_products(&size, 1, sms, false).shape;
+      auto gradients = [&](auto cols) {
+        using End = tb::ScoreGradEnd<T, decltype(cols)::value>;
+        tb::DenseJobs<End, 1> jobs;
+        TRY(set_problem<T>(&jobs.p[0], shape, xs, ws_, size, 1, 1));
+        jobs.end[0] = {dz_map, b, labels, label_bytes, grad, lse, parts.scale, ld, v, classes, sums};
+        return launch_jobs<T, End, 1>(shape, jobs, sms, stream);
+      };
+      if (shape == tb::kDenseOne) TRY(gradients(std::integral_constant<int, 32>()));
+      else TRY(gradients(std::integral_constant<int, 64>()));
       if (grad_b) {
-        tb::tb_column_sum_kernel<T><<<(unsigned)tiles_of(now, 32), 256, 0, stream>>>(parts.bias_sums, tiles_of(n, 32), ld, (T *)grad_b + v, now, parts.scale);
+        tb::tb_column_sum_kernel<T><<<(unsigned)tiles_of(now, 32), 1024, 0, stream>>>(parts.bias_sums, tiles_of(n, 32), ld, (T *)grad_b + v, now, parts.scale);
         CUDA_TRY(cudaGetLastError());
       }
+      Product<T> list[2];
+      int count = 0;
       if (grad_x) {
-        const tb::SumEnd<T> end{parts.sums, parts.ld_sums, (T *)grad_x, nullptr, ld_gx, 0, parts.scale, v == 0, v + now == classes, vec_rows(grad_x, ld_gx), false};
-        TRY((product<T>({dz, ld, false}, {W + v * ld_w, ld_w, true}, n, width, now, end, parts.parts, sms, stream)));
+        Product<T> &q = list[count++];
+        q.a = {dz, ld, false}, q.b = {W + v * ld_w, ld_w, true}, q.size = {n, width, now};
+        TRY(set_result<T>(&q.end, grad_x, ld_gx, n, width, nullptr, 0, nullptr, 0));
+        q.end.scale = parts.scale;
+        if (ld < classes) { // (several pieces)
+          q.end.sums = parts.sums, q.end.ld_sums = parts.ld_sums, q.end.sends = false;
+          q.end.first = v == 0, q.end.last = v + now == classes;
+          q.end.vec_out = q.end.vec_out || !q.end.last; // (the sums are aligned)
+        }
       }
       if (grad_w) {
+        Product<T> &q = list[count++];
         T *to = (T *)grad_w + v * ld_gw;
-        const tb::SumEnd<T> end{nullptr, 0, to, nullptr, ld_gw, 0, parts.scale, true, true, vec_rows(to, ld_gw), false};
-        TRY((product<T>({dz, ld, true}, {x, ld_x, true}, now, width, n, end, parts.parts, sms, stream)));
+        q.a = {dz, ld, true}, q.b = {x, ld_x, true}, q.size = {now, width, n};
+        TRY(set_result<T>(&q.end, to, ld_gw, now, width, nullptr, 0, nullptr, 0));
+        q.end.scale = parts.scale;
       }
+      if (count) TRY(products<T>(list, count, parts.parts, sms, stream));
     }
     return (int)TBK_OK;
   });
