@@ -223,6 +223,7 @@ __global__ void __cluster_dims__(SHAPE == kDenseOne ? 1 : 2, 1, 1) __launch_boun
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+  after_previous_kernel();
 
   bool ok = true;
   if (warp == 0) {
@@ -535,6 +536,16 @@ template <class T> __device__ __forceinline__ void load8(const T *p, float (&v)[
   }
 }
 
+template <class T> __device__ __forceinline__ uint4 raw8(const T *p, int n, bool vec) { // eight elements as they are, n of them there
+  if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+  uint32_t w[4] = {0, 0, 0, 0};
+  const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) w[i / 2] |= (uint32_t)__ldg(q + i) << (i % 2 * 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Results on their way out: a warp puts 32 rows x 32 columns (a row is 64 bytes, its 16-byte pieces swapped
 // around by the row's number, as the tensor map says) into its shared memory and one tensor copy takes them to
 // where they belong; what is behind the last row or column the copy leaves out.
@@ -565,7 +576,7 @@ __device__ __forceinline__ void out_send(const CUtensorMap *map, const unsigned 
 __device__ __forceinline__ void out_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // 32 rows x 32 fp32 values turned around in shared memory, 16-byte pieces swapped around by the row's number,
-// which keeps both directions free of bank conflicts.  f(row, column 0, 8, 16 or 24, eight values) ...
+// which keeps both directions free of bank conflicts.  f(row, column 0, 8, 16 or 24, eight values).
 __device__ __forceinline__ void turn(const uint32_t (&r)[32], unsigned char *mine) {
   const int lane = threadIdx.x % 32;
   uint4 *s = reinterpret_cast<uint4 *>(mine);
@@ -574,11 +585,10 @@ __device__ __forceinline__ void turn(const uint32_t (&r)[32], unsigned char *min
   for (int i = 0; i < 8; ++i) s[lane * 8 + (i ^ (lane & 7))] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
   __syncwarp();
 }
-template <class F> __device__ __forceinline__ void turned(const uint32_t (&r)[32], unsigned char *mine, F f) {
-  turn(r, mine);
+template <class F> __device__ __forceinline__ void turned(const unsigned char *mine, F f) {
   const int lane = threadIdx.x % 32;
   const float4 *s = reinterpret_cast<const float4 *>(mine);
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < 4; ++i) {
     const int row = i * 8 + lane / 4, c = lane % 4;
     const float4 x = s[row * 8 + ((2 * c) ^ (row & 7))], y = s[row * 8 + ((2 * c + 1) ^ (row & 7))];
@@ -586,21 +596,38 @@ template <class F> __device__ __forceinline__ void turned(const uint32_t (&r)[32
     f(row, c * 8, w);
   }
 }
-// ... or f(row, value of the lane's column), for results whose rows begin anywhere: a warp then writes 32
-// neighbouring elements at a time.
-template <class F> __device__ __forceinline__ void turned_columns(const uint32_t (&r)[32], unsigned char *mine, F f) {
-  turn(r, mine);
+
+// The same pieces of 32 rows x 32 columns to and from matrices whose rows begin anywhere, which tensor copies cannot
+// reach: a lane per column, 32 neighbouring elements at a time.  (Calls, as everything that few products need, so
+// that the way of the others stays short: their instructions come from a small cache.)
+template <class T> __device__ __forceinline__ T *out_element(unsigned char *buf, int row) {
   const int lane = threadIdx.x % 32;
-  const float *w = reinterpret_cast<const float *>(mine) + lane % 4;
+  return reinterpret_cast<T *>(buf) + row * 32 + (((lane >> 3) ^ (row >> 1 & 3)) << 3 | (lane & 7));
+}
+template <class T> __device__ __noinline__ void copy_out(T *to, long long ld, int m0, int n, int M, int N, unsigned char *buf) {
+  __syncwarp();
+  if (n + (int)(threadIdx.x % 32) < N) {
+    T *p = to + (long long)m0 * ld + n + threadIdx.x % 32;
+    const int rows = min(32, M - m0);
 #pragma unroll 8
-  for (int row = 0; row < 32; ++row) f(row, w[(row * 8 + ((lane / 4) ^ (row & 7))) * 4]);
+    for (int r = 0; r < rows; ++r) p[r * ld] = *out_element<T>(buf, r);
+  }
+  __syncwarp();
+}
+template <class T> __device__ __noinline__ void copy_in(const T *from, long long ld, int m0, int n, int M, int N, unsigned char *buf) {
+  __syncwarp();
+  const bool there = n + (int)(threadIdx.x % 32) < N;
+  const T *p = from + (long long)m0 * ld + n + threadIdx.x % 32;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) *out_element<T>(buf, r) = there && m0 + r < M ? p[r * ld] : from_float<T>(0.f);
+  __syncwarp();
 }
 
 // What a whole sum c becomes: z = c / scale + bias; out = activation(z) + addend; pre = z.  Or, with `sums`, one
 // piece of a longer sum, added to the pieces before it.  With `parts` the sum is cut into parts, which are kept:
 // parts[split][row][ld_parts].
 template <class T> struct Result {
-  CUtensorMap out_map, pre_map, addend_map; // where `sends`
+  CUtensorMap out_map, pre_map, addend_map; // where the matrix's rows lie at multiples of 16 bytes (tma_*)
   const T *bias, *addend;
   T *out, *pre;
   float *sums; // [rows][ld_sums] or null
@@ -609,23 +636,8 @@ template <class T> struct Result {
   long long ld_addend, ld_out, ld_pre, ld_sums, ld_parts;
   int act;
   bool first, last;                                   // piece of a sum
-  bool sends, vec_addend, vec_out, vec_pre, vec_bias; // rows lie at multiples of 16 bytes
-  __device__ __forceinline__ void finish1(float c, long long m, long long n) const {
-    if (sums) {
-      float *s = sums + m * ld_sums + n;
-      if (!first) c += *s;
-      if (!last) {
-        *s = c;
-        return;
-      }
-    }
-    if (scale) c *= 1.f / *scale;
-    const float z = bias ? c + to_float(bias[n]) : c;
-    if (pre) pre[m * ld_pre + n] = from_float<T>(z);
-    float y = z;
-    with_act(act, [&](auto a) { y = act_value<decltype(a)::value>(make_float2(z, z)).x; });
-    out[m * ld_out + n] = from_float<T>(addend ? y + to_float(addend[m * ld_addend + n]) : y);
-  }
+  bool tma_addend, tma_out, tma_pre;                  // tensor copies reach the matrix
+  bool vec_addend, vec_out, vec_pre, vec_bias;        // every eighth column lies at a multiple of 16 bytes
   __device__ __forceinline__ void finish8(const float (&c)[8], long long m, long long n, long long N) const {
     const int have = (int)min(8ll, N - n);
     float z[8], b[8];
@@ -670,17 +682,28 @@ template <class T> struct Result {
   }
 };
 
-// Finishes sums.  Where all matrices' rows lie at multiples of 16 bytes (`sends`) a lane keeps its row: addends
-// come, and results go, 32 rows x 32 columns at a time by tensor copies.  (Reading them a row per lane took longer
-// than the product.)  A warp has two pieces of 2 KB, which results go through by turns; addends come there, one
-// for each half of the warp's columns, before the sums are done, and the results replace them; where z is kept too,
-// the second is z's.
+// A warp's 32 x 32 sums, turned around in its shared memory, to where parts or pieces of sums are kept.
+template <class T> __device__ __noinline__ void keep_sums(const Result<T> &f, const unsigned char *mine, int m0, int n, int M, int N, int split) {
+  turned(mine, [&](int k, int c, const float (&x)[8]) {
+    if (m0 + k >= M || n + c >= N) return;
+    if (!f.parts) return f.finish8(x, m0 + k, n + c, N);
+    float4 *d = reinterpret_cast<float4 *>(f.parts + ((long long)split * M + m0 + k) * f.ld_parts + n + c);
+    d[0] = make_float4(x[0], x[1], x[2], x[3]);
+    d[1] = make_float4(x[4], x[5], x[6], x[7]);
+  });
+}
+
+// Finishes sums, a row per lane.  Addends come, and results go, 32 rows x 32 columns at a time through shared memory,
+// by tensor copies where these reach the matrix.  (Reading them a row per lane took longer than the product.)  A warp
+// has two pieces of 2 KB, which results go through by turns; addends that tensor copies bring come there, one for
+// each half of the warp's columns, before the sums are done, and the results replace them; where z is kept too, the
+// second is z's.
 template <class T> struct ResultEnd {
   Result<T> f;
   struct State {};
   __device__ __forceinline__ void start(State &, const DenseProblem &, int, const DenseUnit &) const {}
   __device__ __forceinline__ void tile(const DenseProblem &p, int n, DenseWarp &w) const {
-    if (!f.bias || !f.sends) return;
+    if (!f.bias) return;
     T *b = reinterpret_cast<T *>(w.bias);
     __syncwarp();
 #pragma unroll
@@ -695,7 +718,7 @@ template <class T> struct ResultEnd {
   }
   // (row: the lane's; the first lane's is the warp's first)
   __device__ __forceinline__ void ahead(const DenseProblem &p, int row, int n, int columns, DenseWarp &w) const {
-    if (!f.sends || !f.addend || threadIdx.x % 32) return;
+    if (!f.addend || !f.tma_addend || f.parts || threadIdx.x % 32) return;
     const bool two = columns > 32 && n + 32 < p.N && !f.pre;
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); // (the last results may still be on their way)
     dense_expect(w.bar, two ? 2 * kOutBytes : kOutBytes);
@@ -706,23 +729,9 @@ template <class T> struct ResultEnd {
                                         DenseWarp &w, bool second, bool more) const {
     const int lane = threadIdx.x % 32;
     const int m0 = row - lane;
-    if (!f.sends) {
-      if (f.parts)
-        turned(r, w.mine, [&](int k, int c, const float (&x)[8]) {
-          if (m0 + k >= p.M || n + c >= p.N) return;
-          float4 *d = reinterpret_cast<float4 *>(f.parts + ((long long)u.split * p.M + m0 + k) * f.ld_parts + n + c);
-          d[0] = make_float4(x[0], x[1], x[2], x[3]);
-          d[1] = make_float4(x[4], x[5], x[6], x[7]);
-        });
-      else if (f.vec_out)
-        turned(r, w.mine, [&](int k, int c, const float (&x)[8]) {
-          if (m0 + k < p.M && n + c < p.N) f.finish8(x, m0 + k, n + c, p.N);
-        });
-      else
-        turned_columns(r, w.mine, [&](int k, float x) {
-          if (m0 + k < p.M && n + lane < p.N) f.finish1(x, m0 + k, n + lane);
-        });
-      return;
+    if (f.parts || f.sums) {
+      turn(r, w.mine);
+      return keep_sums(f, w.mine, m0, n, p.M, p.N, u.split);
     }
     Two z[16];
 #pragma unroll
@@ -743,22 +752,19 @@ template <class T> struct ResultEnd {
 #pragma unroll
       for (int i = 0; i < 4; ++i) add8(i, b[i]);
     }
-    unsigned char *to = w.mine + (f.pre ? 0 : f.addend ? (second ? kOutBytes : 0) : w.turn);
+    unsigned char *to = w.mine + (f.pre ? 0 : f.addend ? (second ? kOutBytes : 0) : w.turn), *kept = w.mine + kOutBytes;
     w.turn ^= kOutBytes;
+    if (f.addend || f.pre) out_free<0>();
+    else out_free<1>(); // (the other piece's copy may be under way)
     if (f.addend) {
-      if (!second || f.pre) {
+      if (!f.tma_addend) {
+        copy_in(f.addend, f.ld_addend, m0, n, p.M, p.N, to);
+      } else if (!second || f.pre) {
         if (w.ok) w.ok = __all_sync(~0u, dense_wait(w.bar, w.phase));
         w.phase ^= 1;
       }
-    } else if (f.pre) {
-      out_free<0>();
-    } else {
-      out_free<1>(); // (the other piece's copy may be under way)
     }
-    if (f.pre) {
-      if (f.addend) out_free<0>();
-      out_put<T>(w.mine + kOutBytes, z);
-    }
+    if (f.pre) out_put<T>(kept, z);
     with_act(f.act, [&](auto a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) z[i] = Two(act_value<decltype(a)::value>(z[i].get()));
@@ -768,36 +774,125 @@ template <class T> struct ResultEnd {
       for (int i = 0; i < 4; ++i) add8(i, *out_piece(to, i));
     }
     out_put<T>(to, z);
+    if (f.pre && !f.tma_pre) copy_out(f.pre, f.ld_pre, m0, n, p.M, p.N, kept);
+    if (!f.tma_out) copy_out(f.out, f.ld_out, m0, n, p.M, p.N, to);
     out_ready();
-    if (lane) return;
-    if (m0 < p.M) {
-      out_send(&f.out_map, to, m0, n);
-      if (f.pre) out_send(&f.pre_map, w.mine + kOutBytes, m0, n);
-    }
-    out_commit();
-    if (more && f.addend && f.pre) { // (no room for it before)
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      dense_expect(w.bar, kOutBytes);
-      fetch(m0, n + 32, w.mine, w);
+    if (lane == 0) {
+      if (m0 < p.M) {
+        if (f.tma_out) out_send(&f.out_map, to, m0, n);
+        if (f.pre && f.tma_pre) out_send(&f.pre_map, kept, m0, n);
+      }
+      out_commit();
+      if (more && f.addend && f.tma_addend && f.pre) { // (no room for it before)
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        dense_expect(w.bar, kOutBytes);
+        fetch(m0, n + 32, w.mine, w);
+      }
     }
   }
   __device__ __forceinline__ void stop(State &, const DenseProblem &, int, const DenseUnit &, int) const {}
 };
-// Adds the parts up, in order, and finishes them.
+// Adds parts up, in order, and finishes them; adds up rows of column sums.  One launch for what follows a call's
+// products: blocks 0 .. blocks[0] - 1 have the first job, and so on.
+template <class T> struct FinishJobs {
+  unsigned blocks[3];
+  int splits[2];
+  long long M[2], N[2];
+  Result<T> end[2]; // end.parts, end.ld_parts
+  const float *rows; // [count][ld_rows]
+  long long count, ld_rows, columns;
+  T *column_sums;     // sum of a column of `rows` / *scale
+  const float *scale; // or null: 1
+};
 template <class T>
-__global__ void __launch_bounds__(256) tb_dense_join_kernel(const float *parts, int splits, long long ld, long long M, long long N,
-                                                            const __grid_constant__ Result<T> f) {
-  const long long per = ld / 8, i = (long long)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void join_parts(const Result<T> &f, int splits, long long M, long long N, unsigned block) {
+  const long long per = f.ld_parts / 8, i = (long long)block * 256 + threadIdx.x;
   if (i >= M * per) return;
   const long long m = i / per, n = i % per * 8;
   float v[8] = {};
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
-    const float4 *d = reinterpret_cast<const float4 *>(parts + ((long long)s * M + m) * ld + n);
+    const float4 *d = reinterpret_cast<const float4 *>(f.parts + ((long long)s * M + m) * f.ld_parts + n);
     const float4 a = d[0], b = d[1];
     v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
   }
   f.finish8(v, m, n, N);
+}
+template <class T> __global__ void __launch_bounds__(256) tb_dense_finish_kernel(const __grid_constant__ FinishJobs<T> jobs) {
+  __shared__ float part[8][32];
+  after_previous_kernel();
+  unsigned b = blockIdx.x;
+  if (b < jobs.blocks[0]) return join_parts(jobs.end[0], jobs.splits[0], jobs.M[0], jobs.N[0], b);
+  b -= jobs.blocks[0];
+  if (b < jobs.blocks[1]) return join_parts(jobs.end[1], jobs.splits[1], jobs.M[1], jobs.N[1], b);
+  b -= jobs.blocks[1];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const long long c = (long long)b * 32 + lane;
+  float s = 0.f;
+  if (c < jobs.columns)
+#pragma unroll 8
+    for (long long t = warp; t < jobs.count; t += 8) s += jobs.rows[t * jobs.ld_rows + c];
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp || c >= jobs.columns) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += part[i][lane];
+  jobs.column_sums[c] = from_float<T>(jobs.scale ? s / *jobs.scale : s);
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------
+// y for up to ROWS rows of x: a warp per output reads its row of the weights once, eight elements a lane at a time
+// (in one read where VEC), four of these under way; what bounds it is the latency of one such read, then the
+// weights' bytes.
+constexpr int kFewRows = 8;
+template <class T, bool VEC, int ROWS>
+__global__ void __launch_bounds__(256) tb_linear_rows_kernel(const T *x, long long ld_x, const T *weight, long long ld_w,
+                                                             const __grid_constant__ Result<T> f, int rows, int inputs, int outputs) {
+  constexpr int kPer = 8, kAhead = 4;
+  after_previous_kernel();
+  const int lane = threadIdx.x % 32;
+  auto read = [&](const T *p, int k) { return k < inputs ? raw8(p + k, min(8, inputs - k), VEC) : make_uint4(0, 0, 0, 0); };
+  for (long long o = (long long)blockIdx.x * 8 + threadIdx.x / 32; o < outputs; o += gridDim.x * 8ll) {
+    Two acc[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) acc[r] = Two(0.f);
+    const T *row = weight + o * ld_w;
+    for (int k0 = lane * kPer; k0 < inputs; k0 += 32 * kPer * kAhead) {
+      uint4 w[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) w[i] = read(row, k0 + i * 32 * kPer);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const uint4 q = read(x + (r < rows ? r : 0) * ld_x, k0 + i * 32 * kPer);
+          const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[r] = fma2(Two(unpack2<T>(ww[j])), Two(unpack2<T>(qw[j])), acc[r]);
+        }
+      }
+    }
+    float sum[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float2 v = acc[r].get();
+      sum[r] = v.x + v.y;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum[r] += __shfl_xor_sync(~0u, sum[r], d);
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (lane == r) mine = sum[r];
+    if (lane < rows) {
+      const float z = f.bias ? mine + to_float(f.bias[o]) : mine;
+      if (f.pre) f.pre[lane * f.ld_pre + o] = from_float<T>(z);
+      float y = z;
+      with_act(f.act, [&](auto a) { y = act_value<decltype(a)::value>(make_float2(z, z)).x; });
+      f.out[lane * f.ld_out + o] = from_float<T>(f.addend ? y + to_float(f.addend[lane * f.ld_addend + o]) : y);
+    }
+  }
 }
 
 __device__ __forceinline__ long long label_at(const void *labels, int bytes, long long m) {
@@ -881,6 +976,7 @@ constexpr int kJoinWarps = 32;
 __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const float2 *parts, int count, const float *at, const void *labels, int label_bytes,
                                                                        long long classes, float *loss, float *lse, long long rows) {
   __shared__ float2 mine[kJoinWarps][32];
+  after_previous_kernel();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const long long m = (long long)blockIdx.x * 32 + lane;
   float top = -INFINITY, sum = 0.f;
@@ -995,21 +1091,11 @@ template <class T, int COLS> struct ScoreGradEnd {
 
 // dz = grad * activation'(pre), rounded; sums of its columns over 32 rows before that.  32 rows x 256 columns
 // a block, four rows a warp, whose loads are under way together.
-template <class T> __device__ __forceinline__ uint4 raw8(const T *p, int n, bool vec) { // eight elements, n of them there
-  if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
-  uint32_t w[4] = {0, 0, 0, 0};
-  const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) w[i / 2] |= (uint32_t)__ldg(q + i) << (i % 2 * 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 template <class T, int ACT>
-__global__ void __launch_bounds__(256, 4) tb_act_grad_kernel(const T *grad, long long ld_grad, bool vec_grad, const T *pre, long long ld_pre,
-                                                             bool vec_pre, T *dz, long long ld, float *bias_sums, int rows, int cols) {
-  __shared__ float part[8][256];
+__device__ __forceinline__ void act_grad(const T *grad, long long ld_grad, bool vec_grad, const T *pre, long long ld_pre, bool vec_pre, T *dz,
+                                         long long ld, float *bias_sums, int rows, int cols, int bx, int by, float (&part)[8][256]) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int c = (blockIdx.y * 32 + lane) * 8, r0 = blockIdx.x * 32 + warp * 4, have = min(8, cols - c);
+  const int c = (by * 32 + lane) * 8, r0 = bx * 32 + warp * 4, have = min(8, cols - c);
   float sum[8] = {};
   if (have > 0) {
     uint4 g[4], z[4];
@@ -1041,62 +1127,70 @@ __global__ void __launch_bounds__(256, 4) tb_act_grad_kernel(const T *grad, long
   for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = sum[k];
   __syncthreads();
   const int k = threadIdx.x % 8, l = threadIdx.x / 8; // (neighbouring threads have neighbouring columns)
-  const int at = (blockIdx.y * 32 + l) * 8 + k;
+  const int at = (by * 32 + l) * 8 + k;
   if (at >= ld) return;
   float s = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) s += part[w][k * 32 + l];
-  bias_sums[blockIdx.x * ld + at] = s;
+  bias_sums[bx * ld + at] = s;
 }
-
-// out[c] = sum over `count` rows of sums[., c], times 1 / scale: 32 warps take every 32nd row each
-template <class T>
-__global__ void __launch_bounds__(1024) tb_column_sum_kernel(const float *sums, long long count, long long ld, T *out, long long cols, const float *scale) {
-  __shared__ float part[32][32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long long c = (long long)blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (c < cols)
-#pragma unroll 4
-    for (long long t = warp; t < count; t += 32) s += sums[t * ld + c];
-  part[warp][lane] = s;
-  __syncthreads();
-  if (warp || c >= cols) return;
-#pragma unroll
-  for (int i = 1; i < 32; ++i) s += part[i][lane];
-  out[c] = from_float<T>(scale ? s / *scale : s);
-}
-
 // The power of two that brings the largest |v| to about 2^13 (1 where nothing finite and nonzero is there).
-__global__ void __launch_bounds__(1024) tb_scale_kernel(const float *v, long long n, float *scale) {
-  __shared__ float tops[32];
+__device__ __forceinline__ void find_scale(const float *v, long long n, float *scale, float *tops) {
   float top = 0.f;
-  for (long long i = threadIdx.x; i < n; i += 1024)
-    if (fabsf(v[i]) < INFINITY) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll 8
+  for (long long i = threadIdx.x; i < n; i += 256) {
+    const float a = fabsf(v[i]);
+    if (a < INFINITY) top = fmaxf(top, a);
+  }
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
   __syncthreads();
   if (threadIdx.x) return;
-  for (int i = 1; i < 32; ++i) top = fmaxf(top, tops[i]);
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, tops[i]);
   int e = 0;
   if (top > 0.f) frexpf(top, &e);
   *scale = top > 0.f ? ldexpf(1.f, min(max(13 - e, -100), 100)) : 1.f;
 }
-
-// A matrix whose rows do not begin at multiples of 16 bytes, copied to where they do: 16 bytes a thread.
-template <class T>
-__global__ void __launch_bounds__(256) tb_align_rows_kernel(const T *src, long long ld_src, T *dst, long long ld, long long rows, long long cols) {
-  const long long per = ld / 8, all = rows * per;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
-    const long long r = i / per, c = i % per * 8;
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const unsigned short *p = reinterpret_cast<const unsigned short *>(src + r * ld_src + c + 2 * k);
-      w[k] = (c + 2 * k < cols ? __ldg(p) : 0) | (uint32_t)(c + 2 * k + 1 < cols ? __ldg(p + 1) : 0) << 16;
-    }
-    *reinterpret_cast<uint4 *>(dst + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+// What has to be there before a call's products, in one launch: the scale of a loss's gradient, dz of a layer, and
+// matrices whose rows do not begin at multiples of 16 bytes copied to where they do (16 bytes a thread).
+template <class T> struct PrepareJobs {
+  const float *weights; // find_scale
+  long long num_weights;
+  float *scale;
+  const T *grad, *pre; // act_grad
+  long long ld_grad, ld_pre, ld_dz;
+  bool vec_grad, vec_pre;
+  T *dz;
+  float *bias_sums;
+  int rows, cols;
+  unsigned row_blocks;
+  struct {
+    const T *from;
+    T *to;
+    long long ld_from, ld_to, rows, cols;
+  } copy[2];
+  unsigned blocks[4]; // of the scale, of dz, of the copies
+};
+template <class T, int ACT> __global__ void __launch_bounds__(256, 4) tb_dense_prepare_kernel(const __grid_constant__ PrepareJobs<T> jobs) {
+  __shared__ float part[8][256];
+  after_previous_kernel();
+  unsigned b = blockIdx.x;
+  if (b < jobs.blocks[0]) return find_scale(jobs.weights, jobs.num_weights, jobs.scale, part[0]);
+  b -= jobs.blocks[0];
+  if (b < jobs.blocks[1])
+    return act_grad<T, ACT>(jobs.grad, jobs.ld_grad, jobs.vec_grad, jobs.pre, jobs.ld_pre, jobs.vec_pre, jobs.dz, jobs.ld_dz, jobs.bias_sums,
+                            jobs.rows, jobs.cols, b % jobs.row_blocks, b / jobs.row_blocks, part);
+  b -= jobs.blocks[1];
+  const int which = b >= jobs.blocks[2];
+  if (which) b -= jobs.blocks[2];
+  const T *from = which ? jobs.copy[1].from : jobs.copy[0].from;
+  T *to = which ? jobs.copy[1].to : jobs.copy[0].to;
+  const long long ld_from = which ? jobs.copy[1].ld_from : jobs.copy[0].ld_from, ld_to = which ? jobs.copy[1].ld_to : jobs.copy[0].ld_to;
+  const long long rows = which ? jobs.copy[1].rows : jobs.copy[0].rows, cols = which ? jobs.copy[1].cols : jobs.copy[0].cols;
+  const long long per = ld_to / 8, i = (long long)b * 256 + threadIdx.x;
+  if (i >= rows * per) return;
+  const long long r = i / per, c = i % per * 8;
+  *reinterpret_cast<uint4 *>(to + r * ld_to + c) = raw8(from + r * ld_from + c, (int)min(8ll, cols - c), false);
 }
 
 } // namespace tb

@@ -1,4 +1,5 @@
-// Element types of the operators behind a forest's leaves: to fp32 and, rounded to nearest, back.
+// What the kernels behind a forest's leaves share: element types, to fp32 and, rounded to nearest, back; the
+// order of a call's kernels.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -13,5 +14,12 @@ template <class T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Kernels of one call follow one another closely: each is launched while the one before still runs, prepares itself
+// and waits here until that one's results are there (and lets its own follower come).
+__device__ __forceinline__ void after_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 } // namespace tb

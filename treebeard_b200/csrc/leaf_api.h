@@ -73,6 +73,24 @@ int check_workspace(const void *p, uint64_t have, uint64_t need) {
     if (rc__) return rc__;      \
   } while (0)
 
+// Launches a kernel that begins with after_previous_kernel(): it may come while the one before it still runs.
+template <class... P, class... A> int launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, unsigned cluster, A... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster, attrs[1].val.clusterDim.y = 1, attrs[1].val.clusterDim.z = 1;
+  config.attrs = attrs;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  CUDA_TRY(cudaLaunchKernelEx(&config, kernel, P(args)...));
+  return TBK_OK;
+}
+
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Multiprocessors of a device; the figure of the architecture where there is none (workspace sizes on a host).

@@ -141,9 +141,7 @@ template <class T, int SHAPE, class End, int JOBS> int launch_shape(const tb::De
     if (device <= 63) ready.fetch_or(1ull << device);
   }
   const unsigned grid = (unsigned)std::min(jobs.units, slots) * (SHAPE == tb::kDenseOne ? 1 : 2);
-  kernel<<<grid, tb::kDenseThreads, smem, stream>>>(jobs);
-  CUDA_TRY(cudaGetLastError());
-  return TBK_OK;
+  return launch(kernel, grid, tb::kDenseThreads, smem, stream, 1, jobs); // (its cluster is part of the kernel)
 }
 template <class T, class End, int JOBS> int launch_jobs(int shape, tb::DenseJobs<End, JOBS> &jobs, int sms, cudaStream_t stream) {
   jobs.units = jobs.p[0].units + (JOBS > 1 ? jobs.p[JOBS - 1].units : 0);
@@ -165,46 +163,71 @@ template <class T> struct Product {
   Size size;
   tb::Result<T> end;
 };
+// Column sums that are added up with a call's joins.
+template <class T> struct ColumnSums {
+  const float *rows = nullptr; // [count][ld]
+  int64_t count = 0, ld = 0, columns = 0;
+  T *out = nullptr;
+  const float *scale = nullptr;
+};
 // One or two products, which do not depend on one another.  parts: room for what part_floats says.
-template <class T> int products(const Product<T> *list, int count, float *parts, int sms, cudaStream_t stream) {
-  Size sizes[2];
-  for (int i = 0; i < count; ++i) sizes[i] = list[i].size;
-  const Cut cut = plan_products(sizes, count, sms, true);
-  tb::DenseJobs<tb::ResultEnd<T>, 2> jobs;
-  float *room[2] = {};
-  for (int i = 0; i < count; ++i) {
-    const Product<T> &x = list[i];
-    TRY(set_problem<T>(&jobs.p[i], cut.shape, x.a, x.b, x.size, cut.splits[i], 1));
-    jobs.end[i].f = x.end;
-    if (cut.splits[i] == 1) continue;
-    room[i] = parts;
-    jobs.end[i].f.parts = parts, jobs.end[i].f.ld_parts = up8(x.size.n);
-    jobs.end[i].f.sends = false;
-    parts += (uint64_t)cut.splits[i] * x.size.m * up8(x.size.n);
+template <class T>
+int products(const Product<T> *list, int count, const ColumnSums<T> &sums, float *parts, int sms, cudaStream_t stream) {
+  tb::FinishJobs<T> finish;
+  std::memset(static_cast<void *>(&finish), 0, sizeof finish);
+  if (count) {
+    Size sizes[2];
+    for (int i = 0; i < count; ++i) sizes[i] = list[i].size;
+    const Cut cut = plan_products(sizes, count, sms, true);
+    tb::DenseJobs<tb::ResultEnd<T>, 2> jobs;
+    for (int i = 0; i < count; ++i) {
+      const Product<T> &x = list[i];
+      TRY(set_problem<T>(&jobs.p[i], cut.shape, x.a, x.b, x.size, cut.splits[i], 1));
+      jobs.end[i].f = x.end;
+      if (cut.splits[i] == 1) continue;
+      jobs.end[i].f.parts = parts, jobs.end[i].f.ld_parts = up8(x.size.n);
+      finish.end[i] = jobs.end[i].f;
+      finish.splits[i] = cut.splits[i], finish.M[i] = x.size.m, finish.N[i] = x.size.n;
+      finish.blocks[i] = (unsigned)tiles_of(x.size.m * (up8(x.size.n) / 8), 256);
+      parts += (uint64_t)cut.splits[i] * x.size.m * up8(x.size.n);
+    }
+    TRY((launch_some<T, tb::ResultEnd<T>>(cut.shape, jobs, count, sms, stream)));
   }
-  TRY((launch_some<T, tb::ResultEnd<T>>(cut.shape, jobs, count, sms, stream)));
-  for (int i = 0; i < count; ++i) {
-    if (cut.splits[i] == 1) continue;
-    const Size &z = list[i].size;
-    const int64_t ld = up8(z.n);
-    tb::tb_dense_join_kernel<T><<<(unsigned)tiles_of(z.m * (ld / 8), 256), 256, 0, stream>>>(room[i], cut.splits[i], ld, z.m, z.n, list[i].end);
-    CUDA_TRY(cudaGetLastError());
+  if (sums.out) {
+    finish.rows = sums.rows, finish.count = sums.count, finish.ld_rows = sums.ld, finish.columns = sums.columns;
+    finish.column_sums = sums.out, finish.scale = sums.scale;
+    finish.blocks[2] = (unsigned)tiles_of(sums.columns, 32);
   }
-  return TBK_OK;
+  const unsigned blocks = finish.blocks[0] + finish.blocks[1] + finish.blocks[2];
+  return blocks ? launch(tb::tb_dense_finish_kernel<T>, blocks, 256, 0, stream, 1, finish) : (int)TBK_OK;
 }
 
 // Whether tensor copies can read a matrix: rows begin at multiples of 16 bytes.
 bool tma_rows(const void *p, int64_t ld, int64_t rows) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld % 8 == 0 || rows <= 1);
 }
-// The matrix itself, or a copy that tensor copies can read (in `room`, rows x up8(cols)).
-template <class T> int readable(const void **p, int64_t *ld, int64_t rows, int64_t cols, T *room, cudaStream_t stream) {
-  if (tma_rows(*p, *ld, rows)) return TBK_OK;
-  tb::tb_align_rows_kernel<T><<<(unsigned)std::min<int64_t>(tiles_of(rows * (up8(cols) / 8), 256), 1 << 16), 256, 0, stream>>>((const T *)*p, *ld, room, up8(cols), rows, cols);
-  CUDA_TRY(cudaGetLastError());
+// Has a matrix copied to `room` (rows x up8(cols)) where tensor copies cannot read it as it is.
+template <class T> void make_readable(tb::PrepareJobs<T> *jobs, int which, const void **p, int64_t *ld, int64_t rows, int64_t cols, void *room) {
+  if (tma_rows(*p, *ld, rows)) return;
+  jobs->copy[which] = {(const T *)*p, (T *)room, *ld, up8(cols), rows, cols};
+  jobs->blocks[2 + which] = (unsigned)tiles_of(rows * (up8(cols) / 8), 256);
   *p = room;
   *ld = up8(cols);
-  return TBK_OK;
+}
+template <class T> tb::PrepareJobs<T> no_jobs() {
+  tb::PrepareJobs<T> jobs;
+  std::memset(static_cast<void *>(&jobs), 0, sizeof jobs);
+  return jobs;
+}
+template <class T> int prepare(const tb::PrepareJobs<T> &jobs, int act, cudaStream_t stream) {
+  const unsigned blocks = jobs.blocks[0] + jobs.blocks[1] + jobs.blocks[2] + jobs.blocks[3];
+  if (!blocks) return TBK_OK;
+  switch (act) {
+  case TBK_ACT_RELU: return launch(tb::tb_dense_prepare_kernel<T, tb::kActRelu>, blocks, 256, 0, stream, 1, jobs);
+  case TBK_ACT_GELU: return launch(tb::tb_dense_prepare_kernel<T, tb::kActGelu>, blocks, 256, 0, stream, 1, jobs);
+  case TBK_ACT_SILU: return launch(tb::tb_dense_prepare_kernel<T, tb::kActSilu>, blocks, 256, 0, stream, 1, jobs);
+  default: return launch(tb::tb_dense_prepare_kernel<T, tb::kActNone>, blocks, 256, 0, stream, 1, jobs);
+  }
 }
 // Whether 16 bytes at a time can be read or written at every eighth column.
 bool vec_rows(const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
@@ -217,12 +240,28 @@ int set_result(tb::Result<T> *end, void *out, int64_t ld, int64_t rows, int64_t 
   end->addend = (const T *)addend, end->ld_addend = ld_addend, end->vec_addend = vec_rows(addend, ld_addend);
   end->pre = (T *)pre, end->ld_pre = ld_pre, end->vec_pre = vec_rows(pre, ld_pre);
   end->first = end->last = true;
-  end->sends = tma_rows(out, ld, rows) && (!addend || tma_rows(addend, ld_addend, rows)) && (!pre || tma_rows(pre, ld_pre, rows));
-  if (!end->sends) return TBK_OK;
-  TRY(out_map<T>(&end->out_map, out, rows, cols, ld));
-  if (addend) TRY(out_map<T>(&end->addend_map, addend, rows, cols, ld_addend));
-  if (pre) TRY(out_map<T>(&end->pre_map, pre, rows, cols, ld_pre));
+  end->tma_out = tma_rows(out, ld, rows), end->tma_addend = addend && tma_rows(addend, ld_addend, rows), end->tma_pre = pre && tma_rows(pre, ld_pre, rows);
+  if (end->tma_out) TRY(out_map<T>(&end->out_map, out, rows, cols, ld));
+  if (end->tma_addend) TRY(out_map<T>(&end->addend_map, addend, rows, cols, ld_addend));
+  if (end->tma_pre) TRY(out_map<T>(&end->pre_map, pre, rows, cols, ld_pre));
   return TBK_OK;
+}
+
+// A layer of at most kFewRows rows.
+template <class T>
+int few_rows(const T *x, int64_t ld_x, const T *weight, int64_t ld_w, const T *bias, int act, const T *residual, int64_t ld_res, T *out, int64_t ld_out, T *pre, int64_t ld_pre,
+             int n, int inputs, int outputs, int sms, cudaStream_t stream) {
+  tb::Result<T> end;
+  std::memset(static_cast<void *>(&end), 0, sizeof end);
+  end.bias = bias, end.act = act, end.addend = residual, end.ld_addend = ld_res, end.out = out, end.ld_out = ld_out, end.pre = pre, end.ld_pre = ld_pre;
+  const bool vec = tma_rows(x, ld_x, n) && tma_rows(weight, ld_w, outputs);
+  const unsigned blocks = (unsigned)std::min<int64_t>(tiles_of(outputs, 8), 8 * sms);
+  auto run = [&](auto rows) {
+    constexpr int R = decltype(rows)::value;
+    return vec ? launch(tb::tb_linear_rows_kernel<T, true, R>, blocks, 256, 0, stream, 1, x, ld_x, weight, ld_w, end, n, inputs, outputs)
+               : launch(tb::tb_linear_rows_kernel<T, false, R>, blocks, 256, 0, stream, 1, x, ld_x, weight, ld_w, end, n, inputs, outputs);
+  };
+  return n == 1 ? run(std::integral_constant<int, 1>()) : n <= 4 ? run(std::integral_constant<int, 4>()) : run(std::integral_constant<int, 8>());
 }
 
 typedef unsigned short Half; // an element of either 16-bit type
@@ -330,15 +369,19 @@ int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64_t ld_w, co
   return with_half(type, [&](auto t) {
     using T = decltype(t);
     const int sms = multiprocessors(device);
+    if (n <= tb::kFewRows) return few_rows<T>((const T *)x, ld_x, (const T *)weight, ld_w, (const T *)bias, act, (const T *)residual, ld_res, (T *)out, ld_out, (T *)pre,
+                                              ld_pre, (int)n, (int)inputs, (int)outputs, sms, stream);
     Parts w{(unsigned char *)ws};
     LinearParts parts(w, n, inputs, outputs, aligned, sms);
-    TRY(readable(&x, &ld_x, n, inputs, (T *)parts.x, stream));
-    TRY(readable(&weight, &ld_w, outputs, inputs, (T *)parts.weight, stream));
+    tb::PrepareJobs<T> before = no_jobs<T>();
+    make_readable(&before, 0, &x, &ld_x, n, inputs, parts.x);
+    make_readable(&before, 1, &weight, &ld_w, outputs, inputs, parts.weight);
+    TRY(prepare(before, TBK_ACT_IDENTITY, stream));
     Product<T> product{{x, ld_x, false}, {weight, ld_w, false}, {n, outputs, inputs}, {}};
     TRY(set_result<T>(&product.end, out, ld_out, n, outputs, residual, ld_res, pre, ld_pre));
     product.end.bias = (const T *)bias, product.end.vec_bias = vec_rows(bias, 0);
     product.end.act = act;
-    return products<T>(&product, 1, parts.parts, sms, stream);
+    return products<T>(&product, 1, {}, parts.parts, sms, stream);
   });
 }
 
@@ -388,24 +431,18 @@ int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_
     Parts w{(unsigned char *)ws};
     LinearGradParts parts(w, n, inputs, outputs, aligned, sms);
     T *dz = (T *)parts.dz;
-    if (grad_w) TRY(readable(&x, &ld_x, n, inputs, (T *)parts.x, stream));
-    if (grad_x) TRY(readable(&weight, &ld_w, outputs, inputs, (T *)parts.weight, stream));
-    auto slopes = [&](auto a) {
-      tb::tb_act_grad_kernel<T, decltype(a)::value><<<dim3((unsigned)tiles_of(n, 32), (unsigned)tiles_of(outputs, 256)), 256, 0, stream>>>(
-          (const T *)grad, ld_grad, vec_rows(grad, ld_grad), (const T *)pre, ld_pre, vec_rows(pre, ld_pre), dz, parts.ld,
-          grad_b ? parts.bias_sums : nullptr, (int)n, (int)outputs);
-    };
-    switch (act) {
-    case TBK_ACT_RELU: slopes(std::integral_constant<int, tb::kActRelu>()); break;
-    case TBK_ACT_GELU: slopes(std::integral_constant<int, tb::kActGelu>()); break;
-    case TBK_ACT_SILU: slopes(std::integral_constant<int, tb::kActSilu>()); break;
-    default: slopes(std::integral_constant<int, tb::kActNone>());
-    }
-    CUDA_TRY(cudaGetLastError());
-    if (grad_b) {
-      tb::tb_column_sum_kernel<T><<<(unsigned)tiles_of(outputs, 32), 1024, 0, stream>>>(parts.bias_sums, tiles_of(n, 32), parts.ld, (T *)grad_b, outputs, nullptr);
-      CUDA_TRY(cudaGetLastError());
-    }
+    tb::PrepareJobs<T> before = no_jobs<T>();
+    if (grad_w) make_readable(&before, 0, &x, &ld_x, n, inputs, parts.x);
+    if (grad_x) make_readable(&before, 1, &weight, &ld_w, outputs, inputs, parts.weight);
+    before.grad = (const T *)grad, before.ld_grad = ld_grad, before.vec_grad = vec_rows(grad, ld_grad);
+    before.pre = (const T *)pre, before.ld_pre = ld_pre, before.vec_pre = vec_rows(pre, ld_pre);
+    before.dz = dz, before.ld_dz = parts.ld, before.bias_sums = grad_b ? parts.bias_sums : nullptr;
+    before.rows = (int)n, before.cols = (int)outputs;
+    before.row_blocks = (unsigned)tiles_of(n, 32);
+    before.blocks[1] = before.row_blocks * (unsigned)tiles_of(outputs, 256);
+    TRY(prepare(before, act, stream));
+    ColumnSums<T> sums;
+    if (grad_b) sums = {parts.bias_sums, tiles_of(n, 32), parts.ld, outputs, (T *)grad_b, nullptr};
     Product<T> list[2];
     int count = 0;
     if (grad_x) {
@@ -418,7 +455,7 @@ int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_
       q.a = {dz, parts.ld, true}, q.b = {x, ld_x, true}, q.size = {outputs, inputs, n};
       TRY(set_result<T>(&q.end, grad_w, ld_gw, outputs, inputs, nullptr, 0, nullptr, 0));
     }
-    return count ? products<T>(list, count, parts.parts, sms, stream) : (int)TBK_OK;
+    return products<T>(list, count, sums, parts.parts, sms, stream);
   });
 }
 
@@ -458,8 +495,10 @@ int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_w
     const int sms = multiprocessors(device);
     Parts w{(unsigned char *)ws};
     LossParts parts(w, n, width, classes, aligned, sms);
-    TRY(readable(&x, &ld_x, n, width, (T *)parts.x, stream));
-    TRY(readable(&weight, &ld_w, classes, width, (T *)parts.weight, stream));
+    tb::PrepareJobs<T> before = no_jobs<T>();
+    make_readable(&before, 0, &x, &ld_x, n, width, parts.x);
+    make_readable(&before, 1, &weight, &ld_w, classes, width, parts.weight);
+    TRY(prepare(before, TBK_ACT_IDENTITY, stream));
     const Side a{x, ld_x, false}, b{weight, ld_w, false};
     auto scores = [&](auto cols) {
       using End = tb::LseEnd<T, decltype(cols)::value>;
@@ -470,9 +509,8 @@ int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_w
     };
     if (parts.cut.shape == tb::kDenseOne) TRY(scores(std::integral_constant<int, 32>()));
     else TRY(scores(std::integral_constant<int, 64>()));
-    tb::tb_loss_join_kernel<<<(unsigned)tiles_of(n, 32), 32 * tb::kJoinWarps, 0, stream>>>(parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss, lse, n);
-    CUDA_TRY(cudaGetLastError());
-    return (int)TBK_OK;
+    return launch(tb::tb_loss_join_kernel, (unsigned)tiles_of(n, 32), 32 * tb::kJoinWarps, 0, stream, 1, parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss,
+                  lse, n);
   });
 }
 
@@ -512,13 +550,15 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
     const int sms = multiprocessors(device);
     Parts w{(unsigned char *)ws};
     LossGradParts parts(w, n, width, classes, aligned, sms);
-    TRY(readable(&x, &ld_x, n, width, (T *)parts.x, stream));
-    TRY(readable(&weight, &ld_w, classes, width, (T *)parts.weight, stream));
+    tb::PrepareJobs<T> before = no_jobs<T>();
+    make_readable(&before, 0, &x, &ld_x, n, width, parts.x);
+    make_readable(&before, 1, &weight, &ld_w, classes, width, parts.weight);
+    before.weights = grad, before.num_weights = n, before.scale = parts.scale;
+    before.blocks[0] = 1;
+    TRY(prepare(before, TBK_ACT_IDENTITY, stream));
     const T *W = (const T *)weight;
     T *dz = (T *)parts.dz;
     const int64_t ld = parts.piece;
-    tb::tb_scale_kernel<<<1, 1024, 0, stream>>>(grad, n, parts.scale);
-    CUDA_TRY(cudaGetLastError());
     for (int64_t v = 0; v < classes; v += ld) {
       const int64_t now = std::min(ld, classes - v);
       const Side xs{x, ld_x, false}, ws_{W + v * ld_w, ld_w, false};
@@ -537,10 +577,8 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
       };
       if (shape == tb::kDenseOne) TRY(gradients(std::integral_constant<int, 32>()));
       else TRY(gradients(std::integral_constant<int, 64>()));
-      if (grad_b) {
-        tb::tb_column_sum_kernel<T><<<(unsigned)tiles_of(now, 32), 1024, 0, stream>>>(parts.bias_sums, tiles_of(n, 32), ld, (T *)grad_b + v, now, parts.scale);
-        CUDA_TRY(cudaGetLastError());
-      }
+      ColumnSums<T> column_sums;
+      if (grad_b) column_sums = {parts.bias_sums, tiles_of(n, 32), ld, now, (T *)grad_b + v, parts.scale};
       Product<T> list[2];
       int count = 0;
       if (grad_x) {
@@ -549,9 +587,8 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
         TRY(set_result<T>(&q.end, grad_x, ld_gx, n, width, nullptr, 0, nullptr, 0));
         q.end.scale = parts.scale;
         if (ld < classes) { // (several pieces)
-          q.end.sums = parts.sums, q.end.ld_sums = parts.ld_sums, q.end.sends = false;
+          q.end.sums = parts.sums, q.end.ld_sums = parts.ld_sums;
           q.end.first = v == 0, q.end.last = v + now == classes;
-          q.end.vec_out = q.end.vec_out || !q.end.last; // (the sums are aligned)
         }
       }
       if (grad_w) {
@@ -561,7 +598,7 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
         TRY(set_result<T>(&q.end, to, ld_gw, now, width, nullptr, 0, nullptr, 0));
         q.end.scale = parts.scale;
       }
-      if (count) TRY(products<T>(list, count, parts.parts, sms, stream));
+      TRY(products<T>(list, count, column_sums, parts.parts, sms, stream));
     }
     return (int)TBK_OK;
   });

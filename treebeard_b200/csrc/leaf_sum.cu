@@ -203,28 +203,15 @@ int tbk_leaf_sum(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t
     constexpr int V = decltype(v)::value;
     const uint32_t row_bytes = (uint32_t)(ld_table * sizeof(T));
     if (plan.by_row) {
-      cudaLaunchConfig_t config = {};
-      config.gridDim = dim3((unsigned)(n * plan.cluster), plan.columns);
-      config.blockDim = dim3((unsigned)plan.threads);
-      config.stream = stream;
-      cudaLaunchAttribute cluster;
-      cluster.id = cudaLaunchAttributeClusterDimension;
-      cluster.val.clusterDim = {(unsigned)plan.cluster, 1, 1};
-      config.attrs = &cluster;
-      config.numAttrs = 1;
-      CUDA_TRY(cudaLaunchKernelEx(&config, tb::tb_leaf_sum_row_kernel<T, V>, map->view, ids, (long long)ld_ids, (const T *)table, row_bytes,
-                                  (long long)width, plan.lanes_log2, (T *)out, (long long)ld_out, plan.cluster));
-      return (int)TBK_OK;
+      return launch(tb::tb_leaf_sum_row_kernel<T, V>, dim3((unsigned)(n * plan.cluster), plan.columns), plan.threads, 0, stream, plan.cluster, map->view, ids, ld_ids,
+                    (const T *)table, row_bytes, width, plan.lanes_log2, (T *)out, ld_out, plan.cluster);
     }
     float *parts = (float *)ws;
-    tb::tb_leaf_sum_kernel<T, V><<<dim3((unsigned)plan.work.blocks, plan.columns), plan.threads, 0, stream>>>(
-        map->view, ids, ld_ids, (const T *)table, row_bytes, width, plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, n, plan.work);
-    CUDA_TRY(cudaGetLastError());
-    if (plan.max_parts) {
-      const int64_t threads = n * plan.ld_parts / tb::Share<T, V>::kElems;
-      tb::tb_leaf_sum_join_kernel<T, V><<<(unsigned)tiles_of(threads, 256), 256, 0, stream>>>(parts, plan.ld_parts, plan.tile_rows, (T *)out, ld_out, width, n, plan.work);
-      CUDA_TRY(cudaGetLastError());
-    }
+    TRY(launch(tb::tb_leaf_sum_kernel<T, V>, dim3((unsigned)plan.work.blocks, plan.columns), plan.threads, 0, stream, 1, map->view, ids, ld_ids, (const T *)table, row_bytes,
+               width, plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, n, plan.work));
+    if (plan.max_parts)
+      TRY(launch(tb::tb_leaf_sum_join_kernel<T, V>, (unsigned)tiles_of(n * plan.ld_parts / tb::Share<T, V>::kElems, 256), 256, 0, stream, 1, parts, plan.ld_parts, plan.tile_rows,
+                 (T *)out, ld_out, width, n, plan.work));
     return (int)TBK_OK;
   });
 }
@@ -261,9 +248,8 @@ int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n
   const bool narrow = map->max_rows < 0xffff;
   LeafGradParts parts(w, n, width, trees, map->rows, narrow);
   const dim3 blocks((unsigned)std::min<int64_t>(tiles_of(n, tb::kNumberRows), 4096), (unsigned)tiles_of(trees, 32));
-  if (narrow) tb::tb_leaf_numbers_kernel<uint16_t><<<blocks, 256, 0, stream>>>(map->view, ids, ld_ids, (uint16_t *)parts.numbers, parts.ld, n);
-  else tb::tb_leaf_numbers_kernel<uint32_t><<<blocks, 256, 0, stream>>>(map->view, ids, ld_ids, (uint32_t *)parts.numbers, parts.ld, n);
-  CUDA_TRY(cudaGetLastError());
+  if (narrow) TRY(launch(tb::tb_leaf_numbers_kernel<uint16_t>, blocks, 256, 0, stream, 1, map->view, ids, ld_ids, (uint16_t *)parts.numbers, parts.ld, n));
+  else TRY(launch(tb::tb_leaf_numbers_kernel<uint32_t>, blocks, 256, 0, stream, 1, map->view, ids, ld_ids, (uint32_t *)parts.numbers, parts.ld, n));
   return with_piece(type, piece_bytes(type, width, grad, ld_grad, n, out, ld_out, map->rows), [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
@@ -271,16 +257,14 @@ int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n
     const int chunk = (int)std::min<int64_t>(n, tb::kLeafChunk), smem = tb::leaf_grad_smem(chunk, range);
     const dim3 grid((unsigned)trees, (unsigned)tiles_of(width, (int64_t)(16 / size) << lanes_log2), (unsigned)tiles_of(map->max_rows, range));
     if (grid.y > 65535 || grid.z > 65535) return fail(TBK_ERR_UNSUPPORTED, "leaf_sum_backward: too many columns, or leaves of a tree");
-    auto launch = [&](auto number) {
+    auto sorted = [&](auto number) {
       using N = decltype(number);
       const auto kernel = tb::tb_leaf_grad_kernel<T, V, N>;
       CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tb::leaf_grad_smem(tb::kLeafChunk, tb::kLeafRange)));
-      kernel<<<grid, 32 * tb::kLeafGradWarps, smem, stream>>>(map->view, (const N *)parts.numbers, parts.ld, (const T *)grad, (uint32_t)(ld_grad * sizeof(T)),
-                                                              width, lanes_log2, parts.sums, (T *)out, ld_out, n, chunk, range);
-      CUDA_TRY(cudaGetLastError());
-      return (int)TBK_OK;
+      return launch(kernel, grid, 32 * tb::kLeafGradWarps, smem, stream, 1, map->view, (const N *)parts.numbers, parts.ld, (const T *)grad, (uint32_t)(ld_grad * sizeof(T)), width,
+                    lanes_log2, parts.sums, (T *)out, ld_out, n, chunk, range);
     };
-    return narrow ? launch(uint16_t()) : launch(uint32_t());
+    return narrow ? sorted(uint16_t()) : sorted(uint32_t());
   });
 }
 

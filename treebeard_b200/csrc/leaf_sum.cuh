@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kLeafRowThreads) tb_leaf_sum_row_kernel(LeafMa
   using S = Share<T, V>;
   constexpr int P = S::kPairs, kWarps = kLeafRowThreads / 32;
   __shared__ unsigned long long part[kWarps][32][P]; // [0]: the block's sum in the end
+  after_previous_kernel();
   const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), rank = blockIdx.x % blocks;
   const int group = rank * (kLeafRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2), groups = blocks * (kLeafRowThreads >> lanes_log2);
   const long long n = blockIdx.x / blocks, c = ((long long)blockIdx.y * lanes + lane) * S::kElems;
@@ -194,6 +195,7 @@ __global__ void __launch_bounds__(512, 1) tb_leaf_sum_kernel(LeafMapView m, cons
                                                              long long n_rows, LeafStretch work) {
   using S = Share<T, V>;
   constexpr int P = S::kPairs;
+  after_previous_kernel();
   const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), groups = blockDim.x >> lanes_log2;
   const int base = threadIdx.x & 31 & ~(lanes - 1);
   const long long c = ((long long)blockIdx.y * lanes + lane) * S::kElems;
@@ -262,6 +264,7 @@ __global__ void __launch_bounds__(256) tb_leaf_sum_join_kernel(const float *part
                                                                long long width, long long n_rows, LeafStretch work) {
   using S = Share<T, V>;
   constexpr int P = S::kPairs;
+  after_previous_kernel();
   const long long per = ld_parts / S::kElems, i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n_rows * per) return;
   const long long n = i / per, c = i % per * S::kElems, tile = n / tile_rows;
@@ -285,6 +288,7 @@ template <class N>
 __global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, N *numbers, long long ld,
                                                               long long n_rows) {
   __shared__ int32_t tile[32][kNumberRows + 1];
+  after_previous_kernel();
   const int x = threadIdx.x % 32, y = threadIdx.x / 32;
   const long long t0 = (long long)blockIdx.y * 32;
   for (long long n0 = (long long)blockIdx.x * kNumberRows; n0 < n_rows; n0 += (long long)gridDim.x * kNumberRows) {
@@ -330,6 +334,7 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 3) tb_leaf_grad_kernel(Le
   constexpr int P = S::kPairs;
   constexpr uint32_t kNone = (N)~(N)0;
   extern __shared__ __align__(16) unsigned char raw[];
+  after_previous_kernel();
   uint32_t *start = reinterpret_cast<uint32_t *>(raw);                  // [leaves + 1] first place of a leaf
   uint32_t *count = reinterpret_cast<uint32_t *>(raw + kLeafGradFixed); // [warp][leaves]
   unsigned long long *ends = reinterpret_cast<unsigned long long *>(count); // [thread][P] sum of a stretch's first run
