@@ -45,6 +45,10 @@ def test_leaf_map_refuses_malformed_forests():
     c, keep = kernels.forest_arrays_c(forest)
     keep[0][3] = keep[0][2]
     assert create(ctypes.byref(c), 0, ctypes.byref(out)) == INVALID and b"tree 2" in lm.lib().tbk_last_error()
+    forest = synth.generate_forest(0, 5, 4, 8, 0.1, 0.1, synth.Marginal("normal", 8))
+    c, keep = kernels.forest_arrays_c(forest)
+    keep[1][keep[0][3]:keep[0][4]] = 0
+    assert create(ctypes.byref(c), 0, ctypes.byref(out)) == INVALID and b"tree 3 has no leaf" in lm.lib().tbk_last_error()
     assert out.value is None and lm.lib().tbk_leaf_map_rows(None) == -1 and lm.lib().tbk_leaf_map_free(None) == 0
 
 

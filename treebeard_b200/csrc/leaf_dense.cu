@@ -604,14 +604,17 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
   });
 }
 
+int leaf_sum_status(int *word); // (leaf_sum.cu)
+
 int tbk_leaf_check_status(int32_t device) {
   OnDevice on(device);
   CUDA_TRY(on.error);
-  int word = 0, zero = 0;
-  CUDA_TRY(cudaMemcpyFromSymbol(&word, tb::tb_dense_status, sizeof word));
-  if (!word) return TBK_OK;
-  CUDA_TRY(cudaMemcpyToSymbol(tb::tb_dense_status, &zero, sizeof zero));
-  return fail(TBK_ERR_DEVICE_WAIT, "a wait inside a matrix product gave up");
+  int dense = 0, leaf = 0, zero = 0;
+  CUDA_TRY(cudaMemcpyFromSymbol(&dense, tb::tb_dense_status, sizeof dense));
+  if (dense) CUDA_TRY(cudaMemcpyToSymbol(tb::tb_dense_status, &zero, sizeof zero));
+  TRY(leaf_sum_status(&leaf));
+  if (!dense && !leaf) return TBK_OK;
+  return fail(TBK_ERR_DEVICE_WAIT, "a wait inside a %s gave up", dense ? "matrix product" : "leaf sum");
 }
 
 } // extern "C"

@@ -46,16 +46,19 @@ int lanes_of(int64_t width, int32_t type) {
   return log2;
 }
 
+constexpr int kLeafStagedSmem = 227 * 1024 - tb::kLeafStagedFixed;
+
 // How a leaf sum is cut.  Up to two rows per multiprocessor: a cluster of blocks per row.  Above that: tiles of
 // eight rows per lane group, of as few warps as it takes to have enough tiles, whose trees the blocks share
 // out (a block to a multiprocessor, 16 warps, where tiles are many; at most about 16 parts of a tile).  With
 // very many tiles each has a block of its own and there are no parts.
 struct LeafSumPlan {
   bool by_row;
+  int64_t staged_rows = 0; // of a tile
   int lanes_log2, threads, cluster = 1, tile_rows = 0;
   unsigned columns;
   int64_t ld_parts, max_parts = 0;
-  tb::LeafStretch work{};
+  tb::LeafStretch work{}, staged_work{}; // in batches of a tree per lane; of kLeafBatch trees
   LeafSumPlan(int64_t n, int64_t width, int32_t type, int64_t trees, int sms) {
     const int elems = type == TBK_TYPE_F32 ? 4 : 8;
     lanes_log2 = lanes_of(width, type);
@@ -75,12 +78,19 @@ struct LeafSumPlan {
     tile_rows = (int)(warps * rows_per_warp);
     work.tiles = tiles_of(n, tile_rows);
     work.batches = tiles_of(trees, lanes);
-    if (work.tiles >= 8 * sms) {
-      work.blocks = work.tiles;
-      return;
+    staged_rows = tb::kLeafAdders * rows_per_warp;
+    staged_work.tiles = tiles_of(n, staged_rows), staged_work.batches = tiles_of(trees, tb::kLeafBatch);
+    for (tb::LeafStretch *w : {&work, &staged_work}) {
+      w->blocks = w->tiles;
+      if (w->tiles >= 8 * sms) continue;
+      w->blocks = std::min(std::max<int64_t>(1, sms / columns) * (16 / warps), std::min<int64_t>(16 * w->tiles, w->tiles * w->batches));
+      max_parts = std::max(max_parts, std::min<int64_t>(w->blocks, w->batches / (w->tiles * w->batches / w->blocks) + 2));
     }
-    work.blocks = std::min(std::max<int64_t>(1, sms / columns) * (16 / warps), std::min<int64_t>(16 * work.tiles, work.tiles * work.batches));
-    max_parts = std::min<int64_t>(work.blocks, work.batches / (work.tiles * work.batches / work.blocks) + 2);
+  }
+  // Tables of trees are staged where three stages hold the largest and a tile has as many rows as the
+  // largest tree leaves (with fewer, more bytes are copied than read).
+  bool staged(int64_t max_rows, int64_t row_bytes) const {
+    return !by_row && columns == 1 && threads == 512 && staged_rows <= tb::kLeafMostRows && max_rows <= staged_rows && max_rows * row_bytes + tb::kLeafZeros <= kLeafStagedSmem / 3;
   }
 };
 
@@ -124,6 +134,7 @@ int tbk_leaf_map_create(const tbk_forest_arrays *fa, int32_t device, tbk_leaf_ma
         words.push_back(w);
       }
       if (rows > kMost || words.size() > (size_t)kMost) return fail(TBK_ERR_UNSUPPORTED, "more than %lld leaves", (long long)kMost);
+      if (rows == row_off[t]) return fail(TBK_ERR_INVALID, "tree %lld has no leaf", (long long)t);
       map->max_rows = std::max<int64_t>(map->max_rows, rows - row_off[t]);
     }
     tree[trees] = make_int2((int)words.size(), 0);
@@ -207,13 +218,33 @@ int tbk_leaf_sum(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t
                     (const T *)table, row_bytes, width, plan.lanes_log2, (T *)out, ld_out, plan.cluster);
     }
     float *parts = (float *)ws;
-    TRY(launch(tb::tb_leaf_sum_kernel<T, V>, dim3((unsigned)plan.work.blocks, plan.columns), plan.threads, 0, stream, 1, map->view, ids, ld_ids, (const T *)table, row_bytes,
-               width, plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, n, plan.work));
+    tb::LeafStretch work = plan.work;
+    int tile_rows = plan.tile_rows;
+    if (V == 16 && plan.staged(map->max_rows, row_bytes) && ld_table == width && n < kMost) {
+      const int stage_bytes = (int)(map->max_rows * row_bytes), stages = std::min(tb::kLeafMaxStages, kLeafStagedSmem / (stage_bytes + tb::kLeafZeros));
+      const int smem = tb::kLeafStagedFixed + stages * (stage_bytes + tb::kLeafZeros);
+      const bool vec_ids = reinterpret_cast<uintptr_t>(ids) % 16 == 0 && ld_ids % 4 == 0;
+      work = plan.staged_work, tile_rows = (int)plan.staged_rows;
+      CUDA_TRY(cudaFuncSetAttribute(tb::tb_leaf_sum_staged_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, tb::kLeafStagedFixed + kLeafStagedSmem));
+      TRY(launch(tb::tb_leaf_sum_staged_kernel<T>, dim3((unsigned)work.blocks), tb::kLeafStagedThreads, smem, stream, 1, map->view, ids, ld_ids, vec_ids, (const T *)table,
+                 row_bytes, (int)width, plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, (int)n, work, stages, stage_bytes));
+    } else {
+      TRY(launch(tb::tb_leaf_sum_kernel<T, V>, dim3((unsigned)work.blocks, plan.columns), plan.threads, 0, stream, 1, map->view, ids, ld_ids, (const T *)table, row_bytes, width,
+                 plan.lanes_log2, (T *)out, ld_out, parts, plan.ld_parts, n, work));
+    }
     if (plan.max_parts)
-      TRY(launch(tb::tb_leaf_sum_join_kernel<T, V>, (unsigned)tiles_of(n * plan.ld_parts / tb::Share<T, V>::kElems, 256), 256, 0, stream, 1, parts, plan.ld_parts, plan.tile_rows,
-                 (T *)out, ld_out, width, n, plan.work));
+      TRY(launch(tb::tb_leaf_sum_join_kernel<T, V>, (unsigned)tiles_of(n * plan.ld_parts / tb::Share<T, V>::kElems, 256), 256, 0, stream, 1, parts, plan.ld_parts, tile_rows,
+                 (T *)out, ld_out, width, n, work));
     return (int)TBK_OK;
   });
+}
+
+// The status word of the staged leaf sum (see tbk_leaf_check_status).
+int leaf_sum_status(int *word) {
+  int zero = 0;
+  CUDA_TRY(cudaMemcpyFromSymbol(word, tb::tb_leaf_status, sizeof *word));
+  if (*word) CUDA_TRY(cudaMemcpyToSymbol(tb::tb_leaf_status, &zero, sizeof zero));
+  return TBK_OK;
 }
 
 int tbk_leaf_sum_backward_workspace(const tbk_leaf_map *map, int64_t n, int64_t width, int32_t type, uint64_t *bytes) {

@@ -24,13 +24,17 @@ struct LeafMapView {
   long long num_trees;
 };
 
-// Table row of node `id` of a tree; -1: the id is no leaf of it.
-__device__ __forceinline__ int32_t leaf_row(const uint2 *words, int2 tree, int32_t id) {
-  if ((uint32_t)id >= (uint32_t)tree.y) return -1;
-  const uint2 w = __ldg(words + tree.x + (id >> 5));
-  const uint32_t bit = 1u << (id & 31);
-  return w.x & bit ? (int32_t)(w.y + __popc(w.x & (bit - 1))) : -1;
+// Table row of node `id` of a tree; -1: the id is no leaf of it.  Without branches, so that many can be under way; an
+// id beyond the tree reads the tree's first word for nothing.
+__device__ __forceinline__ uint2 leaf_word(const uint2 *words, int2 tree, int32_t id) {
+  return __ldg(words + tree.x + ((uint32_t)id < (uint32_t)tree.y ? id >> 5 : 0));
 }
+__device__ __forceinline__ int32_t leaf_row(uint2 word, int2 tree, int32_t id) {
+  const uint32_t bit = 1u << (id & 31);
+  const int32_t r = (int32_t)(word.y + __popc(word.x & (bit - 1)));
+  return (uint32_t)id < (uint32_t)tree.y && (word.x & bit) ? r : -1;
+}
+__device__ __forceinline__ int32_t leaf_row(const uint2 *words, int2 tree, int32_t id) { return leaf_row(leaf_word(words, tree, id), tree, id); }
 
 // A lane's share of a row: 16 bytes' worth of columns, moved V bytes at a time (V divides the rows' addresses
 // and lengths, so that a piece is inside a row or outside of it as a whole).  Sums are kept as pairs, which the
@@ -123,11 +127,18 @@ __global__ void __launch_bounds__(kLeafRowThreads) tb_leaf_sum_row_kernel(LeafMa
   unsigned long long acc[P] = {};
   for (long long t0 = 0; t0 < m.num_trees; t0 += (long long)groups * 8) {
     int32_t r[8];
+    int2 tree[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long long t = t0 + (long long)i * groups + group;
-      r[i] = t < m.num_trees ? leaf_row(m.words, __ldg(m.trees + t), __ldg(id + t)) : -1;
+      tree[i] = t < m.num_trees ? __ldg(m.trees + t) : make_int2(0, 0);
+      r[i] = t < m.num_trees ? __ldg(id + t) : -1;
     }
+    uint2 word[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[i] = leaf_word(m.words, tree[i], r[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = leaf_row(word[i], tree[i], r[i]);
     uint4 q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = r[i] >= 0 ? S::load(from + (unsigned long long)r[i] * row_bytes, c, width) : make_uint4(0, 0, 0, 0);
@@ -258,6 +269,208 @@ __global__ void __launch_bounds__(512, 1) tb_leaf_sum_kernel(LeafMapView m, cons
     u += b1 - b0;
   }
 }
+// The same where a tree's table rows fit a stage of shared memory and lie one behind the other, and where a row
+// takes a quarter of a warp at least.  One warp copies the tables of the trees to come into a ring of stages, one
+// bulk copy a tree; three look up, eight trees at a time, where in its stage each batch row's table row will lie;
+// twelve add up, a lane group its eight rows: an address and a read of 30 cycles each, instead of the hundreds of an
+// L1 miss.  A table is copied once for a block's tile of rows.  Waits are bounded: one that gives up sets
+// tb_leaf_status.
+__device__ int tb_leaf_status;
+constexpr int kLeafAdders = 12, kLeafFinders = 3, kLeafStagedThreads = 32 * (kLeafAdders + kLeafFinders + 1);
+constexpr int kLeafBatch = 8, kLeafSlots = 3, kLeafMaxStages = 16, kLeafMostRows = 384;
+constexpr int kLeafStagedFixed = 512 + kLeafSlots * kLeafBatch * kLeafMostRows * 2; // barriers; places, in units of 16 bytes
+constexpr int kLeafZeros = 512; // behind each stage: what an id that is no leaf adds
+__device__ __forceinline__ bool leaf_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool leaf_wait(uint32_t bar, uint32_t parity) { // two seconds at most
+  if (leaf_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (leaf_try(bar, parity)) return true;
+    if ((i & 63) == 0 && clock64() - t0 > 4000000000ll) return false;
+  }
+}
+__device__ __forceinline__ void leaf_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+template <class T>
+__global__ void __launch_bounds__(kLeafStagedThreads, 1)
+    tb_leaf_sum_staged_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, bool vec_ids, const T *table, uint32_t row_bytes, int width, int lanes_log2,
+                              T *out, long long ld_out, float *parts, long long ld_parts, int n_rows, LeafStretch work, int stages, int stage_bytes) {
+  using S = Share<T, 16>;
+  constexpr int P = S::kPairs;
+  extern __shared__ __align__(16) unsigned char raw[];
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(raw), full = base, empty = base + 128, found = base + 256, used = base + 256 + 8 * kLeafSlots;
+  uint16_t *places = reinterpret_cast<uint16_t *>(raw + 512); // [slot][tree of the batch][row of the tile]
+  const uint32_t stage0 = base + kLeafStagedFixed;
+  const int pitch = stage_bytes + kLeafZeros, warp = threadIdx.x / 32, wl = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full + 8 * i) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty + 8 * i), "r"(kLeafAdders) : "memory");
+    }
+    for (int i = 0; i < kLeafSlots; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(found + 8 * i), "r"(kLeafFinders) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(used + 8 * i), "r"(kLeafAdders) : "memory");
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int i = threadIdx.x; i < stages * (kLeafZeros / 4); i += kLeafStagedThreads)
+    *reinterpret_cast<uint32_t *>(raw + kLeafStagedFixed + (i / (kLeafZeros / 4)) * pitch + stage_bytes + i % (kLeafZeros / 4) * 4) = 0;
+  __syncthreads();
+  after_previous_kernel();
+  const int lanes = 1 << lanes_log2, groups = (32 * kLeafAdders) >> lanes_log2, tile_rows = groups * kLeafRows;
+  const int batches = (int)work.batches, trees = (int)m.num_trees;
+  const long long u0 = work.begin(blockIdx.x);
+  const int units = (int)(work.begin(blockIdx.x + 1) - u0), tile0 = (int)(u0 / batches), batch0 = (int)(u0 - (long long)tile0 * batches);
+  bool ok = true;
+  if (warp == kLeafAdders + kLeafFinders) {
+    int stage = 0;
+    uint32_t phase = 0;
+    auto fetch = [&](int b) { return __ldg(m.rows + min(b * kLeafBatch + wl, trees)); }; // lanes 0 to 8: where tables begin
+    int32_t next = fetch(batch0); // (a batch ahead: a load per tree would be longer than its copy)
+    for (int u = 0, b = batch0; ok && u < units; ++u) {
+      const int now = min(kLeafBatch, trees - b * kLeafBatch);
+      const int32_t begin = next;
+      if (++b == batches) b = 0;
+      next = fetch(b);
+      for (int j = 0; j < now; ++j) {
+        const int32_t first = __shfl_sync(~0u, begin, j);
+        const uint32_t bytes = (uint32_t)(__shfl_sync(~0u, begin, j + 1) - first) * row_bytes;
+        if (!(ok = __all_sync(~0u, leaf_wait(empty + 8 * stage, phase ^ 1)))) break;
+        if (wl == 0) {
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * stage), "r"(bytes) : "memory");
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(stage0 + stage * pitch), "l"(reinterpret_cast<const unsigned char *>(table) + (unsigned long long)first * row_bytes), "r"(bytes),
+                         "r"(full + 8 * stage) : "memory");
+        }
+        if (++stage == stages) stage = 0, phase ^= 1;
+      }
+    }
+    if (!ok) // copies in flight land before the block ends
+      for (int i = 0; i < stages; ++i) {
+        if (stage-- == 0) stage = stages - 1, phase ^= 1;
+        leaf_wait(full + 8 * stage, phase);
+      }
+  } else if (warp >= kLeafAdders) {
+    int slot = 0;
+    uint32_t phase = 0;
+    const uint32_t none = (uint32_t)stage_bytes / 16, row_units = row_bytes / 16;
+    constexpr int kMost = kLeafMostRows / 32 / kLeafFinders;
+    const int row0 = (warp - kLeafAdders) * 32 + wl; // and every kLeafFinders * 32 rows
+    int32_t id[kMost][kLeafBatch], next[kMost][kLeafBatch];
+    int2 tree, next_tree; // of a batch's tree: lanes 0 to 7 have one each
+    int32_t first, next_first;
+    auto fetch = [&](int tile, int b) { // a batch's ids, one batch ahead of their use
+      const int t0 = b * kLeafBatch, now = min(kLeafBatch, trees - t0);
+#pragma unroll
+      for (int k = 0; k < kMost; ++k) {
+        const int row = row0 + kLeafFinders * 32 * k;
+        // (what is behind the tile's or the batch's last row is not kept)
+        const int32_t *at = ids + (long long)min(tile * tile_rows + min(row, tile_rows - 1), n_rows - 1) * ld_ids + t0;
+        if (vec_ids && now == kLeafBatch) {
+          const int4 a = __ldg(reinterpret_cast<const int4 *>(at)), b = __ldg(reinterpret_cast<const int4 *>(at) + 1);
+          next[k][0] = a.x, next[k][1] = a.y, next[k][2] = a.z, next[k][3] = a.w, next[k][4] = b.x, next[k][5] = b.y, next[k][6] = b.z, next[k][7] = b.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kLeafBatch; ++j) next[k][j] = j < now ? __ldg(at + j) : -1;
+        }
+      }
+      const bool there = wl < now; // (of the trees behind the last one nothing is found)
+      next_tree = there ? __ldg(m.trees + t0 + wl) : make_int2(0, 0);
+      next_first = there ? __ldg(m.rows + t0 + wl) : 0;
+    };
+    if (units) fetch(tile0, batch0);
+    for (int u = 0, tile = tile0, b = batch0; ok && u < units; ++u) {
+#pragma unroll
+      for (int k = 0; k < kMost; ++k)
+#pragma unroll
+        for (int j = 0; j < kLeafBatch; ++j) id[k][j] = next[k][j];
+      tree = next_tree, first = next_first;
+      if (++b == batches) b = 0, ++tile;
+      if (u + 1 < units) fetch(tile, b);
+      if (!(ok = __all_sync(~0u, leaf_wait(used + 8 * slot, phase ^ 1)))) break;
+      uint16_t *to = places + slot * kLeafBatch * kLeafMostRows + row0;
+#pragma unroll
+      for (int j0 = 0; j0 < kLeafBatch; j0 += 4) {
+        uint2 word[4][kMost]; // (sixteen reads under way)
+        int2 of[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          of[j] = make_int2(__shfl_sync(~0u, tree.x, j0 + j), __shfl_sync(~0u, tree.y, j0 + j));
+#pragma unroll
+          for (int k = 0; k < kMost; ++k) word[j][k] = leaf_word(m.words, of[j], id[k][j0 + j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int32_t from = __shfl_sync(~0u, first, j0 + j);
+#pragma unroll
+          for (int k = 0; k < kMost; ++k) {
+            const int32_t r = leaf_row(word[j][k], of[j], id[k][j0 + j]);
+            if (row0 + kLeafFinders * 32 * k < tile_rows) to[(j0 + j) * kLeafMostRows + kLeafFinders * 32 * k] = (uint16_t)(r < 0 ? none : (uint32_t)(r - from) * row_units);
+          }
+        }
+      }
+      __syncwarp();
+      if (wl == 0) leaf_arrive(found + 8 * slot);
+      if (++slot == kLeafSlots) slot = 0, phase ^= 1;
+    }
+  } else {
+    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2;
+    const int c = lane * S::kElems;
+    int stage = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0;
+    int tile = tile0, b0 = batch0;
+    for (int u = 0; ok && u < units; ++tile, b0 = 0) {
+      const int b1 = min(batches, b0 + (units - u));
+      unsigned long long acc[kLeafRows][P] = {};
+      for (int b = b0; ok && b < b1; ++b) {
+        const int now = min(kLeafBatch, trees - b * kLeafBatch);
+        if (!(ok = __all_sync(~0u, leaf_wait(found + 8 * slot, slot_phase)))) break;
+        const uint16_t *place = places + slot * kLeafBatch * kLeafMostRows + group * kLeafRows;
+        for (int j = 0; j < now; ++j) {
+          const uint4 o = *reinterpret_cast<const uint4 *>(place + j * kLeafMostRows);
+          if (!(ok = __all_sync(~0u, leaf_wait(full + 8 * stage, phase)))) break;
+          const uint32_t at = stage0 + stage * pitch + lane * 16, w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int h = 0; h < kLeafRows; h += 4) {
+            uint4 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t v = w[(h + i) / 2], from = at + (i % 2 ? v >> 16 : v & 0xffffu) * 16;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w) : "r"(from));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S::add(acc[h + i], q[i]);
+          }
+          __syncwarp();
+          if (wl == 0) leaf_arrive(empty + 8 * stage);
+          if (++stage == stages) stage = 0, phase ^= 1;
+        }
+        if (wl == 0) leaf_arrive(used + 8 * slot);
+        if (++slot == kLeafSlots) slot = 0, slot_phase ^= 1;
+      }
+      const bool whole = b0 == 0 && b1 == batches;
+      const long long part = whole ? 0 : blockIdx.x - work.block_of((long long)tile * batches);
+#pragma unroll
+      for (int i = 0; i < kLeafRows; ++i) {
+        const long long n = (long long)tile * tile_rows + group * kLeafRows + i;
+        if (n >= n_rows) break;
+        if (whole) {
+          S::store(out + n * ld_out + c, c, width, acc[i]);
+        } else if (c < ld_parts) {
+          unsigned long long *d = reinterpret_cast<unsigned long long *>(parts + (part * n_rows + n) * ld_parts + c);
+#pragma unroll
+          for (int k = 0; k < P; ++k) d[k] = acc[i][k];
+        }
+      }
+      u += b1 - b0;
+    }
+  }
+  if (!ok) atomicExch(&tb_leaf_status, 4);
+}
 // Adds the parts of the tiles that several blocks had, in order.
 template <class T, int V>
 __global__ void __launch_bounds__(256) tb_leaf_sum_join_kernel(const float *parts, long long ld_parts, int tile_rows, T *out, long long ld_out,
@@ -287,29 +500,37 @@ constexpr int kNumberRows = 128;
 template <class N>
 __global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, const int32_t *ids, long long ld_ids, N *numbers, long long ld,
                                                               long long n_rows) {
-  __shared__ int32_t tile[32][kNumberRows + 1];
+  __shared__ int2 tile[32][kNumberRows / 2 + 1]; // [tree][pair of rows]
   after_previous_kernel();
   const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-  const long long t0 = (long long)blockIdx.y * 32;
+  const int t0 = blockIdx.y * 32, trees = (int)min(32ll, m.num_trees - t0);
   for (long long n0 = (long long)blockIdx.x * kNumberRows; n0 < n_rows; n0 += (long long)gridDim.x * kNumberRows) {
+    const int rows = (int)min((long long)kNumberRows, n_rows - n0);
     __syncthreads();
     const int32_t *from = ids + n0 * ld_ids + t0 + x;
-    int32_t v[kNumberRows / 8];
+    int32_t v[kNumberRows / 8]; // of rows 16 i + 2 y and the next
 #pragma unroll
-    for (int i = 0; i < kNumberRows / 8; ++i) v[i] = n0 + y + 8 * i < n_rows && t0 + x < m.num_trees ? __ldg(from + (y + 8 * i) * ld_ids) : -1;
+    for (int i = 0; i < kNumberRows / 8; ++i) {
+      const int row = i / 2 * 16 + 2 * y + i % 2;
+      v[i] = row < rows && x < trees ? __ldg(from + row * ld_ids) : -1;
+    }
 #pragma unroll
-    for (int i = 0; i < kNumberRows / 8; ++i) tile[x][y + 8 * i] = v[i];
+    for (int i = 0; i < kNumberRows / 16; ++i) tile[x][i * 8 + y] = make_int2(v[2 * i], v[2 * i + 1]);
     __syncthreads();
+    for (int i = y; i < trees; i += 8) {
+      const int2 tree = __ldg(m.trees + t0 + i);
+      const int32_t first = __ldg(m.rows + t0 + i);
+      N *to = numbers + (t0 + i) * ld + n0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long t = t0 + y * 4 + i;
-      if (t >= m.num_trees) break;
-      const int2 tree = __ldg(m.trees + t);
-      const int32_t first = __ldg(m.rows + t);
-#pragma unroll
-      for (int k = 0; k < kNumberRows / 32; ++k) {
-        const int32_t r = leaf_row(m.words, tree, tile[y * 4 + i][x + 32 * k]);
-        if (n0 + x + 32 * k < n_rows) numbers[t * ld + n0 + x + 32 * k] = r < 0 ? (N)~(N)0 : (N)(r - first);
+      for (int k = 0; k < kNumberRows / 64; ++k) {
+        const int2 id = tile[i][x + 32 * k];
+        const int32_t a = leaf_row(m.words, tree, id.x), b = leaf_row(m.words, tree, id.y);
+        const N pair[2] = {a < 0 ? (N)~(N)0 : (N)(a - first), b < 0 ? (N)~(N)0 : (N)(b - first)};
+        const int row = 2 * (x + 32 * k); // (ld is a multiple of 8: the second of a pair is there, used or not)
+        if (row < rows) {
+          if constexpr (sizeof(N) == 2) *reinterpret_cast<uint32_t *>(to + row) = *reinterpret_cast<const uint32_t *>(pair);
+          else *reinterpret_cast<uint2 *>(to + row) = *reinterpret_cast<const uint2 *>(pair);
+        }
       }
     }
   }
@@ -321,13 +542,14 @@ __global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, con
 // which add up runs of equal leaves.  A leaf inside one group's stretch is finished there; the ends of
 // stretches are joined in order afterwards.  Batches above kLeafChunk rows come in pieces, with fp32 sums in
 // `sums` in between.
-constexpr int kLeafRange = 1024, kLeafChunk = 32768, kLeafGradWarps = 8;
+constexpr int kLeafRange = 1024, kLeafChunk = 32768, kLeafGradWarps = 16;
 constexpr int kLeafGradFixed = kLeafRange * 4 + 16;
 __host__ __device__ constexpr int leaf_grad_smem(int chunk, int range) { // counters and, after them, the ends of stretches share their place
-  return kLeafGradFixed + (kLeafGradWarps * range * 4 > 8192 ? kLeafGradWarps * range * 4 : 8192) + (chunk + 15) / 8 * 16; // order: two bytes a row
+  return kLeafGradFixed + (kLeafGradWarps * range * 4 > kLeafGradWarps * 1024 ? kLeafGradWarps * range * 4 : kLeafGradWarps * 1024) +
+         (chunk + 15) / 8 * 16; // order: two bytes a row
 }
 template <class T, int V, class N>
-__global__ void __launch_bounds__(32 * kLeafGradWarps, 3) tb_leaf_grad_kernel(LeafMapView m, const N *numbers, long long ld_numbers, const T *grad,
+__global__ void __launch_bounds__(32 * kLeafGradWarps, 2) tb_leaf_grad_kernel(LeafMapView m, const N *numbers, long long ld_numbers, const T *grad,
                                                                               uint32_t row_bytes, long long width, int lanes_log2, float *sums, T *out,
                                                                               long long ld_out, long long n_rows, int chunk, int range) {
   using S = Share<T, V>;
@@ -402,20 +624,31 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 3) tb_leaf_grad_kernel(Le
       uint32_t ls[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) ls[k] = i0 + 32 * k + wl < to ? (uint32_t)__ldg(mine + b0 + i0 + 32 * k + wl) : kNone;
+      // (the equal ones of 32 rows get their places from one of them, whose counter tells how many came before;
+      // a warp's additions to a counter happen in the order of the program, so all eight can be under way)
+      uint32_t same[kAhead], at[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (i0 + 32 * k >= to) break;
-        const uint32_t l = ls[k] == kNone || ls[k] - first_leaf >= (uint32_t)leaves ? kNone : ls[k] - first_leaf;
-        const uint32_t same = __match_any_sync(~0u, l);
-        const uint32_t rank = __popc(same & ((1u << wl) - 1));
-        uint32_t at = 0;
-        if (l != kNone) at = own[l];
-        __syncwarp();
-        if (l != kNone) {
-          order[at + rank] = (uint16_t)(i0 + 32 * k + wl);
-          if (rank == 0) own[l] = at + __popc(same);
+        ls[k] = ls[k] == kNone || ls[k] - first_leaf >= (uint32_t)leaves ? kNone : ls[k] - first_leaf;
+        const uint32_t there = __ballot_sync(~0u, ls[k] != kNone);
+        same[k] = ls[k] != kNone ? there : ~there;
+      }
+      for (int b = 0; (1 << b) < leaves; ++b) // (a vote a bit: several times faster than a match instruction)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const bool set = ls[k] >> b & 1;
+          const uint32_t with = __ballot_sync(~0u, set);
+          same[k] &= set ? with : ~with;
         }
-        __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const bool leads = (same[k] & ((1u << wl) - 1)) == 0 && ls[k] != kNone;
+        at[k] = leads ? atomicAdd(own + ls[k], (uint32_t)__popc(same[k])) : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint32_t place = __shfl_sync(~0u, at[k], __ffs(same[k]) - 1) + __popc(same[k] & ((1u << wl) - 1));
+        if (ls[k] != kNone) order[place] = (uint16_t)(i0 + 32 * k + wl);
       }
     }
     __syncthreads();
