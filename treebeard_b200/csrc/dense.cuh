@@ -971,13 +971,13 @@ template <class T, int COLS> struct LseEnd {
   }
 };
 
-// A row's logarithm and loss from its parts: a lane per row, the parts over the block's warps.
+// A row's logarithm and loss from its parts: a lane per row, the parts over the block's warps (kJoinWarps at most).
 constexpr int kJoinWarps = 32;
 __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const float2 *parts, int count, const float *at, const void *labels, int label_bytes,
                                                                        long long classes, float *loss, float *lse, long long rows) {
   __shared__ float2 mine[kJoinWarps][32];
   after_previous_kernel();
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
   const long long m = (long long)blockIdx.x * 32 + lane;
   float top = -INFINITY, sum = 0.f;
   auto join = [&](float2 q) {
@@ -987,13 +987,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const flo
   };
   if (m < rows) {
 #pragma unroll 4
-    for (int t = warp; t < count; t += kJoinWarps) join(parts[(long long)t * rows + m]);
+    for (int t = warp; t < count; t += warps) join(parts[(long long)t * rows + m]);
   }
   mine[warp][lane] = make_float2(top, sum);
   __syncthreads();
   if (warp || m >= rows) return;
 #pragma unroll 4
-  for (int w = 1; w < kJoinWarps; ++w) join(mine[w][lane]);
+  for (int w = 1; w < warps; ++w) join(mine[w][lane]);
   const float l = fmaf(top == -INFINITY ? 0.f : top, kLn2, logf(sum));
   const long long label = label_at(labels, label_bytes, m);
   lse[m] = l;

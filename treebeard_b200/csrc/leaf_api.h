@@ -4,6 +4,7 @@
 #include "last_error.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -95,11 +96,14 @@ int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Multiprocessors of a device; the figure of the architecture where there is none (workspace sizes on a host).
 int multiprocessors(int device) {
+  static std::atomic<int> known[64];
+  if (device >= 0 && device < 64 && known[device].load() > 0) return known[device].load();
   int n = 0;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 2) {
     cudaGetLastError();
     return 148;
   }
+  if (device < 64) known[device].store(n);
   return n;
 }
 

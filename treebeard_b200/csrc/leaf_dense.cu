@@ -22,7 +22,8 @@ template <class F> int with_half(int32_t type, F f) { return type == TBK_TYPE_F1
 
 // How products are cut: into tiles of one of the three shapes of tb_dense_kernel and, where that leaves
 // multiprocessors without work, the sums into parts that a second kernel joins.  Cycles per 64 k of a tile, around a
-// tile and for the join follow measurements; the cheapest cut of a launch's one or two products is taken.
+// tile (`heavy`: with an activation of many instructions a result) and for the join follow measurements; the cheapest
+// cut of a launch's one or two products is taken.
 struct Size {
   int64_t m, n, k;
 };
@@ -30,9 +31,10 @@ struct Cut {
   int shape = tb::kDenseOne;
   int splits[2] = {1, 1};
 };
-Cut plan_products(const Size *sizes, int count, int sms, bool may_split) {
+Cut find_cut(const Size *sizes, int count, int sms, bool may_split, bool heavy) {
   static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
-  constexpr double kPer64[] = {700, 750, 1385}, kAround[] = {900, 900, 2900};
+  constexpr double kPer64[] = {700, 750, 1385};
+  const double kAround[] = {900, heavy ? 3300. : 900., heavy ? 10000. : 2900.};
   Cut best;
   double least = 1e300;
   for (int shape = 0; shape < 3; ++shape) {
@@ -70,9 +72,27 @@ Cut plan_products(const Size *sizes, int count, int sms, bool may_split) {
   }
   return best;
 }
+// The same, remembered: a program's sizes are mostly alike, and a search takes microseconds.
+Cut plan_products(const Size *sizes, int count, int sms, bool may_split, bool heavy = false) {
+  struct Entry {
+    int64_t key[8] = {-1};
+    Cut cut;
+  };
+  static thread_local Entry entries[64];
+  int64_t key[8] = {count * 4 + may_split * 2 + heavy, sms, sizes[0].m, sizes[0].n, sizes[0].k, 0, 0, 0};
+  if (count > 1) key[5] = sizes[1].m, key[6] = sizes[1].n, key[7] = sizes[1].k;
+  uint64_t h = 0;
+  for (const int64_t k : key) h = (h ^ (uint64_t)k) * 0x9e3779b97f4a7c15ull;
+  Entry &e = entries[h >> 58];
+  if (std::memcmp(e.key, key, sizeof key) != 0) {
+    e.cut = find_cut(sizes, count, sms, may_split, heavy);
+    std::memcpy(e.key, key, sizeof key);
+  }
+  return e.cut;
+}
 // fp32 room for the parts of a launch's products
-uint64_t part_floats(const Size *sizes, int count, int sms) {
-  const Cut cut = plan_products(sizes, count, sms, true);
+uint64_t part_floats(const Size *sizes, int count, int sms, bool heavy = false) {
+  const Cut cut = plan_products(sizes, count, sms, true, heavy);
   uint64_t sum = 0;
   for (int i = 0; i < count; ++i)
     if (cut.splits[i] > 1) sum += (uint64_t)cut.splits[i] * sizes[i].m * up8(sizes[i].n);
@@ -178,7 +198,8 @@ int products(const Product<T> *list, int count, const ColumnSums<T> &sums, float
   if (count) {
     Size sizes[2];
     for (int i = 0; i < count; ++i) sizes[i] = list[i].size;
-    const Cut cut = plan_products(sizes, count, sms, true);
+    const bool heavy = list[0].end.act >= tb::kActGelu; // (a layer's product is alone)
+    const Cut cut = plan_products(sizes, count, sms, true, heavy);
     tb::DenseJobs<tb::ResultEnd<T>, 2> jobs;
     for (int i = 0; i < count; ++i) {
       const Product<T> &x = list[i];
@@ -269,11 +290,11 @@ typedef unsigned short Half; // an element of either 16-bit type
 struct LinearParts {
   Half *x, *weight;
   float *parts;
-  LinearParts(Parts &w, int64_t n, int64_t inputs, int64_t outputs, bool aligned, int sms)
-      : x(w.take<Half>(aligned ? 0 : n * up8(inputs))), weight(w.take<Half>(aligned ? 0 : outputs * up8(inputs))),
-        parts(nullptr) {
+  LinearParts(Parts &w, int64_t n, int64_t inputs, int64_t outputs, bool aligned, int sms) : x(nullptr), weight(nullptr), parts(nullptr) {
+    if (n <= tb::kFewRows) return; // (read and written as they are)
     const Size size{n, outputs, inputs};
-    parts = w.take<float>(n > 0 ? part_floats(&size, 1, sms) : 0);
+    x = w.take<Half>(aligned ? 0 : n * up8(inputs)), weight = w.take<Half>(aligned ? 0 : outputs * up8(inputs));
+    parts = w.take<float>(std::max(part_floats(&size, 1, sms), part_floats(&size, 1, sms, true)));
   }
 };
 struct LinearGradParts {
@@ -509,7 +530,7 @@ int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_w
     };
     if (parts.cut.shape == tb::kDenseOne) TRY(scores(std::integral_constant<int, 32>()));
     else TRY(scores(std::integral_constant<int, 64>()));
-    return launch(tb::tb_loss_join_kernel, (unsigned)tiles_of(n, 32), 32 * tb::kJoinWarps, 0, stream, 1, parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss,
+    return launch(tb::tb_loss_join_kernel, (unsigned)tiles_of(n, 32), 32 * (unsigned)std::clamp(parts.cut.parts / 4, 1, tb::kJoinWarps), 0, stream, 1, parts.part, parts.cut.parts, parts.at, labels, label_bytes, classes, loss,
                   lse, n);
   });
 }

@@ -12,24 +12,24 @@ The reference ends at the forest's own prediction and has no counterpart.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
+
+import torch
 
 from . import kernels
-from .kernels import TbkError, _stream_ptr, _torch
+from .kernels import TbkError, _stream_ptr
 
 ACTIVATIONS = {"identity": 0, "relu": 1, "gelu": 2, "silu": 3}
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INVALID, _UNSUPPORTED = 1, 3
-_bound = False
-_types = {}
+_lib = None
 
 
 def lib():
-    global _bound
-    L = kernels.lib()
-    if not _bound:
-        torch = _torch()
-        _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    global _lib
+    if _lib is None:
+        L = kernels.lib()
         vp, i64, i32, u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint64
         size = ctypes.POINTER(u64)
         L.tbk_leaf_map_create.argtypes = [vp, i32, ctypes.POINTER(vp)]
@@ -49,8 +49,8 @@ def lib():
         L.tbk_class_loss.argtypes = [vp, i64, vp, i64, vp, vp, i32, vp, vp, i64, i64, i64, i32, vp, u64, i32, vp]
         L.tbk_class_loss_backward.argtypes = [vp, vp, i64, vp, i64, vp, vp, i32, vp, vp, i64, vp, i64, vp, i64, i64, i64,
                                               i32, vp, u64, i32, vp]
-        _bound = True
-    return L
+        _lib = L
+    return _lib
 
 
 def _check(rc):
@@ -64,36 +64,40 @@ def _refuse(message):
 
 def _matrix(name, t, dtype, rows=None, cols=None):
     """Checks a row-major matrix; returns its row stride."""
-    if t.dim() != 2 or t.dtype is not dtype:
+    shape = t.shape
+    if len(shape) != 2 or t.dtype is not dtype:
         _refuse(f"{name}: a 2-d tensor of {dtype} is wanted, not {t.dim()}-d of {t.dtype}")
-    n, m = t.shape
+    n, m = shape
     if (rows is not None and n != rows) or (cols is not None and m != cols):
         _refuse(f"{name} has shape ({n}, {m}), wanted are ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
     ld, step = t.stride()
+    if ld >= m and (step == 1 or m == 1):
+        return ld
     if n and ((step != 1 and m > 1) or (ld < m and n > 1)):
         _refuse(f"{name}: the elements of a row have to lie one behind the other, the rows apart")
-    return max(ld, m)
+    return m
 
 
 def _vector(name, t, dtype, length):
-    if t.dim() != 1 or t.dtype is not dtype or t.shape[0] != length:
+    if t.shape != (length,) or t.dtype is not dtype:
         _refuse(f"{name}: {length} elements of {dtype} are wanted, not {tuple(t.shape)} of {t.dtype}")
-    if t.stride(0) != 1 and length > 1:
+    if length > 1 and t.stride(0) != 1:
         _refuse(f"{name}: the elements have to lie one behind the other")
 
 
-def _device(*tensors):
-    """The CUDA device that all tensors lie on."""
-    device = tensors[0].device
+def _device(first, *tensors):
+    """Number of the CUDA device that all tensors lie on."""
+    index = first.get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != device):
-            _refuse("all tensors have to be on one CUDA device")
-    return device
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        _refuse("all tensors have to be on one CUDA device")
+    return index
 
 
 def _half(t, what):
-    lib()
-    kind = _types.get(t.dtype)
+    kind = _TYPES.get(t.dtype)
     if kind == 0:
         raise TbkError(_UNSUPPORTED, f"{what} takes 16-bit floating point types (fp16, bf16)")
     if kind is None:
@@ -116,19 +120,31 @@ def _apart(name, out, *inputs):
                 _refuse(f"{name} overlaps another tensor of the call")
 
 
-def _on(stream):
-    """Where a call's own memory comes from: the stream that its work is ordered by."""
-    return _torch().cuda.stream(stream) if stream is not None else contextlib.nullcontext()
+def _on_stream(call):
+    """``stream=`` of a call: the stream that its work is ordered by and its own memory comes from."""
+    @functools.wraps(call)
+    def wrapper(*args, stream=None, **kwargs):
+        if stream is None:
+            return call(*args, **kwargs)
+        with torch.cuda.stream(stream):
+            return call(*args, **kwargs)
+    return wrapper
 
 
-def _workspace(name, device, *sizes):
+@functools.lru_cache(maxsize=1024)
+def _size(function, *sizes):
+    """Bytes of a call's workspace: a function of its sizes alone."""
     need = ctypes.c_uint64()
-    _check(getattr(lib(), name + "_workspace")(*sizes, ctypes.byref(need)))
-    if not need.value:
-        return None, None, 0
-    torch = _torch()
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr(), need.value
+    _check(getattr(lib(), function)(*sizes, ctypes.byref(need)))
+    return need.value
+
+
+def _workspace(like, size):
+    """(tensor to keep until the call returns, its address)"""
+    if not size:
+        return None, None
+    ws = like.new_empty(size, dtype=torch.uint8)
+    return ws, ws.data_ptr()
 
 
 def _readable(x, ld_x, weight, ld_w):
@@ -137,7 +153,7 @@ def _readable(x, ld_x, weight, ld_w):
 
 
 def check_status(device: int = 0):
-    """Waits for the device; raises TbkError if a bounded wait inside a matrix product gave up since the last check."""
+    """Waits for the device; raises TbkError if a bounded wait inside one of these kernels gave up since the last check."""
     _check(lib().tbk_leaf_check_status(device))
 
 
@@ -158,6 +174,7 @@ class LeafMap:
         self.device = device
         self.num_trees = len(keep[0]) - 1
         self.num_rows = int(lib().tbk_leaf_map_rows(h))
+        self._size = functools.lru_cache(maxsize=256)(lambda function, *sizes: _size.__wrapped__(function, h, *sizes))
 
     def close(self):
         if getattr(self, "_h", None):
@@ -171,126 +188,126 @@ class LeafMap:
 
 
 def _leaf_call(leaves, ids, other, what):
-    torch = _torch()
-    lib()
     ld = _matrix("ids", ids, torch.int32, None, leaves.num_trees)
-    if other.dtype not in _types:
+    kind = _TYPES.get(other.dtype)
+    if kind is None:
         _refuse(f"{what}: {other.dtype} is no type of an embedding table")
     device = _device(ids, other)
-    if device.index != leaves.device:
-        _refuse(f"the leaf map is on device {leaves.device}, the tensors on {device.index}")
-    return ld, device
+    if device != leaves.device:
+        _refuse(f"the leaf map is on device {leaves.device}, the tensors on {device}")
+    return ld, device, kind
 
 
-def leaf_sum(leaves: LeafMap, ids, table, out=None, stream=None):
+@_on_stream
+def leaf_sum(leaves: LeafMap, ids, table, out=None):
     """out[n] = sum over trees of the table row of the leaf that row n reached.  ids: int32 [n, trees] as
     predict_leaf_ids gives them; an id that is no leaf of its tree (-1 for a padded row) adds nothing.
     table: [leaves.num_rows, width], fp32, fp16 or bf16.  Returns [n, width] of table's type."""
-    torch = _torch()
     ld_table = _matrix("table", table, table.dtype, leaves.num_rows)
-    ld_ids, device = _leaf_call(leaves, ids, table, "leaf_sum")
-    n, width, kind = ids.shape[0], table.shape[1], _types[table.dtype]
-    with _on(stream):
-        if out is None:
-            out = torch.empty((n, width), dtype=table.dtype, device=device)
-        else:
-            _device(ids, out)
-            _apart("out", out, ids, table)
+    ld_ids, device, kind = _leaf_call(leaves, ids, table, "leaf_sum")
+    n, width = ids.shape[0], table.shape[1]
+    if out is None:
+        out, ld_out = table.new_empty((n, width)), width
+    else:
         ld_out = _matrix("out", out, table.dtype, n, width)
-        keep, ws, size = _workspace("tbk_leaf_sum", device, leaves._h, n, width, kind)
-        _check(lib().tbk_leaf_sum(leaves._h, ids.data_ptr(), n, ld_ids, table.data_ptr(), ld_table, width, kind,
-                                  out.data_ptr(), ld_out, ws, size, _stream_ptr(stream, device.index)))
+        _device(ids, out)
+        _apart("out", out, ids, table)
+    L = lib()
+    size = leaves._size("tbk_leaf_sum_workspace", n, width, kind)
+    keep, ws = _workspace(table, size)
+    _check(L.tbk_leaf_sum(leaves._h, ids.data_ptr(), n, ld_ids, table.data_ptr(), ld_table, width, kind, out.data_ptr(), ld_out,
+                          ws, size, _stream_ptr(None, device)))
     return out
 
 
-def leaf_sum_backward(leaves: LeafMap, ids, grad, out=None, stream=None):
+@_on_stream
+def leaf_sum_backward(leaves: LeafMap, ids, grad, out=None):
     """Gradient of leaf_sum with respect to the table, [leaves.num_rows, width] of grad's type, from grad
     [n, width], the gradient of its result."""
-    torch = _torch()
     n, width = ids.shape[0], grad.shape[-1]
     ld_grad = _matrix("grad", grad, grad.dtype, n)
-    ld_ids, device = _leaf_call(leaves, ids, grad, "leaf_sum_backward")
-    kind = _types[grad.dtype]
-    with _on(stream):
-        if out is None:
-            out = torch.empty((leaves.num_rows, width), dtype=grad.dtype, device=device)
-        else:
-            _device(ids, out)
-            _apart("out", out, ids, grad)
+    ld_ids, device, kind = _leaf_call(leaves, ids, grad, "leaf_sum_backward")
+    if out is None:
+        out, ld_out = grad.new_empty((leaves.num_rows, width)), width
+    else:
         ld_out = _matrix("out", out, grad.dtype, leaves.num_rows, width)
-        keep, ws, size = _workspace("tbk_leaf_sum_backward", device, leaves._h, n, width, kind)
-        _check(lib().tbk_leaf_sum_backward(leaves._h, ids.data_ptr(), n, ld_ids, grad.data_ptr(), ld_grad, width, kind,
-                                           out.data_ptr(), ld_out, ws, size, _stream_ptr(stream, device.index)))
+        _device(ids, out)
+        _apart("out", out, ids, grad)
+    L = lib()
+    size = leaves._size("tbk_leaf_sum_backward_workspace", n, width, kind)
+    keep, ws = _workspace(grad, size)
+    _check(L.tbk_leaf_sum_backward(leaves._h, ids.data_ptr(), n, ld_ids, grad.data_ptr(), ld_grad, width, kind, out.data_ptr(), ld_out,
+                                   ws, size, _stream_ptr(None, device)))
     return out
 
 
-def linear(x, weight, bias=None, activation: str = "identity", residual=None, keep_pre: bool = False, out=None,
-           stream=None):
+@_on_stream
+def linear(x, weight, bias=None, activation: str = "identity", residual=None, keep_pre: bool = False, out=None):
     """activation(x weight^T + bias) + residual.  x [n, inputs], weight [outputs, inputs], bias [outputs],
     residual [n, outputs], all fp16 or all bf16; activation: identity, relu, gelu (by the normal
     distribution's integral) or silu.  Returns [n, outputs]; with keep_pre also the value before the
     activation, which linear_backward takes.  out may be residual."""
-    torch = _torch()
     kind = _half(x, "linear")
-    ld_x = _matrix("x", x, x.dtype)
+    dtype = x.dtype
+    ld_x = _matrix("x", x, dtype)
     n, inputs = x.shape
-    ld_w = _matrix("weight", weight, x.dtype, None, inputs)
+    ld_w = _matrix("weight", weight, dtype, None, inputs)
     outputs = weight.shape[0]
     if bias is not None:
-        _vector("bias", bias, x.dtype, outputs)
-    ld_r = _matrix("residual", residual, x.dtype, n, outputs) if residual is not None else 0
-    if activation not in ACTIVATIONS:
+        _vector("bias", bias, dtype, outputs)
+    ld_r = _matrix("residual", residual, dtype, n, outputs) if residual is not None else 0
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         _refuse(f"unknown activation {activation!r}")
     device = _device(x, weight, bias, residual)
-    with _on(stream):
-        if out is None:
-            out = torch.empty((n, outputs), dtype=x.dtype, device=device)
-            ld_o = outputs
-        else:
-            ld_o = _matrix("out", out, x.dtype, n, outputs)
-            _device(x, out)
-            same = residual is not None and out.data_ptr() == residual.data_ptr() and ld_o == ld_r
-            _apart("out", out, x, weight, bias, None if same else residual)
-        pre = torch.empty((n, outputs), dtype=x.dtype, device=device) if keep_pre else None
-        keep, ws, size = _workspace("tbk_linear", device, n, inputs, outputs, kind, _readable(x, ld_x, weight, ld_w), device.index)
-        _check(lib().tbk_linear(x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), ACTIVATIONS[activation],
-                                _ptr(residual), ld_r, out.data_ptr(), ld_o, _ptr(pre), outputs, n, inputs, outputs, kind,
-                                ws, size, device.index, _stream_ptr(stream, device.index)))
+    if out is None:
+        out, ld_o = x.new_empty((n, outputs)), outputs
+    else:
+        ld_o = _matrix("out", out, dtype, n, outputs)
+        _device(x, out)
+        same = residual is not None and out.data_ptr() == residual.data_ptr() and ld_o == ld_r
+        _apart("out", out, x, weight, bias, None if same else residual)
+    pre = x.new_empty((n, outputs)) if keep_pre else None
+    L = lib()
+    size = _size("tbk_linear_workspace", n, inputs, outputs, kind, _readable(x, ld_x, weight, ld_w), device)
+    keep, ws = _workspace(x, size)
+    _check(L.tbk_linear(x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), act, _ptr(residual), ld_r, out.data_ptr(), ld_o,
+                        _ptr(pre), outputs, n, inputs, outputs, kind, ws, size, device, _stream_ptr(None, device)))
     return (out, pre) if keep_pre else out
 
 
-def linear_backward(grad, x, weight, pre=None, activation: str = "identity", bias: bool = True, skip=None,
-                    stream=None):
+@_on_stream
+def linear_backward(grad, x, weight, pre=None, activation: str = "identity", bias: bool = True, skip=None):
     """Gradients of linear from grad, the gradient of its result (which is the residual's gradient too):
     (of x, of weight) and, with ``bias``, of the bias.  pre is what linear kept; identity needs none.
     skip [n, inputs] is added to x's gradient: grad itself, where x was the residual too."""
-    torch = _torch()
     kind = _half(x, "linear_backward")
-    ld_x = _matrix("x", x, x.dtype)
+    dtype = x.dtype
+    ld_x = _matrix("x", x, dtype)
     n, inputs = x.shape
-    ld_w = _matrix("weight", weight, x.dtype, None, inputs)
+    ld_w = _matrix("weight", weight, dtype, None, inputs)
     outputs = weight.shape[0]
-    ld_g = _matrix("grad", grad, x.dtype, n, outputs)
-    if activation not in ACTIVATIONS:
+    ld_g = _matrix("grad", grad, dtype, n, outputs)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         _refuse(f"unknown activation {activation!r}")
-    if pre is None and activation != "identity":
+    if pre is None and act:
         _refuse(f"{activation} needs the values before the activation (pre)")
-    ld_p = _matrix("pre", pre, x.dtype, n, outputs) if pre is not None else 0
-    ld_s = _matrix("skip", skip, x.dtype, n, inputs) if skip is not None else 0
+    ld_p = _matrix("pre", pre, dtype, n, outputs) if pre is not None else 0
+    ld_s = _matrix("skip", skip, dtype, n, inputs) if skip is not None else 0
     device = _device(grad, x, weight, pre, skip)
-    with _on(stream):
-        grad_x, grad_w = torch.empty((n, inputs), dtype=x.dtype, device=device), torch.empty((outputs, inputs), dtype=x.dtype, device=device)
-        grad_b = torch.empty(outputs, dtype=x.dtype, device=device) if bias else None
-        keep, ws, size = _workspace("tbk_linear_backward", device, n, inputs, outputs, kind, _readable(x, ld_x, weight, ld_w), device.index)
-        _check(lib().tbk_linear_backward(grad.data_ptr(), ld_g, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(pre), ld_p,
-                                         ACTIVATIONS[activation], _ptr(skip), ld_s, grad_x.data_ptr(), inputs, grad_w.data_ptr(), inputs,
-                                         _ptr(grad_b), n, inputs, outputs, kind, ws, size, device.index,
-                                         _stream_ptr(stream, device.index)))
+    grad_x, grad_w = x.new_empty((n, inputs)), x.new_empty((outputs, inputs))
+    grad_b = x.new_empty(outputs) if bias else None
+    L = lib()
+    size = _size("tbk_linear_backward_workspace", n, inputs, outputs, kind, _readable(x, ld_x, weight, ld_w), device)
+    keep, ws = _workspace(x, size)
+    _check(L.tbk_linear_backward(grad.data_ptr(), ld_g, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(pre), ld_p, act, _ptr(skip),
+                                 ld_s, grad_x.data_ptr(), inputs, grad_w.data_ptr(), inputs, _ptr(grad_b), n, inputs, outputs, kind,
+                                 ws, size, device, _stream_ptr(None, device)))
     return (grad_x, grad_w, grad_b) if bias else (grad_x, grad_w)
 
 
 def _class_call(what, x, weight, labels, bias):
-    torch = _torch()
     kind = _half(x, what)
     ld_x = _matrix("x", x, x.dtype)
     n, width = x.shape
@@ -304,39 +321,39 @@ def _class_call(what, x, weight, labels, bias):
     return kind, ld_x, ld_w, n, width, classes
 
 
-def class_loss(x, weight, labels, bias=None, stream=None):
+@_on_stream
+def class_loss(x, weight, labels, bias=None):
     """Softmax cross entropy over the classes with scores z = x weight^T + bias, which are never stored.
     x [n, width], weight [classes, width], bias [classes], all fp16 or all bf16; labels [n], int64 or int32:
     a label outside 0 .. classes-1 leaves its row out (loss 0).  Returns fp32 (loss [n], lse [n]) with
     lse = log sum exp z."""
-    torch = _torch()
     kind, ld_x, ld_w, n, width, classes = _class_call("class_loss", x, weight, labels, bias)
     device = _device(x, weight, labels, bias)
-    with _on(stream):
-        loss, lse = torch.empty(n, dtype=torch.float32, device=device), torch.empty(n, dtype=torch.float32, device=device)
-        keep, ws, size = _workspace("tbk_class_loss", device, n, width, classes, kind, _readable(x, ld_x, weight, ld_w), device.index)
-        _check(lib().tbk_class_loss(x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), labels.data_ptr(),
-                                    labels.element_size(), loss.data_ptr(), lse.data_ptr(), n, width, classes, kind, ws, size,
-                                    device.index, _stream_ptr(stream, device.index)))
+    loss, lse = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
+    L = lib()
+    size = _size("tbk_class_loss_workspace", n, width, classes, kind, _readable(x, ld_x, weight, ld_w), device)
+    keep, ws = _workspace(x, size)
+    _check(L.tbk_class_loss(x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), labels.data_ptr(), labels.element_size(),
+                            loss.data_ptr(), lse.data_ptr(), n, width, classes, kind, ws, size, device, _stream_ptr(None, device)))
     return loss, lse
 
 
-def class_loss_backward(grad_loss, x, weight, labels, lse, bias=None, stream=None):
+@_on_stream
+def class_loss_backward(grad_loss, x, weight, labels, lse, bias=None):
     """Gradients of sum(grad_loss * loss) with respect to x, weight and, where one is given, bias.
     grad_loss: fp32 [n], every row's weight in the objective (1/n for the mean); lse: what class_loss gave."""
-    torch = _torch()
     kind, ld_x, ld_w, n, width, classes = _class_call("class_loss_backward", x, weight, labels, bias)
     _vector("grad_loss", grad_loss, torch.float32, n)
     _vector("lse", lse, torch.float32, n)
     device = _device(x, weight, labels, bias, grad_loss, lse)
-    with _on(stream):
-        grad_x, grad_w = torch.empty((n, width), dtype=x.dtype, device=device), torch.empty((classes, width), dtype=x.dtype, device=device)
-        grad_b = torch.empty(classes, dtype=x.dtype, device=device) if bias is not None else None
-        keep, ws, size = _workspace("tbk_class_loss_backward", device, n, width, classes, kind, _readable(x, ld_x, weight, ld_w), device.index)
-        _check(lib().tbk_class_loss_backward(grad_loss.data_ptr(), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias),
-                                             labels.data_ptr(), labels.element_size(), lse.data_ptr(), grad_x.data_ptr(), width,
-                                             grad_w.data_ptr(), width, _ptr(grad_b), n, width, classes, kind, ws, size,
-                                             device.index, _stream_ptr(stream, device.index)))
+    grad_x, grad_w = x.new_empty((n, width)), x.new_empty((classes, width))
+    grad_b = x.new_empty(classes) if bias is not None else None
+    L = lib()
+    size = _size("tbk_class_loss_backward_workspace", n, width, classes, kind, _readable(x, ld_x, weight, ld_w), device)
+    keep, ws = _workspace(x, size)
+    _check(L.tbk_class_loss_backward(grad_loss.data_ptr(), x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(bias), labels.data_ptr(),
+                                     labels.element_size(), lse.data_ptr(), grad_x.data_ptr(), width, grad_w.data_ptr(), width,
+                                     _ptr(grad_b), n, width, classes, kind, ws, size, device, _stream_ptr(None, device)))
     return (grad_x, grad_w, grad_b) if bias is not None else (grad_x, grad_w)
 
 
@@ -349,7 +366,7 @@ class LeafModel:
     by reference: an optimiser updates them in place."""
 
     def __init__(self, forest, table, layers, weight, bias=None, batch_hint: int = 0, **schedule):
-        device = _device(table, weight, bias, *(t for l in layers for t in l[:2])).index
+        device = _device(table, weight, bias, *(t for l in layers for t in l[:2]))
         self.forest = kernels.DeviceForest(forest, device=device, batch_hint=batch_hint, **(schedule or {"representation": "auto"}))
         self.leaves = LeafMap(forest, device)
         self.table, self.layers, self.weight, self.bias = table, list(layers), weight, bias
@@ -388,7 +405,6 @@ class LeafModel:
     def loss_and_grads(self, rows, labels, row_weights=None):
         """(loss [n], gradients of sum(row_weights * loss)); row_weights: fp32 [n], 1/n each if None.
         Gradients: {"table", "layers": [(weight, bias or None)], "weight", "bias" or None}."""
-        torch = _torch()
         kept = []
         h = self.features(rows, kept)
         loss, lse = class_loss(h, self.weight, labels, self.bias)
