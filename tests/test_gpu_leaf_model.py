@@ -463,3 +463,130 @@ def test_a_model_from_rows_to_gradients(dtype):
         assert (got[k].double() - q[k].grad).norm() <= 8 * half * q[k].grad.norm(), k
     scores = model.scores(rows[:1])
     assert scores.shape == (1, 700) and (scores.double() - z[:1].detach()).norm() <= 8 * half * z[:1].norm()
+
+
+def complete_forest(trees, levels):
+    """Complete trees as flat arrays, leaves last; the row of leaf i of tree t is t << levels | i."""
+    from types import SimpleNamespace
+    inner, nodes = (1 << levels) - 1, (2 << levels) - 1
+    at = np.arange(nodes)
+    return SimpleNamespace(num_trees=trees, tree_off=np.arange(trees + 1, dtype=np.int64) * nodes,
+                           left=np.tile(np.where(at < inner, 2 * at + 1, -1).astype(np.int32), trees),
+                           right=np.tile(np.where(at < inner, 2 * at + 2, -1).astype(np.int32), trees),
+                           feat=np.zeros(trees * nodes, np.int32), thr=np.zeros(trees * nodes, np.float32),
+                           class_id=np.zeros(trees, np.int32), num_classes=0, transform=0, initial_value=0.0, num_features=1)
+
+
+@pytest.mark.parametrize("dtype,trees,levels,n,width", [
+    (torch.bfloat16, 37, 6, 10001, 64), (torch.float16, 100, 8, 19999, 64), (torch.bfloat16, 20, 7, 12345, 120),
+    (torch.float32, 21, 5, 11111, 100), (torch.float16, 5, 4, 160001, 256), (torch.bfloat16, 9, 9, 20000, 64)])
+def test_leaf_sum_of_many_rows(dtype, trees, levels, n, width):
+    """Tables in shared memory (and, in the last case, too large for it), ragged tiles and batches of trees, struck-out
+    ids, ids at odd addresses, tables that do not lie row behind row."""
+    forest = complete_forest(trees, levels)
+    leaves = lm.LeafMap(forest)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(trees)
+    leaf = (torch.rand(n, trees, generator=g, device="cuda") ** 2 * (1 << levels)).int()
+    ids = leaf + (1 << levels) - 1
+    gone = torch.rand(n, trees, generator=g, device="cuda") < 0.05
+    ids[gone] = torch.randint(-3, (1 << levels) - 1, (int(gone.sum()),), generator=g, device="cuda", dtype=torch.int32)
+    table = normal(leaves.num_rows, width, dtype=dtype)
+    want, mass = torch.zeros(n, width, dtype=torch.float64, device="cuda"), torch.zeros(n, width, dtype=torch.float64, device="cuda")
+    for t in range(trees):
+        rows = table.double()[(t << levels) + leaf[:, t].long()] * ~gone[:, t, None]
+        want += rows
+        mass += rows.abs()
+    near(lm.leaf_sum(leaves, ids, table), want, trees * STEP * mass)
+    odd = torch.full((n, trees + 3), -1, dtype=torch.int32, device="cuda")
+    odd[:, 1:trees + 1] = ids
+    assert torch.equal(lm.leaf_sum(leaves, odd[:, 1:trees + 1], table), lm.leaf_sum(leaves, ids, table))
+    near(lm.leaf_sum(leaves, ids, strided(table, 8)), want, trees * STEP * mass)
+    near(lm.leaf_sum(leaves, ids, strided(table, 1)), want, trees * STEP * mass)
+
+
+def test_leaf_gradient_of_trees_beyond_two_byte_leaf_numbers():
+    forest = complete_forest(2, 17)
+    leaves = lm.LeafMap(forest)
+    leaf = torch.randint(0, 1 << 17, (5000, 2), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    leaf[::3] = (1 << 17) - 1
+    grad = normal(5000, 8)
+    rows = leaf + torch.tensor([0, 1 << 17], device="cuda")
+    want = torch.zeros(leaves.num_rows, 8, dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(want)
+    for t in range(2):
+        want.index_add_(0, rows[:, t], grad.double())
+        mass.index_add_(0, rows[:, t], grad.double().abs())
+    near(lm.leaf_sum_backward(leaves, (leaf + (1 << 17) - 1).int(), grad), want, 5000 * STEP * mass)
+
+
+@pytest.mark.parametrize("n", [3, 700])
+def test_leaf_sum_past_four_gigabytes_of_table(n):
+    trees, levels, width = 70, 16, 512
+    leaves = lm.LeafMap(complete_forest(trees, levels))
+    table = torch.empty(leaves.num_rows, width, dtype=torch.float16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    assert table.numel() > 1 << 31
+    leaf = torch.randint(0, 1 << levels, (n, trees), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    rows = leaf + (torch.arange(trees, device="cuda") << levels)
+    picked = table[rows.reshape(-1)].view(n, trees, width).double()
+    near(lm.leaf_sum(leaves, (leaf + (1 << levels) - 1).int(), table), picked.sum(1), trees * STEP * picked.abs().sum(1))
+
+
+@pytest.mark.parametrize("outputs", [4100, 4104])
+def test_linear_past_two_gigaelements(outputs):
+    n, inputs = 530000, 24
+    assert n * outputs > 1 << 31
+    x, w = normal(n, inputs, dtype=torch.bfloat16), normal(outputs, inputs, dtype=torch.bfloat16, seed=1)
+    got = lm.linear(x, w)
+    for a in (0, 523000, n - 300):
+        z, mass = x[a:a + 300].double() @ w.double().t(), x[a:a + 300].double().abs() @ w.double().abs().t()
+        near(got[a:a + 300], z, (inputs + 2) * STEP * mass)
+
+
+@pytest.mark.parametrize("n", [7, 8, 9, 16])
+def test_linear_around_few_rows(n):
+    for inputs, outputs in ((100, 70), (1032, 515), (8, 9)):
+        x, w, b, r = (normal(*s, dtype=torch.float16, seed=i) for i, s in enumerate(((n, inputs), (outputs, inputs), (outputs,), (n, outputs))))
+        z, mass = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t()
+        off = (inputs + 2) * STEP * (mass + z.abs())
+        got, pre = lm.linear(x, w, b, "silu", r, keep_pre=True)
+        near(pre, z, off)
+        want = ACT["silu"][0](z) + r.double()
+        near(got, want, SLOPE * off + EVAL * (z.abs() + want.abs()))
+
+
+def test_calls_of_two_streams_at_once():
+    forest, _ = grown(60, 6)
+    leaves = lm.LeafMap(forest)
+    ids = draw_ids(forest, 12000)
+    table = normal(leaves.num_rows, 64, dtype=torch.bfloat16)
+    x, w = normal(3000, 200, dtype=torch.bfloat16), normal(5000, 200, dtype=torch.bfloat16)
+    labels, weights = torch.arange(3000, device="cuda"), torch.full((3000,), 1 / 3000, device="cuda")
+
+    def work():
+        loss, lse = lm.class_loss(x, w, labels)
+        return [lm.leaf_sum(leaves, ids, table), lm.leaf_sum_backward(leaves, ids, lm.leaf_sum(leaves, ids, table)), loss,
+                *lm.class_loss_backward(weights, x, w, labels, lse), *lm.linear_backward(x, x, w[:200], None, "identity")]
+    want = work()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(work())
+    torch.cuda.synchronize()
+    for outs in got[0] + got[1]:
+        assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
+def test_extreme_values_of_activations():
+    """Far tails, zeros of both signs and infinities, as the formulas have them."""
+    z = torch.tensor([-60000.0, -100.0, -20.0, -6.0, -5e-8, -0.0, 0.0, 5e-8, 6.0, 20.0, 100.0, 60000.0, float("inf")], device="cuda").half()
+    x, one = z[:, None].contiguous(), torch.ones(1, 1, dtype=torch.float16, device="cuda")
+    wide = torch.ones(40, 1, dtype=torch.float16, device="cuda")
+    for name in ("relu", "gelu", "silu"):
+        want = ACT[name][0](z.double())
+        for got in (lm.linear(x, one, activation=name)[:, 0], lm.linear(x[:5], one, activation=name)[:, 0], lm.linear(x, wide, activation=name)[:, 33]):
+            near(got, want[:len(got)], EVAL * z[:len(got)].double().abs().clamp(max=1e5))
+        dz = lm.linear_backward(torch.ones_like(x[:-1]), x[:-1], one, x[:-1], name)[0][:, 0]
+        near(dz, ACT[name][1](z[:-1].double()), EVAL * (z[:-1].double().abs().clamp(max=100) + 1) + 2.0 ** -11)

@@ -448,32 +448,35 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
-// Phi(z), the integral of the normal distribution, and exp(-z^2 / 2), of two z.  erfc's shape after Hastings
+// -Phi(-|z|), Phi the integral of the normal distribution, and exp(-z^2 / 2), of two z.  erfc's shape after Hastings
 // (Approximations for Digital Computers, 1955): Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.33 |z|);
 // P was fitted here, by reweighted least squares, for the relative error: below 1e-6 for all z.  Without
 // branches, since a warp's values need both sides of any (the library's erff took most of a layer's time).
-__device__ __forceinline__ float2 normal_integral(float2 z, float2 *bell) {
-  const float2 d = fma2(Two(fabsf(z.x), fabsf(z.y)), Two(0.33f), Two(1.f)).get();
-  const Two t(inverse_fast(d.x), inverse_fast(d.y)), zz(z.x, z.y);
-  Two p = fma2(Two(0.0332859295f), t, Two(-0.105665717f));
-  p = fma2(p, t, Two(0.067432403f));
-  p = fma2(p, t, Two(0.0334278586f));
-  p = fma2(p, t, Two(0.0910052722f));
-  p = fma2(p, t, Two(0.117216671f));
-  p = fma2(p, t, Two(0.13164699f));
-  p = fma2(p, t, Two(0.131651081f));
+__device__ __forceinline__ Two normal_tail(float2 z, float2 size, float2 *bell) { // size: |z|, finite
+  const Two zz(z), a(size);
+  const float2 d = fma2(a, Two(0.33f), Two(1.f)).get();
+  const Two t(inverse_fast(d.x), inverse_fast(d.y));
+  Two p = fma2(Two(-0.0332859295f), t, Two(0.105665717f));
+  p = fma2(p, t, Two(-0.067432403f));
+  p = fma2(p, t, Two(-0.0334278586f));
+  p = fma2(p, t, Two(-0.0910052722f));
+  p = fma2(p, t, Two(-0.117216671f));
+  p = fma2(p, t, Two(-0.13164699f));
+  p = fma2(p, t, Two(-0.131651081f));
   const float2 e = (zz * (zz * Two(-0.5f * kLog2e))).get();
   *bell = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-  const float2 tail = (Two(bell->x, bell->y) * t * p).get();
-  return make_float2(z.x >= 0.f ? 1.f - tail.x : tail.x, z.y >= 0.f ? 1.f - tail.y : tail.y);
+  return Two(*bell) * (t * p);
+}
+__device__ __forceinline__ float2 size_of(float2 z) { // (an infinite z has tail 0)
+  return make_float2(fminf(fabsf(z.x), 1e18f), fminf(fabsf(z.y), 1e18f));
 }
 enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 template <int ACT> __device__ __forceinline__ float2 act_value(float2 z) {
   if constexpr (ACT == kActRelu) return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y); // (NaN stays)
-  if constexpr (ACT == kActGelu) {
+  if constexpr (ACT == kActGelu) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
     float2 bell;
-    const float2 w = normal_integral(z, &bell);
-    return make_float2(z.x * w.x, z.y * w.y);
+    const float2 a = size_of(z);
+    return fma2(Two(a), normal_tail(z, a, &bell), Two(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f))).get();
   }
   if constexpr (ACT == kActSilu)
     return make_float2(z.x * inverse_fast(1.f + exp2_fast(-kLog2e * z.x)), z.y * inverse_fast(1.f + exp2_fast(-kLog2e * z.y)));
@@ -481,10 +484,10 @@ template <int ACT> __device__ __forceinline__ float2 act_value(float2 z) {
 }
 template <int ACT> __device__ __forceinline__ float2 act_slope(float2 z) {
   if constexpr (ACT == kActRelu) return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
-  if constexpr (ACT == kActGelu) {
+  if constexpr (ACT == kActGelu) { // Phi(z) + z phi(z)
     float2 bell;
-    const float2 w = normal_integral(z, &bell);
-    return make_float2(fmaf(z.x * 0.39894228f, bell.x, w.x), fmaf(z.y * 0.39894228f, bell.y, w.y));
+    const float2 tail = normal_tail(z, size_of(z), &bell).get();
+    return make_float2(fmaf(z.x * 0.39894228f, bell.x, z.x >= 0.f ? 1.f + tail.x : -tail.x), fmaf(z.y * 0.39894228f, bell.y, z.y >= 0.f ? 1.f + tail.y : -tail.y));
   }
   if constexpr (ACT == kActSilu) {
     const float s = inverse_fast(1.f + exp2_fast(-kLog2e * z.x)), t = inverse_fast(1.f + exp2_fast(-kLog2e * z.y));
@@ -908,6 +911,12 @@ __device__ __forceinline__ void stage_bias(const T *bias, int n, int N, float *d
   __syncwarp();
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { // (not a number: the others)
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Sum of a row's exponentials over the tiles of a unit, relative to the largest score of them, in one pass:
 // the sum so far is scaled down whenever a larger score comes.  parts[4 * chunk + part][row]
 template <class T, int COLS> struct LseEnd {
@@ -942,7 +951,7 @@ template <class T, int COLS> struct LseEnd {
     }
     const ulonglong2 *b2 = reinterpret_cast<const ulonglong2 *>(w.bias) + n % COLS / 4;
     Two z[16];
-    float top = s.top;
+    float tops[2] = {s.top, s.top};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const ulonglong2 b = b2[j];
@@ -951,10 +960,10 @@ template <class T, int COLS> struct LseEnd {
       z[2 * j] = fma2(Two(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])), Two(kLog2e), lo);
       z[2 * j + 1] = fma2(Two(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])), Two(kLog2e), hi);
       const float2 x = z[2 * j].get(), y = z[2 * j + 1].get();
-      top = fmaxf(top, fmaxf(x.x, x.y));
-      top = fmaxf(top, fmaxf(y.x, y.y));
+      tops[j & 1] = max3(tops[j & 1], x.x, x.y);
+      tops[j & 1] = max3(tops[j & 1], y.x, y.y);
     }
-    const float ref = top == -INFINITY ? 0.f : top; // (all so far forbidden: exponentials are 0)
+    const float top = fmaxf(tops[0], tops[1]), ref = top == -INFINITY ? 0.f : top; // (all so far forbidden: exponentials are 0)
     const Two less(-ref);
     Two sum[2] = {Two(0.f), Two(0.f)};
 #pragma unroll
