@@ -94,12 +94,16 @@ struct LeafSumPlan {
   }
 };
 
+// Up to so many ids the gradient looks them up itself: 100 trees of 1024 rows took 16 us with the numbers of a kernel
+// of their own.
+constexpr int64_t kFewIds = 1 << 19;
+
 struct LeafGradParts {
   int64_t ld;
   unsigned char *numbers; // two bytes each, or four where a tree has very many leaves
   float *sums;
   LeafGradParts(Parts &w, int64_t n, int64_t width, int64_t trees, int64_t rows, bool narrow)
-      : ld(up8(n)), numbers(w.take<unsigned char>((uint64_t)trees * ld * (narrow ? 2 : 4))), sums(w.take<float>(n > tb::kLeafChunk ? rows * width : 0)) {}
+      : ld(up8(n)), numbers(w.take<unsigned char>(n * trees <= kFewIds ? 0 : (uint64_t)trees * ld * (narrow ? 2 : 4))), sums(w.take<float>(n > tb::kLeafChunk ? rows * width : 0)) {}
 };
 
 } // namespace
@@ -279,7 +283,9 @@ int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n
   const bool narrow = map->max_rows < 0xffff;
   LeafGradParts parts(w, n, width, trees, map->rows, narrow);
   const dim3 blocks((unsigned)std::min<int64_t>(tiles_of(n, tb::kNumberRows), 4096), (unsigned)tiles_of(trees, 32));
-  if (narrow) TRY(launch(tb::tb_leaf_numbers_kernel<uint16_t>, blocks, 256, 0, stream, 1, map->view, ids, ld_ids, (uint16_t *)parts.numbers, parts.ld, n));
+  const bool few = n * trees <= kFewIds;
+  if (few) ;
+  else if (narrow) TRY(launch(tb::tb_leaf_numbers_kernel<uint16_t>, blocks, 256, 0, stream, 1, map->view, ids, ld_ids, (uint16_t *)parts.numbers, parts.ld, n));
   else TRY(launch(tb::tb_leaf_numbers_kernel<uint32_t>, blocks, 256, 0, stream, 1, map->view, ids, ld_ids, (uint32_t *)parts.numbers, parts.ld, n));
   return with_piece(type, piece_bytes(type, width, grad, ld_grad, n, out, ld_out, map->rows), [&](auto t, auto v) {
     using T = decltype(t);
@@ -292,10 +298,10 @@ int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n
       using N = decltype(number);
       const auto kernel = tb::tb_leaf_grad_kernel<T, V, N>;
       CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tb::leaf_grad_smem(tb::kLeafChunk, tb::kLeafRange)));
-      return launch(kernel, grid, 32 * tb::kLeafGradWarps, smem, stream, 1, map->view, (const N *)parts.numbers, parts.ld, (const T *)grad, (uint32_t)(ld_grad * sizeof(T)), width,
+      return launch(kernel, grid, 32 * tb::kLeafGradWarps, smem, stream, 1, map->view, few ? (const N *)ids : (const N *)parts.numbers, few ? ld_ids : parts.ld, (const T *)grad, (uint32_t)(ld_grad * sizeof(T)), width,
                     lanes_log2, parts.sums, (T *)out, ld_out, n, chunk, range);
     };
-    return narrow ? sorted(uint16_t()) : sorted(uint32_t());
+    return few ? sorted(int32_t()) : narrow ? sorted(uint16_t()) : sorted(uint32_t());
   });
 }
 

@@ -554,7 +554,10 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 2) tb_leaf_grad_kernel(Le
                                                                               long long ld_out, long long n_rows, int chunk, int range) {
   using S = Share<T, V>;
   constexpr int P = S::kPairs;
-  constexpr uint32_t kNone = (N)~(N)0;
+  // N: two- or four-byte leaf numbers of tb_leaf_numbers_kernel, or (int32_t) the ids themselves, looked up here
+  // twice: of few rows and trees that is less than another launch
+  constexpr bool kIds = std::is_same<N, int32_t>::value;
+  constexpr uint32_t kNone = kIds ? 0xffffffffu : (uint32_t)(N)~(N)0;
   extern __shared__ __align__(16) unsigned char raw[];
   after_previous_kernel();
   uint32_t *start = reinterpret_cast<uint32_t *>(raw);                  // [leaves + 1] first place of a leaf
@@ -568,7 +571,17 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 2) tb_leaf_grad_kernel(Le
   const int leaves = min(range, m.rows[t + 1] - row0);
   if (leaves <= 0) return;
   const uint32_t first_leaf = blockIdx.z * (uint32_t)range;
-  const N *mine = numbers + t * ld_numbers;
+  const N *mine = kIds ? numbers + t : numbers + t * ld_numbers;
+  const int2 tree = kIds ? __ldg(m.trees + t) : make_int2(0, 0);
+  const int32_t tree_row = kIds ? __ldg(m.rows + t) : 0;
+  auto number = [&](long long i) -> uint32_t {
+    if constexpr (kIds) {
+      const int32_t r = leaf_row(m.words, tree, __ldg(mine + i * ld_numbers));
+      return r < 0 ? kNone : (uint32_t)(r - tree_row);
+    } else {
+      return __ldg(mine + i);
+    }
+  };
 
   for (long long b0 = 0; b0 < n_rows; b0 += chunk) {
     const int now = (int)min((long long)chunk, n_rows - b0);
@@ -582,7 +595,7 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 2) tb_leaf_grad_kernel(Le
     for (int i0 = from + wl; i0 < to; i0 += 32 * kAhead) {
       uint32_t l[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) l[k] = i0 + 32 * k < to ? (uint32_t)__ldg(mine + b0 + i0 + 32 * k) : kNone;
+      for (int k = 0; k < kAhead; ++k) l[k] = i0 + 32 * k < to ? number(b0 + i0 + 32 * k) : kNone;
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
         if (l[k] != kNone && l[k] - first_leaf < (uint32_t)leaves) atomicAdd(own + (l[k] - first_leaf), 1u);
@@ -623,7 +636,7 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 2) tb_leaf_grad_kernel(Le
     for (int i0 = from; i0 < to; i0 += 32 * kAhead) {
       uint32_t ls[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) ls[k] = i0 + 32 * k + wl < to ? (uint32_t)__ldg(mine + b0 + i0 + 32 * k + wl) : kNone;
+      for (int k = 0; k < kAhead; ++k) ls[k] = i0 + 32 * k + wl < to ? number(b0 + i0 + 32 * k + wl) : kNone;
       // (the equal ones of 32 rows get their places from one of them, whose counter tells how many came before;
       // a warp's additions to a counter happen in the order of the program, so all eight can be under way)
       uint32_t same[kAhead], at[kAhead];
