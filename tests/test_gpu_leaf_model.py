@@ -27,8 +27,12 @@ def rounding(want, dtype):
 
 
 def near(got, want, extra):
-    """|got - want| <= rounding of got's type + extra; equal where want is not finite."""
+    """|got - want| <= rounding of got's type + extra; equal where want is not finite.  A value of half a step or more
+    above the type's largest number rounds to infinity (65504 + 16 in fp16, whose step there is 32)."""
     assert got.shape == want.shape
+    kind = torch.finfo(got.dtype)
+    beyond = want.abs() + extra >= kind.max * (1 + kind.eps / 4)
+    want = torch.where(beyond & torch.isinf(got) & (got.sign() == want.sign()), got.double(), want)
     odd = ~torch.isfinite(want)
     assert torch.equal(got[odd].double().nan_to_num(7e300), want[odd].nan_to_num(7e300))
     err = torch.where(odd, 0.0, (got.double() - want).abs())
@@ -590,3 +594,60 @@ def test_extreme_values_of_activations():
             near(got, want[:len(got)], EVAL * z[:len(got)].double().abs().clamp(max=1e5))
         dz = lm.linear_backward(torch.ones_like(x[:-1]), x[:-1], one, x[:-1], name)[0][:, 0]
         near(dz, ACT[name][1](z[:-1].double()), EVAL * (z[:-1].double().abs().clamp(max=100) + 1) + 2.0 ** -11)
+
+
+def test_a_graph_that_forks_and_joins():
+    """Calls behind waits for another stream's events, inside one captured graph."""
+    forest, _ = grown(20, 5)
+    leaves = lm.LeafMap(forest)
+    ids = draw_ids(forest, 500)
+    table, w = normal(leaves.num_rows, 64, dtype=torch.bfloat16), normal(300, 64, dtype=torch.bfloat16)
+    labels = torch.arange(500, device="cuda") % 300
+
+    def forked(side):
+        h = lm.leaf_sum(leaves, ids, table)
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            y = lm.linear(h, w, activation="gelu")
+        loss, lse = lm.class_loss(h, w, labels)
+        here.wait_stream(side)
+        dx, dw = lm.linear_backward(y, h, w, y, "silu", bias=False)
+        return [h, y, loss, lse, dx, dw, lm.leaf_sum_backward(leaves, ids, dx)]
+    side = torch.cuda.Stream()
+    want = forked(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = forked(side)
+    for _ in range(3):
+        for o in got:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_small_and_large_weights_of_rows():
+    """Row weights far outside fp16's range, rows of weight zero among them, and one that is not finite."""
+    for dtype in HALVES:
+        for size in (1e-30, 1e-9, 1.0, 1e6):
+            x, w, b, labels = class_case(300, 48, 500, dtype)
+            z, lse, _, live, at = plain_loss(x, w, b, labels)
+            weights = torch.rand(300, device="cuda") * size
+            weights[::7] = 0
+            p = torch.exp(z - lse.float().double()[:, None])
+            p.scatter_add_(1, at[:, None], torch.full((300, 1), -1.0, dtype=torch.float64, device="cuda"))
+            dz = p * torch.where(live, weights.double(), 0.0)[:, None]
+            outs = lm.class_loss_backward(weights, x, w, labels, lse.float(), b)
+            rel, tiny = 1.01 * torch.finfo(dtype).eps / 2 + 1e-4, weights.max().double() * 2.0 ** -37
+            # results below the type's own range round to its grid: half a step of its smallest subnormal number
+            grid = 2.0 ** -25 if dtype is torch.float16 else 2.0 ** -134
+            mass = dz.abs() * rel + tiny
+            near(outs[1], dz.t() @ x.double(), mass.t() @ x.double().abs() + 300 * STEP * (dz.abs().t() @ x.double().abs()) + grid)
+            near(outs[2], dz.sum(0), 1e-4 * dz.abs().sum(0) + 300 * STEP * dz.abs().sum(0) + grid)
+    # (the last weights are beyond fp16's range themselves: the other rows stay what they were, infinities among them)
+    before, rest = outs[0], [i for i in range(300) if i != 5]
+    weights[5], labels[5] = float("inf"), 3
+    outs = lm.class_loss_backward(weights, x, w, labels, lse.float(), b)
+    assert torch.equal(outs[0][rest], before[rest]) and not torch.isfinite(outs[0][5]).any()
