@@ -576,6 +576,10 @@ __device__ __forceinline__ void out_send(const CUtensorMap *map, const unsigned 
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
                ::"l"(map), "r"(n), "r"(m), "r"(dense_smem(buf)) : "memory");
 }
+__device__ __forceinline__ void out_send3(const CUtensorMap *map, const unsigned char *buf, int split, int m, int n) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+               ::"l"(map), "r"(n), "r"(m), "r"(split), "r"(dense_smem(buf)) : "memory");
+}
 __device__ __forceinline__ void out_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // 32 rows x 32 fp32 values turned around in shared memory, 16-byte pieces swapped around by the row's number,
@@ -630,6 +634,7 @@ template <class T> __device__ __noinline__ void copy_in(const T *from, long long
 // piece of a longer sum, added to the pieces before it.  With `parts` the sum is cut into parts, which are kept:
 // parts[split][row][ld_parts].
 template <class T> struct Result {
+  CUtensorMap parts_map; // of `parts`
   CUtensorMap out_map, pre_map, addend_map; // where the matrix's rows lie at multiples of 16 bytes (tma_*)
   const T *bias, *addend;
   T *out, *pre;
@@ -685,14 +690,10 @@ template <class T> struct Result {
   }
 };
 
-// A warp's 32 x 32 sums, turned around in its shared memory, to where parts or pieces of sums are kept.
-template <class T> __device__ __noinline__ void keep_sums(const Result<T> &f, const unsigned char *mine, int m0, int n, int M, int N, int split) {
+// A warp's 32 x 32 sums, turned around in its shared memory, to where pieces of sums are kept.
+template <class T> __device__ __noinline__ void keep_sums(const Result<T> &f, const unsigned char *mine, int m0, int n, int M, int N) {
   turned(mine, [&](int k, int c, const float (&x)[8]) {
-    if (m0 + k >= M || n + c >= N) return;
-    if (!f.parts) return f.finish8(x, m0 + k, n + c, N);
-    float4 *d = reinterpret_cast<float4 *>(f.parts + ((long long)split * M + m0 + k) * f.ld_parts + n + c);
-    d[0] = make_float4(x[0], x[1], x[2], x[3]);
-    d[1] = make_float4(x[4], x[5], x[6], x[7]);
+    if (m0 + k < M && n + c < N) f.finish8(x, m0 + k, n + c, N);
   });
 }
 
@@ -732,9 +733,19 @@ template <class T> struct ResultEnd {
                                         DenseWarp &w, bool second, bool more) const {
     const int lane = threadIdx.x % 32;
     const int m0 = row - lane;
-    if (f.parts || f.sums) {
+    if (f.parts) { // (4 KB a time, turned around as their map says)
+      out_free<0>();
       turn(r, w.mine);
-      return keep_sums(f, w.mine, m0, n, p.M, p.N, u.split);
+      out_ready();
+      if (lane == 0) {
+        if (m0 < p.M) out_send3(&f.parts_map, w.mine, u.split, m0, n);
+        out_commit();
+      }
+      return;
+    }
+    if (f.sums) {
+      turn(r, w.mine);
+      return keep_sums(f, w.mine, m0, n, p.M, p.N);
     }
     Two z[16];
 #pragma unroll

@@ -133,6 +133,17 @@ template <class T> int side_map(CUtensorMap *map, const Side &s, int64_t rows, i
 // Where a warp's 32 rows and columns of a result go.
 template <class T> int out_map(CUtensorMap *map, const void *p, int64_t rows, int64_t cols, int64_t ld) { return encode_map<T>(map, p, cols, rows, ld, 32, 32); }
 
+// Parts of sums, fp32: [splits][rows][ld], 32 x 32 at a time.
+int parts_map(CUtensorMap *map, const void *p, int splits, int64_t rows, int64_t cols, int64_t ld) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return fail(TBK_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)splits}, strides[2] = {(cuuint64_t)ld * 4, (cuuint64_t)(ld * rows) * 4};
+  const cuuint32_t box[3] = {32, 32, 1}, one[3] = {1, 1, 1};
+  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? TBK_OK : fail(TBK_ERR_CUDA, "cuTensorMapEncodeTiled: %d (%d x %lld x %lld)", (int)rc, splits, (long long)rows, (long long)cols);
+}
+
 template <class T> int set_problem(tb::DenseProblem *p, int shape, const Side &a, const Side &b, const Size &size, int splits, int run) {
   TRY(side_map<T>(&p->a, a, size.m, size.k));
   TRY(side_map<T>(&p->b, b, size.n, size.k));
@@ -207,6 +218,7 @@ int products(const Product<T> *list, int count, const ColumnSums<T> &sums, float
       jobs.end[i].f = x.end;
       if (cut.splits[i] == 1) continue;
       jobs.end[i].f.parts = parts, jobs.end[i].f.ld_parts = up8(x.size.n);
+      TRY(parts_map(&jobs.end[i].f.parts_map, parts, cut.splits[i], x.size.m, up8(x.size.n), up8(x.size.n)));
       finish.end[i] = jobs.end[i].f;
       finish.splits[i] = cut.splits[i], finish.M[i] = x.size.m, finish.N[i] = x.size.n;
       finish.blocks[i] = (unsigned)tiles_of(x.size.m * (up8(x.size.n) / 8), 256);
