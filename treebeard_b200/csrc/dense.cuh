@@ -756,10 +756,10 @@ template <class T> struct ResultEnd {
       for (int i = 0; i < 16; ++i) z[i] = z[i] * d;
     }
     auto add8 = [&](int i, uint4 q) {
-      z[4 * i] = z[4 * i] + Two(unpack2<T>(q.x));
-      z[4 * i + 1] = z[4 * i + 1] + Two(unpack2<T>(q.y));
-      z[4 * i + 2] = z[4 * i + 2] + Two(unpack2<T>(q.z));
-      z[4 * i + 3] = z[4 * i + 3] + Two(unpack2<T>(q.w));
+      add_halves<T>(z[4 * i].v, q.x);
+      add_halves<T>(z[4 * i + 1].v, q.y);
+      add_halves<T>(z[4 * i + 2].v, q.z);
+      add_halves<T>(z[4 * i + 3].v, q.w);
     };
     if (f.bias) {
       const uint4 *b = reinterpret_cast<const uint4 *>(w.bias) + n % 64 / 8;

@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <cstdint>
+#include <type_traits>
 
 namespace tb {
 
@@ -14,6 +16,16 @@ template <class T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Adds two 16-bit elements to two fp32 sums: widened (exactly) and added by one instruction each.
+template <class T> __device__ __forceinline__ void add_halves(unsigned long long &sums, uint32_t halves) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("{\n .reg .b16 c, d;\n .reg .f32 a, b;\n mov.b64 {a, b}, %0;\n mov.b32 {c, d}, %1;\n add.rn.f32.f16 a, c, a;\n add.rn.f32.f16 b, d, b;\n"
+        " mov.b64 %0, {a, b};\n}" : "+l"(sums) : "r"(halves));
+  else
+    asm("{\n .reg .b16 c, d;\n .reg .f32 a, b;\n mov.b64 {a, b}, %0;\n mov.b32 {c, d}, %1;\n add.rn.f32.bf16 a, c, a;\n add.rn.f32.bf16 b, d, b;\n"
+        " mov.b64 %0, {a, b};\n}" : "+l"(sums) : "r"(halves));
+}
 
 // Kernels of one call follow one another closely: each is launched while the one before still runs, prepares itself
 // and waits here until that one's results are there (and lets its own follower come).

@@ -61,10 +61,6 @@ template <class T, int V> struct Share {
     }
     return q;
   }
-  static __device__ __forceinline__ float2 pair(uint32_t w) { // (of a 16-bit type)
-    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  }
   static __device__ __forceinline__ void add(unsigned long long &acc, float2 v) {
     asm("{\n .reg .b64 t;\n mov.b64 t, {%1, %2};\n add.rn.f32x2 %0, %0, t;\n}" : "+l"(acc) : "f"(v.x), "f"(v.y));
   }
@@ -73,10 +69,10 @@ template <class T, int V> struct Share {
       add(acc[0], make_float2(__uint_as_float(q.x), __uint_as_float(q.y)));
       add(acc[1], make_float2(__uint_as_float(q.z), __uint_as_float(q.w)));
     } else {
-      add(acc[0], pair(q.x));
-      add(acc[1], pair(q.y));
-      add(acc[2], pair(q.z));
-      add(acc[3], pair(q.w));
+      add_halves<T>(acc[0], q.x);
+      add_halves<T>(acc[1], q.y);
+      add_halves<T>(acc[2], q.z);
+      add_halves<T>(acc[3], q.w);
     }
   }
   static __device__ __forceinline__ float2 get(unsigned long long a) {
