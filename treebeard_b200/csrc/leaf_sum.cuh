@@ -424,26 +424,38 @@ __global__ void __launch_bounds__(kLeafStagedThreads, 1)
       unsigned long long acc[kLeafRows][P] = {};
       for (int b = b0; ok && b < b1; ++b) {
         const int now = min(kLeafBatch, trees - b * kLeafBatch);
-        if (!(ok = __all_sync(~0u, leaf_wait(found + 8 * slot, slot_phase)))) break;
+        if (!(ok = __all_sync(~0u, ok && leaf_wait(found + 8 * slot, slot_phase)))) break;
         const uint16_t *place = places + slot * kLeafBatch * kLeafMostRows + group * kLeafRows;
-        for (int j = 0; j < now; ++j) {
-          const uint4 o = *reinterpret_cast<const uint4 *>(place + j * kLeafMostRows);
-          if (!(ok = __all_sync(~0u, leaf_wait(full + 8 * stage, phase)))) break;
-          const uint32_t at = stage0 + stage * pitch + lane * 16, w[4] = {o.x, o.y, o.z, o.w};
+        // two trees at a time; a wait that gave up is looked at after the batch (what is read is shared memory still)
+        for (int j = 0; j < now; j += 2) {
+          const bool two = j + 1 < now;
+          const int other = stage + 1 == stages ? 0 : stage + 1;
+          const uint32_t other_phase = phase ^ (other == 0);
+          uint4 o[2];
+          o[0] = *reinterpret_cast<const uint4 *>(place + j * kLeafMostRows);
+          if (two) o[1] = *reinterpret_cast<const uint4 *>(place + (j + 1) * kLeafMostRows);
+          if (ok) ok = leaf_wait(full + 8 * stage, phase);
+          if (two && ok) ok = leaf_wait(full + 8 * other, other_phase);
 #pragma unroll
-          for (int h = 0; h < kLeafRows; h += 4) {
-            uint4 q[4];
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !two) break;
+            const uint32_t at = stage0 + (h ? other : stage) * pitch + lane * 16, w[4] = {o[h].x, o[h].y, o[h].z, o[h].w};
+            uint4 q[kLeafRows];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t v = w[(h + i) / 2], from = at + (i % 2 ? v >> 16 : v & 0xffffu) * 16;
+            for (int i = 0; i < kLeafRows; ++i) {
+              const uint32_t from = at + (i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu) * 16;
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w) : "r"(from));
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S::add(acc[h + i], q[i]);
+            for (int i = 0; i < kLeafRows; ++i) S::add(acc[i], q[i]);
           }
           __syncwarp();
-          if (wl == 0) leaf_arrive(empty + 8 * stage);
-          if (++stage == stages) stage = 0, phase ^= 1;
+          if (wl == 0) {
+            leaf_arrive(empty + 8 * stage);
+            if (two) leaf_arrive(empty + 8 * other);
+          }
+          for (int k = 0; k < 1 + two; ++k)
+            if (++stage == stages) stage = 0, phase ^= 1;
         }
         if (wl == 0) leaf_arrive(used + 8 * slot);
         if (++slot == kLeafSlots) slot = 0, slot_phase ^= 1;
