@@ -549,7 +549,7 @@ def test_linear_past_two_gigaelements(outputs):
 
 @pytest.mark.parametrize("n", [7, 8, 9, 16])
 def test_linear_around_few_rows(n):
-    for inputs, outputs in ((100, 70), (1032, 515), (8, 9)):
+    for inputs, outputs in ((100, 70), (1032, 515), (8, 9), (2056, 1000)):
         x, w, b, r = (normal(*s, dtype=torch.float16, seed=i) for i, s in enumerate(((n, inputs), (outputs, inputs), (outputs,), (n, outputs))))
         z, mass = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t()
         off = (inputs + 2) * STEP * (mass + z.abs())

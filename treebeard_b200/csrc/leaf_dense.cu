@@ -297,13 +297,19 @@ int few_rows(const T *x, int64_t ld_x, const T *weight, int64_t ld_w, const T *b
   return n == 1 ? run(std::integral_constant<int, 1>()) : n <= 4 ? run(std::integral_constant<int, 4>()) : run(std::integral_constant<int, 8>());
 }
 
+// Whether a layer goes to tb_linear_rows_kernel.  Its time grows with the rows, the other kernel's hardly: 1, 4, 8 rows
+// of 1024 x 1024 take 2.5, 4.8, 8.5 us (8.6, 8.7, 9.1 there), of 4096 x 4096 8, 17, 31 (13 to 15).
+bool is_few_rows(int64_t n, int64_t inputs, int64_t outputs) {
+  return n == 1 || (n <= tb::kFewRows && (double)(n * n) * inputs * outputs <= 1 << 26);
+}
+
 typedef unsigned short Half; // an element of either 16-bit type
 
 struct LinearParts {
   Half *x, *weight;
   float *parts;
   LinearParts(Parts &w, int64_t n, int64_t inputs, int64_t outputs, bool aligned, int sms) : x(nullptr), weight(nullptr), parts(nullptr) {
-    if (n <= tb::kFewRows) return; // (read and written as they are)
+    if (is_few_rows(n, inputs, outputs)) return; // (read and written as they are)
     const Size size{n, outputs, inputs};
     x = w.take<Half>(aligned ? 0 : n * up8(inputs)), weight = w.take<Half>(aligned ? 0 : outputs * up8(inputs));
     parts = w.take<float>(std::max(part_floats(&size, 1, sms), part_floats(&size, 1, sms, true)));
@@ -402,7 +408,7 @@ int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64_t ld_w, co
   return with_half(type, [&](auto t) {
     using T = decltype(t);
     const int sms = multiprocessors(device);
-    if (n <= tb::kFewRows) return few_rows<T>((const T *)x, ld_x, (const T *)weight, ld_w, (const T *)bias, act, (const T *)residual, ld_res, (T *)out, ld_out, (T *)pre,
+    if (is_few_rows(n, inputs, outputs)) return few_rows<T>((const T *)x, ld_x, (const T *)weight, ld_w, (const T *)bias, act, (const T *)residual, ld_res, (T *)out, ld_out, (T *)pre,
                                               ld_pre, (int)n, (int)inputs, (int)outputs, sms, stream);
     Parts w{(unsigned char *)ws};
     LinearParts parts(w, n, inputs, outputs, aligned, sms);

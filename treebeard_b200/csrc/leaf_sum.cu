@@ -48,7 +48,8 @@ int lanes_of(int64_t width, int32_t type) {
 
 constexpr int kLeafStagedSmem = 227 * 1024 - tb::kLeafStagedFixed;
 
-// How a leaf sum is cut.  Up to two rows per multiprocessor: a cluster of blocks per row.  Above that: tiles of
+// How a leaf sum is cut.  Up to six rows per multiprocessor: a cluster of blocks per row (1000 trees, width 64: 4.5 us
+// for 64 rows, 13 for 296, 20 for 512, 37 for 1024; tiles take 35 to 38 us for all of them).  Above that: tiles of
 // eight rows per lane group, of as few warps as it takes to have enough tiles, whose trees the blocks share
 // out (a block to a multiprocessor, 16 warps, where tiles are many; at most about 16 parts of a tile).  With
 // very many tiles each has a block of its own and there are no parts.
@@ -65,7 +66,7 @@ struct LeafSumPlan {
     const int lanes = 1 << lanes_log2;
     columns = (unsigned)tiles_of(width, (int64_t)elems << lanes_log2);
     ld_parts = tiles_of(width, elems) * elems;
-    by_row = n <= 2 * sms;
+    by_row = n <= 6 * sms;
     if (by_row) {
       threads = tb::kLeafRowThreads;
       while (cluster < 8 && (int64_t)cluster * 8 * (threads / lanes) < trees) cluster *= 2;
@@ -94,9 +95,9 @@ struct LeafSumPlan {
   }
 };
 
-// Up to so many ids the gradient looks them up itself: 100 trees of 1024 rows took 16 us with the numbers of a kernel
-// of their own.
-constexpr int64_t kFewIds = 1 << 19;
+// Up to so many ids the gradient looks them up itself, above that a kernel of their own does (100 trees of 8 levels,
+// width 64: 15.1 and 17.6 us for 1024 rows, 35.9 and 34.4 for 5243, 90 and 99 for 20000).
+constexpr int64_t kFewIds = 1 << 21;
 
 struct LeafGradParts {
   int64_t ld;
