@@ -16,6 +16,8 @@
 //   kDensePair  two blocks on 256 x 256 results, 128 rows of each operand: 64 + 64, measured at three quarters of
 //               the tall one's rate; two tiles' accumulators, one taken out while the other is computed.
 //   kDenseOne   one block on 128 x 128 results, for products with few tiles: 128 + 128, half the rate.
+// Plain products, bf16: 8192 x 8192 x 8192 at 1.50 to 1.53 PFLOP/s (cuBLAS 1.60), 32768 x 1024 -> 4096 at 1.35 to 1.39
+// (1.40), in 198 to 205 us; with gelu and the value before it as a second result 284.
 //
 // All waits are bounded: one that gives up ends the launch with a word in tb_dense_status.
 #pragma once

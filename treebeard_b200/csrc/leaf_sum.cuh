@@ -269,7 +269,9 @@ __global__ void __launch_bounds__(512, 1) tb_leaf_sum_kernel(LeafMapView m, cons
 // takes a quarter of a warp at least.  One warp copies the tables of the trees to come into a ring of stages, one
 // bulk copy a tree; three look up, eight trees at a time, where in its stage each batch row's table row will lie;
 // twelve add up, a lane group its eight rows: an address and a read of 30 cycles each, instead of the hundreds of an
-// L1 miss.  A table is copied once for a block's tile of rows.  Waits are bounded: one that gives up sets
+// L1 miss.  A table is copied once for a block's tile of rows.  20011 rows, 1000 trees of 256 leaves, 64 bf16: 221 us
+// with the join (the kernel above: 253); 60 % of shared memory's cycles and 2.1 of 4 instructions a cycle are used, so
+// latency bounds it.  Waits are bounded: one that gives up sets
 // tb_leaf_status.
 __device__ int tb_leaf_status;
 constexpr int kLeafAdders = 12, kLeafFinders = 3, kLeafStagedThreads = 32 * (kLeafAdders + kLeafFinders + 1);
@@ -549,7 +551,8 @@ __global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, con
 // equal leaves keep the order of the rows); then the sorted rows are shared out evenly among the lane groups,
 // which add up runs of equal leaves.  A leaf inside one group's stretch is finished there; the ends of
 // stretches are joined in order afterwards.  Batches above kLeafChunk rows come in pieces, with fp32 sums in
-// `sums` in between.
+// `sums` in between.  20011 rows, 1000 trees of 256 leaves, 64 bf16: 304 us and 41 for the numbers; 2.75 of 4
+// instructions a cycle, 8.8 TB/s from L2: instructions bound it.
 constexpr int kLeafRange = 1024, kLeafChunk = 32768, kLeafGradWarps = 16;
 constexpr int kLeafGradFixed = kLeafRange * 4 + 16;
 __host__ __device__ constexpr int leaf_grad_smem(int chunk, int range) { // counters and, after them, the ends of stretches share their place
