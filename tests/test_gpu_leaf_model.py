@@ -651,3 +651,27 @@ def test_small_and_large_weights_of_rows():
     weights[5], labels[5] = float("inf"), 3
     outs = lm.class_loss_backward(weights, x, w, labels, lse.float(), b)
     assert torch.equal(outs[0][rest], before[rest]) and not torch.isfinite(outs[0][5]).any()
+
+
+def test_a_closed_map_is_not_read():
+    forest, _ = grown(3, 3)
+    leaves = lm.LeafMap(forest)
+    ids, rows = draw_ids(forest, 5), leaves.num_rows
+    lm.leaf_sum(leaves, ids, normal(rows, 8))
+    leaves.close()
+    for call in (lambda: lm.leaf_sum(leaves, ids, normal(rows, 8)), lambda: lm.leaf_sum_backward(leaves, ids, normal(5, 8))):
+        with pytest.raises(kernels.TbkError) as e:
+            call()
+        assert e.value.status == 1
+
+
+@pytest.mark.parametrize("n", [0, 1])
+def test_a_model_of_few_or_no_rows(n):
+    forest, marg = grown(4, 3)
+    params = [normal(int((np.asarray(forest.left) < 0).sum()), 16, dtype=torch.bfloat16), normal(16, 16, dtype=torch.bfloat16, seed=1), normal(9, 16, dtype=torch.bfloat16)]
+    model = lm.LeafModel(forest, params[0], [(params[1], None, "silu", True)], params[2])
+    rows = torch.from_numpy(marg.sample_rows(np.random.default_rng(0), 2))[:n].cuda()
+    loss, grads = model.loss_and_grads(rows, torch.zeros(n, dtype=torch.int64, device="cuda"))
+    assert loss.shape == (n,) and model.scores(rows).shape == (n, 9)
+    for got, like in ((grads["table"], params[0]), (grads["layers"][0][0], params[1]), (grads["weight"], params[2])):
+        assert got.shape == like.shape and torch.isfinite(got).all() and bool((got != 0).any()) == (n > 0)

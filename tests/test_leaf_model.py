@@ -169,3 +169,46 @@ def test_overlap_is_seen_by_bytes():
     m = torch.zeros(10, 8)
     with refused(INVALID, "overlaps"):   # columns of one matrix interlace
         lm._apart("out", m[:, :4], m[:, 4:])
+
+
+def test_a_closed_leaf_map_is_refused():
+    leaves = lm.LeafMap.__new__(lm.LeafMap)
+    leaves._h, leaves._size = None, lambda *a: 0   # (as if it held a handle)
+    leaves.close()
+    with refused(INVALID, "closed"):
+        leaves._size("tbk_leaf_sum_workspace", 1, 8, 0)
+
+
+def test_a_stream_of_another_device_is_refused():
+    other = SimpleNamespace(device=torch.device("cuda", 1))
+    tensor = SimpleNamespace(is_cuda=True, get_device=lambda: 0)
+    called = []
+    call = lm._on_stream(lambda *a, **k: called.append(a))
+    with refused(INVALID, "stream"):
+        call(None, _like(tensor), stream=other)
+    with refused(INVALID, "stream"):
+        call(None, bias=_like(tensor), stream=other)
+    assert not called
+
+
+def _like(fake):
+    class Tensor(torch.Tensor):
+        get_device = staticmethod(fake.get_device)
+    return torch.zeros(1).as_subclass(Tensor)
+
+
+def test_more_trees_than_a_launch_reaches_are_refused():
+    forest = synth.generate_forest(0, 5, 4, 8, 0.1, 0.1, synth.Marginal("normal", 8))
+    c, keep = kernels.forest_arrays_c(forest)
+    out = ctypes.c_void_p()
+    c.num_trees = 65535 * 32 + 1   # (refused before an array is read)
+    assert lm.lib().tbk_leaf_map_create(ctypes.byref(c), 0, ctypes.byref(out)) == UNSUPPORTED
+    assert b"2097120 trees" in lm.lib().tbk_last_error()
+
+
+def test_tensors_without_dimensions_are_refused():
+    leaves = SimpleNamespace(_h=1, device=0, num_trees=3, num_rows=12)
+    with refused(INVALID):
+        lm.leaf_sum_backward(leaves, torch.zeros((), dtype=torch.int32), torch.zeros(2, 8))
+    with refused(INVALID):
+        lm.leaf_sum_backward(leaves, torch.zeros(2, 3, dtype=torch.int32), torch.zeros(()))

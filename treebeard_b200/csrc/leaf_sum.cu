@@ -116,7 +116,7 @@ int tbk_leaf_map_create(const tbk_forest_arrays *fa, int32_t device, tbk_leaf_ma
   *out = nullptr;
   if (!fa || !fa->tree_off || !fa->left) return fail(TBK_ERR_INVALID, "null forest array");
   if (fa->num_trees < 1) return fail(TBK_ERR_INVALID, "a leaf map needs a tree at least");
-  if (fa->num_trees > 1 << 21) return fail(TBK_ERR_UNSUPPORTED, "more than %d trees", 1 << 21);
+  if (fa->num_trees > 65535 * 32) return fail(TBK_ERR_UNSUPPORTED, "more than %d trees", 65535 * 32); // (32 to a row of a grid)
   if (fa->tree_off[0] != 0) return fail(TBK_ERR_INVALID, "tree_off does not begin with 0");
   for (int64_t t = 0; t < fa->num_trees; ++t)
     if (fa->tree_off[t + 1] <= fa->tree_off[t] || fa->tree_off[t + 1] - fa->tree_off[t] > kMost) return fail(TBK_ERR_INVALID, "tree %lld has no nodes, or too many", (long long)t);

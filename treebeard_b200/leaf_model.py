@@ -126,6 +126,9 @@ def _on_stream(call):
     def wrapper(*args, stream=None, **kwargs):
         if stream is None:
             return call(*args, **kwargs)
+        for t in (*args, *kwargs.values()):
+            if isinstance(t, torch.Tensor) and t.get_device() != stream.device.index:
+                _refuse(f"the stream is on {stream.device}, a tensor of the call is not")
         with torch.cuda.stream(stream):
             return call(*args, **kwargs)
     return wrapper
@@ -161,6 +164,10 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _closed(*_):
+    _refuse("the leaf map is closed")
+
+
 class LeafMap:
     """Which row of an embedding table each leaf of a forest stands for: the leaves of all trees, numbered
     tree by tree in node order (``num_rows`` of them).  ``forest`` is any object with the flat forest
@@ -183,6 +190,7 @@ class LeafMap:
             except TypeError:      # interpreter shutdown: module globals are already gone
                 pass
         self._h = None
+        self._size = _closed       # (what was there holds the handle)
 
     __del__ = close
 
@@ -224,9 +232,9 @@ def leaf_sum(leaves: LeafMap, ids, table, out=None):
 def leaf_sum_backward(leaves: LeafMap, ids, grad, out=None):
     """Gradient of leaf_sum with respect to the table, [leaves.num_rows, width] of grad's type, from grad
     [n, width], the gradient of its result."""
-    n, width = ids.shape[0], grad.shape[-1]
-    ld_grad = _matrix("grad", grad, grad.dtype, n)
+    ld_grad = _matrix("grad", grad, grad.dtype, ids.shape[0] if ids.dim() else None)
     ld_ids, device, kind = _leaf_call(leaves, ids, grad, "leaf_sum_backward")
+    n, width = grad.shape
     if out is None:
         out, ld_out = grad.new_empty((leaves.num_rows, width)), width
     else:
