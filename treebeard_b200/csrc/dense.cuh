@@ -8,8 +8,9 @@
 // theirs is one chain of short steps, so that eight warps took twice as long as sixteen).  Blocks are
 // persistent and walk over units: a row tile, a run of column tiles, a part of the sum.
 //
-// Three shapes (kernel template SHAPE).  What bounds them is shared memory: 128 bytes a cycle are written by the
-// tensor copies and read by the matrix unit.  With 64 k at a time, bytes written + read per cycle of matrix work:
+// Three shapes (kernel template SHAPE).  Their rates follow what they move through shared memory (128 bytes a cycle),
+// which tensor copies write and the matrix unit reads.  With 64 k at a time, bytes written + read per cycle of matrix
+// work:
 //   kDenseTall  two blocks on 512 x 256 results, 256 rows of A and 128 of B each: 48 + 64.  Both accumulators,
 //               128 x 256 a block, belong to one tile; so that one is taken out while the other is still computed,
 //               the first runs ahead of the second by up to three stages at a tile's beginning and two at its end.
@@ -18,6 +19,9 @@
 //   kDenseOne   one block on 128 x 128 results, for products with few tiles: 128 + 128, half the rate.
 // Plain products, bf16: 8192 x 8192 x 8192 at 1.50 to 1.53 PFLOP/s (cuBLAS 1.60), 32768 x 1024 -> 4096 at 1.35 to 1.39
 // (1.40), in 198 to 205 us; with gelu and the value before it as a second result 284.
+// Those bytes are not all: of 4096 x 512 -> 100003 classes (327 us; the tensor pipe is busy 68 % of the cycles, at 1.65 GHz)
+// a pair that kept A in shared memory for eight tiles, 32 + 64, took 358, one with six stages instead of four as
+// long as this.
 //
 // All waits are bounded: one that gives up ends the launch with a word in tb_dense_status.
 #pragma once
