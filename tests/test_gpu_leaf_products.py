@@ -1,0 +1,73 @@
+"""Launches that carry both products of a backward pass, at sizes where blocks pass from one to the other and the two
+leave their results in different ways (by find_cut on 148 multiprocessors; the comments say how).
+
+Tolerances as in test_gpu_leaf_model.py."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_leaf_model import HALVES, STEP, class_case, near, no_wait_gave_up, normal, plain_loss  # noqa: F401
+from treebeard_b200 import leaf_model as lm
+
+pytestmark = pytest.mark.gpu
+
+
+def class_gradients_are_near(outs, x, w, b, labels, weights, z, lse, live, at):
+    """lse: what the call was given.  Errors of dz: scores off by their sums' steps, arguments of the exponentials by a
+    step of their size, the rounding to 16 bits, and below fp16's normal range half of 2^-24 in units of
+    1 / scale <= 2^-12 of the largest weight of a row with a label."""
+    (n, width), classes = x.shape, w.shape[0]
+    X, W, dtype = x.double(), w.double(), x.dtype
+    p = torch.exp(z - lse.double()[:, None])
+    gl = torch.where(live, weights.double(), 0.0)[:, None]
+    zoff = (width + 4) * STEP * (X.abs() @ W.abs().t() + z.abs())
+    raw = gl.abs() * (p * (zoff + 8 * STEP * (z.abs() + lse.double().abs()[:, None] + 1)) + STEP)
+    del zoff
+    dz = gl * p.scatter_add_(1, at[:, None], torch.full((n, 1), -1.0, dtype=torch.float64, device="cuda"))
+    tiny = gl.abs().max() * 2.0 ** -37 if dtype is torch.float16 else 0.0
+    off = raw + torch.finfo(dtype).eps / 2 * dz.abs() * 1.01 + tiny
+    near(outs[0], dz @ W, off @ W.abs() + (classes + 4) * STEP * (dz.abs() @ W.abs()))
+    near(outs[1], dz.t() @ X, off.t() @ X.abs() + (n + 4) * STEP * (dz.abs().t() @ X.abs()))
+    if b is not None:
+        near(outs[2], dz.sum(0), raw.sum(0) + (n + 4) * STEP * dz.abs().sum(0))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n,width,classes", [
+    (128, 64, 32768),     # 128 x 128: 32 parts of x's gradient, then whole tiles of the weights'
+    (1024, 512, 32000),   # 256 x 256: 8 parts, then whole tiles
+    (200, 600, 20000),    # 256 x 256: 16 parts, then whole tiles, ragged
+    (2048, 2048, 50257),  # 512 x 256: 2 parts, then whole tiles
+])
+def test_class_gradient_of_parts_and_whole_sums(n, width, classes, dtype):
+    x, w, b, labels = class_case(n, width, classes, dtype)
+    z, lse, _, live, at = plain_loss(x, w, b, labels)
+    weights = (torch.rand(n, device="cuda") + 0.5) / n
+    lse = lse.float()
+    outs = lm.class_loss_backward(weights, x, w, labels, lse, b)
+    for _ in range(20):    # (nothing that depends on which copy ends when)
+        assert all(torch.equal(p, q) for p, q in zip(outs, lm.class_loss_backward(weights, x, w, labels, lse, b)))
+    class_gradients_are_near(outs, x, w, b, labels, weights, z, lse, live, at)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("n,inputs,outputs", [
+    (100, 37900, 100),    # 128 x 128: each block has two tiles with skip, then two of the weights'
+    (60, 40000, 120),
+    (801, 3823, 33),      # one tile with skip, then one of the weights'
+    (132, 2414, 1907),    # 256 x 256: five parts, then whole tiles
+    (6189, 598, 33),      # whole tiles with skip, then twenty parts
+    (272, 3577, 1760),    # whole tiles of either
+])
+def test_layer_gradient_with_skip_and_the_weights_in_one_launch(n, inputs, outputs, dtype):
+    x, w = normal(n, inputs, dtype=dtype), normal(outputs, inputs, dtype=dtype, scale=inputs ** -0.5, seed=1)
+    g, skip = normal(n, outputs, dtype=dtype, seed=2), normal(n, inputs, dtype=dtype, seed=4)
+    G, X, W = g.double(), x.double(), w.double()
+    for add in (skip, None):
+        outs = lm.linear_backward(g, x, w, skip=add)
+        for _ in range(20):
+            assert all(torch.equal(p, q) for p, q in zip(outs, lm.linear_backward(g, x, w, skip=add)))
+        want = G @ W + (add.double() if add is not None else 0.0)
+        near(outs[0], want, (outputs + 2) * STEP * (G.abs() @ W.abs() + want.abs()))
+        near(outs[1], G.t() @ X, (n + 2) * STEP * (G.abs().t() @ X.abs()))
+        near(outs[2], G.sum(0), (n + 2) * STEP * G.abs().sum(0))

@@ -1,0 +1,57 @@
+"""Results that leave through a warp's two pieces of shared memory: no piece is written while a copy may read it,
+whatever products follow one another.  The bookkeeping is the kernel's own header, compiled for the host; the
+copies are those of a model that lets each finish as late as the waits allow."""
+import os
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+# every sequence of eight results; p: a part of a sum (both pieces), k: a result and what it was before the activation
+# (both), a, b: the first and second half of a tile with an addend, r: any other result, s: a sum kept without a copy
+MODEL = r"""
+#include "treebeard_b200/csrc/out_pieces.h"
+#include <cstdio>
+#include <cstring>
+int main() {
+  const char kinds[] = "pkabrs";
+  long waits = 0, all = 0;
+  for (long code = 0; code < 1679616; ++code) {   // 6^8
+    tb::OutPieces out{0};
+    unsigned under_way[2] = {0, 0};                   // read by the newest copy and the one before it
+    long c = code;
+    for (int i = 0; i < 8; ++i, c /= 6) {
+      const char k = kinds[c % 6];
+      const unsigned pieces = k == 'p' || k == 'k' || k == 's' ? 3 : k == 'a' ? 1 : k == 'b' ? 2 : out.other();
+      const unsigned may = out.claim(pieces);
+      if (k == 's') out.read = 0;
+      if (may > 1) return 1;
+      under_way[1] = 0;                               // all but the newest `may` copies have ended
+      if (!may) under_way[0] = 0, ++waits;
+      ++all;
+      if (pieces & (under_way[0] | under_way[1])) return printf("written while read: code %ld at %d\n", code, i), 1;
+      if (k != 's') under_way[1] = under_way[0], under_way[0] = pieces;
+      else if (under_way[0]) return printf("kept sums over a copy: code %ld at %d\n", code, i), 1;
+    }
+  }
+  // a product of plain results never waits for the copy before
+  tb::OutPieces out{0};
+  for (int i = 0; i < 100; ++i)
+    if (!out.claim(out.other())) return 2;
+  return 0;
+}
+"""
+
+
+def test_no_piece_is_written_while_it_is_copied_out(tmp_path):
+    (tmp_path / "model.cpp").write_text(MODEL)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", ROOT, "-o", str(tmp_path / "model"), str(tmp_path / "model.cpp")], check=True)
+    done = subprocess.run([str(tmp_path / "model")], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout
+
+
+def test_the_kernels_ask_before_they_write():
+    """Every wait for copies out of a warp's pieces goes through that bookkeeping."""
+    text = open(os.path.join(ROOT, "treebeard_b200", "csrc", "dense.cuh")).read()
+    body = text.split("void out_claim(", 1)
+    assert "out_free<" not in body[0].split("void out_free()")[0]
+    inside, after = body[1].split("\n}\n", 1)
+    assert inside.count("out_free<") == 2 and "out_free<" not in after

@@ -29,6 +29,7 @@
 #include <cstdint>
 #include <type_traits>
 #include "element.cuh"
+#include "out_pieces.h"
 
 namespace tb {
 
@@ -165,7 +166,7 @@ struct DenseWarp {
   unsigned char *mine;
   unsigned char *bias;
   uint32_t bar, phase;
-  uint32_t turn; // which 2 KB the next result goes through
+  OutPieces out; // of `mine`, 2 KB each
   bool ok;
 };
 
@@ -346,7 +347,7 @@ __global__ void __cluster_dims__(SHAPE == kDenseOne ? 1 : 2, 1, 1) __launch_boun
     }
   } else if (warp >= 4) {
     const int e = warp - 4, part = e / 4;
-    DenseWarp me{end_p + e * kDenseEndBytes, end_p + kDenseEndWarps * kDenseEndBytes + e * kDenseBiasBytes, own + 8 * e, 0, 0, true};
+    DenseWarp me{end_p + e * kDenseEndBytes, end_p + kDenseEndWarps * kDenseEndBytes + e * kDenseBiasBytes, own + 8 * e, 0, {0}, true};
     const uint32_t free_bar = PAIR ? dense_first(tempty) : tempty;
     int buf = 0;
     uint32_t tphase = 0;
@@ -563,6 +564,11 @@ template <int BUT> __device__ __forceinline__ void out_free() { // all copies bu
   if (threadIdx.x % 32 == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUT) : "memory");
   __syncwarp();
 }
+// The same before `pieces` of the warp's shared memory are written and copied out.
+__device__ __forceinline__ void out_claim(DenseWarp &w, uint32_t pieces) {
+  if (w.out.claim(pieces)) out_free<1>();
+  else out_free<0>();
+}
 __device__ __forceinline__ uint4 *out_piece(unsigned char *buf, int i) { // the lane's row's columns 8 i ...
   const int lane = threadIdx.x % 32;
   return reinterpret_cast<uint4 *>(buf) + lane * 4 + (i ^ (lane >> 1 & 3));
@@ -707,7 +713,7 @@ template <class T> __device__ __noinline__ void keep_sums(const Result<T> &f, co
 // by tensor copies where these reach the matrix.  (Reading them a row per lane took longer than the product.)  A warp
 // has two pieces of 2 KB, which results go through by turns; addends that tensor copies bring come there, one for
 // each half of the warp's columns, before the sums are done, and the results replace them; where z is kept too, the
-// second is z's.
+// second is z's, and parts of sums take both.  The two products of a launch use them differently: see OutPieces.
 template <class T> struct ResultEnd {
   Result<T> f;
   struct State {};
@@ -740,7 +746,7 @@ template <class T> struct ResultEnd {
     const int lane = threadIdx.x % 32;
     const int m0 = row - lane;
     if (f.parts) { // (4 KB a time, turned around as their map says)
-      out_free<0>();
+      out_claim(w, 3);
       turn(r, w.mine);
       out_ready();
       if (lane == 0) {
@@ -750,6 +756,8 @@ template <class T> struct ResultEnd {
       return;
     }
     if (f.sums) {
+      out_claim(w, 3);
+      w.out.read = 0; // (nothing is copied out of it)
       turn(r, w.mine);
       return keep_sums(f, w.mine, m0, n, p.M, p.N);
     }
@@ -772,10 +780,9 @@ template <class T> struct ResultEnd {
 #pragma unroll
       for (int i = 0; i < 4; ++i) add8(i, b[i]);
     }
-    unsigned char *to = w.mine + (f.pre ? 0 : f.addend ? (second ? kOutBytes : 0) : w.turn), *kept = w.mine + kOutBytes;
-    w.turn ^= kOutBytes;
-    if (f.addend || f.pre) out_free<0>();
-    else out_free<1>(); // (the other piece's copy may be under way)
+    const uint32_t pieces = f.pre ? 3 : f.addend ? (second ? 2 : 1) : w.out.other();
+    unsigned char *to = w.mine + (pieces == 2 ? kOutBytes : 0), *kept = w.mine + kOutBytes;
+    out_claim(w, pieces);
     if (f.addend) {
       if (!f.tma_addend) {
         copy_in(f.addend, f.ld_addend, m0, n, p.M, p.N, to);
@@ -1057,8 +1064,8 @@ template <class T, int COLS> struct ScoreGradEnd {
   __device__ __forceinline__ void chunk(State &s, const DenseProblem &p, const uint32_t (&r)[32], int row, int n, const DenseUnit &,
                                         DenseWarp &w, bool, bool) const {
     const int lane = threadIdx.x % 32;
-    unsigned char *mine = w.mine + w.turn;
-    w.turn ^= kOutBytes;
+    const uint32_t piece = w.out.other();
+    unsigned char *mine = w.mine + (piece == 2 ? kOutBytes : 0);
     const ulonglong2 *b2 = reinterpret_cast<const ulonglong2 *>(w.bias) + n % COLS / 4;
     const Two less(-s.lse2), weight(s.weight);
     Two v[16];
@@ -1084,7 +1091,7 @@ template <class T, int COLS> struct ScoreGradEnd {
         v[j] = Two(2 * j == at ? x.x - s.weight : x.x, 2 * j + 1 == at ? x.y - s.weight : x.y);
       }
     }
-    out_free<1>(); // (the other piece's copy may be under way)
+    out_claim(w, piece);
     out_put<T>(mine, v);
     const int m0 = row - lane;
     out_ready();
