@@ -71,3 +71,23 @@ def test_layer_gradient_with_skip_and_the_weights_in_one_launch(n, inputs, outpu
         near(outs[0], want, (outputs + 2) * STEP * (G.abs() @ W.abs() + want.abs()))
         near(outs[1], G.t() @ X, (n + 2) * STEP * (G.abs().t() @ X.abs()))
         near(outs[2], G.sum(0), (n + 2) * STEP * G.abs().sum(0))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("size", [0.0, 1e6, 1e9, 1e30, float("inf"), float("nan")])
+def test_weights_of_rows_without_a_label_do_not_count(size, dtype):
+    """Rows without a label have zeros for dz: their weights change no bit of the gradients."""
+    n, width, classes = 300, 64, 1000
+    x, w, b, labels = class_case(n, width, classes, dtype)
+    z, lse, _, live, at = plain_loss(x, w, b, labels)
+    assert 3 < int((~live).sum()) < n // 2
+    weights = torch.full((n,), 1.0 / n, device="cuda")
+    outs = []
+    for kind in (torch.int64, torch.int32):
+        given = torch.where(live, weights, size)
+        outs.append(lm.class_loss_backward(given, x, w, labels.to(kind), lse.float(), b))
+        assert all(torch.equal(p, q) for p, q in zip(outs[-1], lm.class_loss_backward(weights, x, w, labels, lse.float(), b)))
+    class_gradients_are_near(outs[0], x, w, b, labels, weights, z, lse.float(), live, at)
+    # no row with a label: zeros everywhere
+    for o in lm.class_loss_backward(given, x, w, torch.full_like(labels, -100), lse.float(), b):
+        assert (o == 0).all()

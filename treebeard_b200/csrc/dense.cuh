@@ -1167,13 +1167,15 @@ __device__ __forceinline__ void act_grad(const T *grad, long long ld_grad, bool 
   for (int w = 0; w < 8; ++w) s += part[w][k * 32 + l];
   bias_sums[bx * ld + at] = s;
 }
-// The power of two that brings the largest |v| to about 2^13 (1 where nothing finite and nonzero is there).
-__device__ __forceinline__ void find_scale(const float *v, long long n, float *scale, float *tops) {
+// The power of two that brings the largest |v| of the rows that have a label to about 2^13 (1 where nothing finite and
+// nonzero is there).  The other rows' dz are zeros, whatever their weights.
+__device__ __forceinline__ void find_scale(const float *v, const void *labels, int label_bytes, long long classes, long long n, float *scale, float *tops) {
   float top = 0.f;
 #pragma unroll 8
   for (long long i = threadIdx.x; i < n; i += 256) {
     const float a = fabsf(v[i]);
-    if (a < INFINITY) top = fmaxf(top, a);
+    const long long label = label_at(labels, label_bytes, i);
+    if (a < INFINITY && label >= 0 && label < classes) top = fmaxf(top, a);
   }
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
@@ -1188,7 +1190,9 @@ __device__ __forceinline__ void find_scale(const float *v, long long n, float *s
 // matrices whose rows do not begin at multiples of 16 bytes copied to where they do (16 bytes a thread).
 template <class T> struct PrepareJobs {
   const float *weights; // find_scale
-  long long num_weights;
+  const void *labels;
+  int label_bytes;
+  long long num_weights, classes;
   float *scale;
   const T *grad, *pre; // act_grad
   long long ld_grad, ld_pre, ld_dz;
@@ -1208,7 +1212,7 @@ template <class T, int ACT> __global__ void __launch_bounds__(256, 4) tb_dense_p
   __shared__ float part[8][256];
   after_previous_kernel();
   unsigned b = blockIdx.x;
-  if (b < jobs.blocks[0]) return find_scale(jobs.weights, jobs.num_weights, jobs.scale, part[0]);
+  if (b < jobs.blocks[0]) return find_scale(jobs.weights, jobs.labels, jobs.label_bytes, jobs.classes, jobs.num_weights, jobs.scale, part[0]);
   b -= jobs.blocks[0];
   if (b < jobs.blocks[1])
     return act_grad<T, ACT>(jobs.grad, jobs.ld_grad, jobs.vec_grad, jobs.pre, jobs.ld_pre, jobs.vec_pre, jobs.dz, jobs.ld_dz, jobs.bias_sums,

@@ -593,6 +593,7 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
     make_readable(&before, 0, &x, &ld_x, n, width, parts.x);
     make_readable(&before, 1, &weight, &ld_w, classes, width, parts.weight);
     before.weights = grad, before.num_weights = n, before.scale = parts.scale;
+    before.labels = labels, before.label_bytes = label_bytes, before.classes = classes;
     before.blocks[0] = 1;
     TRY(prepare(before, TBK_ACT_IDENTITY, stream));
     const T *W = (const T *)weight;
