@@ -107,8 +107,10 @@ TBK_EXPORT int tbk_class_loss_backward(const float *grad_loss, const void *x, in
                                        int64_t classes, int32_t type, void *workspace, uint64_t workspace_bytes,
                                        int32_t device, void *stream);
 
-/* Reads the status words of these kernels on a device (synchronises with it): TBK_ERR_DEVICE_WAIT if a bounded
- * wait inside one gave up since the last check, else TBK_OK. */
+/* Waits for a device and reads the status words of these kernels on it: TBK_ERR_DEVICE_WAIT if a bounded wait inside
+ * one gave up since the last check, else TBK_OK.  The words are the device's, and reading clears them: of several
+ * threads that use it, the first to ask learns of it.  What the calls since the last check wrote is not to be
+ * trusted then. */
 TBK_EXPORT int tbk_leaf_check_status(int32_t device);
 
 #ifdef __cplusplus

@@ -91,3 +91,19 @@ def test_weights_of_rows_without_a_label_do_not_count(size, dtype):
     # no row with a label: zeros everywhere
     for o in lm.class_loss_backward(given, x, w, torch.full_like(labels, -100), lse.float(), b):
         assert (o == 0).all()
+
+
+def test_the_status_waits_for_every_stream():
+    """Streams of torch do not wait for the legacy stream, nor it for them."""
+    x, w = normal(256, 256, dtype=torch.bfloat16), normal(256, 256, dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    lm.linear(x, w, stream=side)           # (kernels are loaded, memory is there: neither waits below)
+    torch.cuda._sleep(1000)
+    lm.check_status(0)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)     # about a tenth of a second
+        lm.linear(x, w)
+        after = torch.cuda.Event()
+        after.record()
+    lm.check_status(0)
+    assert after.query()

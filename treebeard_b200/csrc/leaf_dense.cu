@@ -650,6 +650,7 @@ int tbk_leaf_check_status(int32_t device) {
   OnDevice on(device);
   CUDA_TRY(on.error);
   int dense = 0, leaf = 0, zero = 0;
+  CUDA_TRY(cudaDeviceSynchronize()); // (copies of symbols wait for no stream that was made non-blocking)
   CUDA_TRY(cudaMemcpyFromSymbol(&dense, tb::tb_dense_status, sizeof dense));
   if (dense) CUDA_TRY(cudaMemcpyToSymbol(tb::tb_dense_status, &zero, sizeof zero));
   TRY(leaf_sum_status(&leaf));

@@ -156,7 +156,9 @@ def _readable(x, ld_x, weight, ld_w):
 
 
 def check_status(device: int = 0):
-    """Waits for the device; raises TbkError if a bounded wait inside one of these kernels gave up since the last check."""
+    """Waits for the device (all of its streams); raises TbkError if a bounded wait inside one of these kernels gave up
+    since the last check.  The status is the device's and is cleared by the check: of several threads, the first to ask
+    learns of it."""
     _check(lib().tbk_leaf_check_status(device))
 
 
