@@ -167,7 +167,7 @@ struct DenseWarp {
   unsigned char *bias;
   uint32_t bar, phase;
   OutPieces out; // of `mine`, 2 KB each
-  bool ok;
+  bool ok, coming; // coming (lane 0): a copy was asked for and has not been waited for
 };
 
 // End: what becomes of a tile.  A thread of a finishing warp has one row and 32 columns at a time:
@@ -347,7 +347,7 @@ __global__ void __cluster_dims__(SHAPE == kDenseOne ? 1 : 2, 1, 1) __launch_boun
     }
   } else if (warp >= 4) {
     const int e = warp - 4, part = e / 4;
-    DenseWarp me{end_p + e * kDenseEndBytes, end_p + kDenseEndWarps * kDenseEndBytes + e * kDenseBiasBytes, own + 8 * e, 0, {0}, true};
+    DenseWarp me{end_p + e * kDenseEndBytes, end_p + kDenseEndWarps * kDenseEndBytes + e * kDenseBiasBytes, own + 8 * e, 0, {0}, true, false};
     const uint32_t free_bar = PAIR ? dense_first(tempty) : tempty;
     int buf = 0;
     uint32_t tphase = 0;
@@ -357,7 +357,7 @@ __global__ void __cluster_dims__(SHAPE == kDenseOne ? 1 : 2, 1, 1) __launch_boun
       typename End::State state[MT];
 #pragma unroll
       for (int j = 0; j < MT; ++j) end.start(state[j], p, row + j * 256, w);
-      for (int n = w.n0; ok && n < w.n1; ++n) {
+      for (int n = w.n0; ok && me.ok && n < w.n1; ++n) {
         const int col = n * BN + part * kColumns;
         end.tile(p, col, me);
 #pragma unroll(sizeof(state) > 2 ? 2 : 1)
@@ -389,13 +389,16 @@ __global__ void __cluster_dims__(SHAPE == kDenseOne ? 1 : 2, 1, 1) __launch_boun
         if (MT == 2) tphase ^= 1;
         else if (++buf == 2) buf = 0, tphase ^= 1;
       }
+      ok = ok && me.ok;
       if (ok) {
 #pragma unroll
         for (int j = 0; j < MT; ++j) end.stop(state[j], p, row + j * 256, w, part);
       }
     });
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); // (stores under way read shared memory)
-    ok = ok && me.ok;
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); // (stores under way read shared memory)
+      if (me.coming) dense_wait(me.bar, me.phase);              // (after a wait that gave up: copies land before the way out)
+    }
   }
   if (!ok) atomicExch(&tb_dense_status, 4);
   __syncwarp();
@@ -734,10 +737,11 @@ template <class T> struct ResultEnd {
   }
   // (row: the lane's; the first lane's is the warp's first)
   __device__ __forceinline__ void ahead(const DenseProblem &p, int row, int n, int columns, DenseWarp &w) const {
-    if (!f.addend || !f.tma_addend || f.parts || threadIdx.x % 32) return;
+    if (!f.addend || !f.tma_addend || f.parts || !w.ok || threadIdx.x % 32) return;
     const bool two = columns > 32 && n + 32 < p.N && !f.pre;
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); // (the last results may still be on their way)
     dense_expect(w.bar, two ? 2 * kOutBytes : kOutBytes);
+    w.coming = true;
     fetch(row, n, w.mine, w);
     if (two) fetch(row, n + 32, w.mine + kOutBytes, w);
   }
@@ -787,8 +791,7 @@ template <class T> struct ResultEnd {
       if (!f.tma_addend) {
         copy_in(f.addend, f.ld_addend, m0, n, p.M, p.N, to);
       } else if (!second || f.pre) {
-        if (w.ok) w.ok = __all_sync(~0u, dense_wait(w.bar, w.phase));
-        w.phase ^= 1;
+        if (w.ok && (w.ok = __all_sync(~0u, dense_wait(w.bar, w.phase)))) w.phase ^= 1, w.coming = false;
       }
     }
     if (f.pre) out_put<T>(kept, z);
@@ -810,9 +813,10 @@ template <class T> struct ResultEnd {
         if (f.pre && f.tma_pre) out_send(&f.pre_map, kept, m0, n);
       }
       out_commit();
-      if (more && f.addend && f.tma_addend && f.pre) { // (no room for it before)
+      if (more && f.addend && f.tma_addend && f.pre && w.ok) { // (no room for it before)
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         dense_expect(w.bar, kOutBytes);
+        w.coming = true;
         fetch(m0, n + 32, w.mine, w);
       }
     }
