@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kLeafStagedThreads, 1)
     for (int u = 0; ok && u < units; ++tile, b0 = 0) {
       const int b1 = min(batches, b0 + (units - u));
       unsigned long long acc[kLeafRows][P] = {};
-      for (int b = b0; ok && b < b1; ++b) {
+      for (int b = b0; b < b1; ++b) { // (all lanes leave it together: the warp votes)
         const int now = min(kLeafBatch, trees - b * kLeafBatch);
         if (!(ok = __all_sync(~0u, ok && leaf_wait(found + 8 * slot, slot_phase)))) break;
         const uint16_t *place = places + slot * kLeafBatch * kLeafMostRows + group * kLeafRows;
@@ -462,6 +462,7 @@ __global__ void __launch_bounds__(kLeafStagedThreads, 1)
         if (wl == 0) leaf_arrive(used + 8 * slot);
         if (++slot == kLeafSlots) slot = 0, slot_phase ^= 1;
       }
+      ok = __all_sync(~0u, ok);
       const bool whole = b0 == 0 && b1 == batches;
       const long long part = whole ? 0 : blockIdx.x - work.block_of((long long)tile * batches);
 #pragma unroll
