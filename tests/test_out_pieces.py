@@ -2,6 +2,7 @@
 whatever products follow one another.  The bookkeeping is the kernel's own header, compiled for the host; the
 copies are those of a model that lets each finish as late as the waits allow."""
 import os
+import re
 import subprocess
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -55,3 +56,12 @@ def test_the_kernels_ask_before_they_write():
     assert "out_free<" not in body[0].split("void out_free()")[0]
     inside, after = body[1].split("\n}\n", 1)
     assert inside.count("out_free<") == 2 and "out_free<" not in after
+
+
+def test_only_the_leaf_map_is_read_as_constant():
+    """Kernels that are resident while their predecessor runs read its results by plain loads."""
+    csrc = os.path.join(ROOT, "treebeard_b200", "csrc")
+    for name in ("leaf_sum.cuh", "dense.cuh", "element.cuh"):
+        code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+        assert "ld.global.nc" not in code and "__restrict__" not in code
+        assert not [a for a in re.findall(r"__ldg\(([^;]*)", code) if not re.match(r"(m\.(trees|rows)|words) \+", a)]

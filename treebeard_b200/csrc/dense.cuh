@@ -550,12 +550,12 @@ template <class T> __device__ __forceinline__ void load8(const T *p, float (&v)[
 }
 
 template <class T> __device__ __forceinline__ uint4 raw8(const T *p, int n, bool vec) { // eight elements as they are, n of them there
-  if (vec && n >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+  if (vec && n >= 8) return *reinterpret_cast<const uint4 *>(p);
   uint32_t w[4] = {0, 0, 0, 0};
   const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (i < n) w[i / 2] |= (uint32_t)__ldg(q + i) << (i % 2 * 16);
+    if (i < n) w[i / 2] |= (uint32_t)q[i] << (i % 2 * 16);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 

@@ -28,10 +28,34 @@ template <class T> __device__ __forceinline__ void add_halves(unsigned long long
 }
 
 // Kernels of one call follow one another closely: each is launched while the one before still runs, prepares itself
-// and waits here until that one's results are there (and lets its own follower come).
+// and waits here until that one's results are there (and lets its own follower come).  What is read afterwards is read
+// by plain loads: __ldg is for data that nothing writes while the grid is resident.
 __device__ __forceinline__ void after_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Loads of such results.  (As statements of their own, which stay behind the wait but may be moved past shuffles and
+// past stores to shared memory, where those of plain expressions may not.)
+__device__ __forceinline__ uint4 load_result(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 load_result(const uint2 *p) {
+  uint2 v;
+  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t load_result(const uint32_t *p) {
+  uint32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint16_t load_result(const uint16_t *p) {
+  uint16_t v;
+  asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(p));
+  return v;
 }
 
 } // namespace tb

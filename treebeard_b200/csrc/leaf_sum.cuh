@@ -14,6 +14,10 @@
 
 namespace tb {
 
+// The leaf map alone is read through __ldg: it does not change while it exists.  What an earlier kernel of the stream may
+// have written is not: these kernels are resident while that one still runs, and such loads may be moved ahead of the
+// wait for it.
+//
 // Which table row a leaf has: leaves are numbered in node order, so a leaf's number is the count of leaves
 // before it -- the leaves of earlier words of 32 nodes, kept, and those of its own word, counted from its
 // bits.  A tree of 8 levels is 128 bytes of this, one line, where a number per node would be sixteen.
@@ -45,17 +49,17 @@ template <class T, int V> struct Share {
   static __device__ __forceinline__ uint4 load(const unsigned char *p, long long c, long long width) {
     uint4 q = make_uint4(0, 0, 0, 0);
     if constexpr (V == 16) {
-      if (c < width) q = __ldg(reinterpret_cast<const uint4 *>(p));
+      if (c < width) q = load_result(reinterpret_cast<const uint4 *>(p));
     } else {
       uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
         if (c + i * kPer < width) {
           if constexpr (V == 8) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+            const uint2 x = load_result(reinterpret_cast<const uint2 *>(p) + i);
             w[2 * i] = x.x, w[2 * i + 1] = x.y;
-          } else if constexpr (V == 4) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
-          else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + i) << (i % 2 * 16);
+          } else if constexpr (V == 4) w[i] = load_result(reinterpret_cast<const uint32_t *>(p) + i);
+          else w[i / 2] |= (uint32_t)load_result(reinterpret_cast<const uint16_t *>(p) + i) << (i % 2 * 16);
         }
       q = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(kLeafRowThreads) tb_leaf_sum_row_kernel(LeafMa
     for (int i = 0; i < 8; ++i) {
       const long long t = t0 + (long long)i * groups + group;
       tree[i] = t < m.num_trees ? __ldg(m.trees + t) : make_int2(0, 0);
-      r[i] = t < m.num_trees ? __ldg(id + t) : -1;
+      r[i] = t < m.num_trees ? id[t] : -1;
     }
     uint2 word[8];
 #pragma unroll
@@ -224,7 +228,7 @@ __global__ void __launch_bounds__(512, 1) tb_leaf_sum_kernel(LeafMapView m, cons
       const int2 tree = there ? __ldg(m.trees + t) : make_int2(0, 0);
       int32_t row[kLeafRows];
 #pragma unroll
-      for (int i = 0; i < kLeafRows; ++i) row[i] = there ? __ldg(id_at[i] + t) : -1;
+      for (int i = 0; i < kLeafRows; ++i) row[i] = there ? id_at[i][t] : -1;
       bool all = true;
 #pragma unroll
       for (int i = 0; i < kLeafRows; ++i) {
@@ -369,11 +373,11 @@ __global__ void __launch_bounds__(kLeafStagedThreads, 1)
         // (what is behind the tile's or the batch's last row is not kept)
         const int32_t *at = ids + (long long)min(tile * tile_rows + min(row, tile_rows - 1), n_rows - 1) * ld_ids + t0;
         if (vec_ids && now == kLeafBatch) {
-          const int4 a = __ldg(reinterpret_cast<const int4 *>(at)), b = __ldg(reinterpret_cast<const int4 *>(at) + 1);
+          const int4 a = reinterpret_cast<const int4 *>(at)[0], b = reinterpret_cast<const int4 *>(at)[1];
           next[k][0] = a.x, next[k][1] = a.y, next[k][2] = a.z, next[k][3] = a.w, next[k][4] = b.x, next[k][5] = b.y, next[k][6] = b.z, next[k][7] = b.w;
         } else {
 #pragma unroll
-          for (int j = 0; j < kLeafBatch; ++j) next[k][j] = j < now ? __ldg(at + j) : -1;
+          for (int j = 0; j < kLeafBatch; ++j) next[k][j] = j < now ? at[j] : -1;
         }
       }
       const bool there = wl < now; // (of the trees behind the last one nothing is found)
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(256) tb_leaf_numbers_kernel(LeafMapView m, con
 #pragma unroll
     for (int i = 0; i < kNumberRows / 8; ++i) {
       const int row = i / 2 * 16 + 2 * y + i % 2;
-      v[i] = row < rows && x < trees ? __ldg(from + row * ld_ids) : -1;
+      v[i] = row < rows && x < trees ? from[row * ld_ids] : -1;
     }
 #pragma unroll
     for (int i = 0; i < kNumberRows / 16; ++i) tile[x][i * 8 + y] = make_int2(v[2 * i], v[2 * i + 1]);
@@ -588,10 +592,10 @@ __global__ void __launch_bounds__(32 * kLeafGradWarps, 2) tb_leaf_grad_kernel(Le
   const int32_t tree_row = kIds ? __ldg(m.rows + t) : 0;
   auto number = [&](long long i) -> uint32_t {
     if constexpr (kIds) {
-      const int32_t r = leaf_row(m.words, tree, __ldg(mine + i * ld_numbers));
+      const int32_t r = leaf_row(m.words, tree, mine[i * ld_numbers]);
       return r < 0 ? kNone : (uint32_t)(r - tree_row);
     } else {
-      return __ldg(mine + i);
+      return mine[i];
     }
   };
 
