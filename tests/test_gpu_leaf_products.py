@@ -107,3 +107,32 @@ def test_the_status_waits_for_every_stream():
         after.record()
     lm.check_status(0)
     assert after.query()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("classes", [1, 2, 31, 300, 1500])
+def test_losses_of_sure_rows(classes, bias, dtype):
+    """Scores up to 300 that no sum rounds (small whole numbers): a loss is off only by its own exponentials and
+    logarithm, however large the scores are, and never below 0; with one class it is 0, and so are all gradients."""
+    n = 200
+    g = torch.Generator().manual_seed(classes)
+    x = torch.randint(-6, 7, (n, 8), generator=g).to(dtype).cuda()
+    w = torch.randint(-6, 7, (classes, 8), generator=g).to(dtype).cuda()
+    b = torch.randint(-12, 13, (classes,), generator=g).to(dtype).cuda() if bias else None
+    z = x.double() @ w.double().t() + (b.double() if bias else 0.0)
+    labels = z.argmax(1)                      # (the sure ones; every third row something else)
+    labels[::3] = torch.arange(n, device="cuda")[::3] % classes
+    loss, lse = lm.class_loss(x, w, labels, b)
+    top = z.max(1, keepdim=True).values
+    rest = torch.exp(z - top).sum(1).log()
+    want = (top - z.gather(1, labels[:, None]))[:, 0] + rest
+    # a sum of exponentials relative to the largest: each is off by 2^-22 and, e^-d d <= 0.37, by the roundings of its
+    # argument d; 32 additions one behind the other in a chunk and one for each chunk and part: (8 + 16 + classes / 32) steps
+    off = (24 + classes / 32) * STEP
+    assert (loss >= 0).all() and z.abs().max() > 50
+    near(loss, want, off + STEP * want)
+    near(lse, top[:, 0] + rest, off + STEP * z.abs().max())
+    outs = lm.class_loss_backward(torch.full((n,), 1 / n, device="cuda"), x, w, labels, lse, b)
+    if classes == 1:
+        assert (loss == 0).all() and torch.equal(lse.double(), z[:, 0]) and all((o == 0).all() for o in outs)
