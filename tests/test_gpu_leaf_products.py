@@ -136,3 +136,21 @@ def test_losses_of_sure_rows(classes, bias, dtype):
     outs = lm.class_loss_backward(torch.full((n,), 1 / n, device="cuda"), x, w, labels, lse, b)
     if classes == 1:
         assert (loss == 0).all() and torch.equal(lse.double(), z[:, 0]) and all((o == 0).all() for o in outs)
+
+
+@pytest.mark.parametrize("classes", [5, 300, 3000])
+def test_infinite_scores(classes):
+    """A row with an infinite score has an infinite logarithm, and so has its loss unless the label is that class."""
+    n = 70
+    x, w, b, labels = class_case(n, 16, classes, torch.bfloat16)
+    b[-1] = float("inf")
+    x[3, 0] = float("nan")
+    z, lse, loss, live, at = plain_loss(x, w, b, labels)
+    got, got_lse = lm.class_loss(x, w, labels, b)
+    rest = [i for i in range(n) if i != 3]
+    assert (got_lse[rest] == float("inf")).all() and got_lse[3].isnan()
+    hit = live & (labels == classes - 1)
+    assert hit.any() and got[hit].isnan().all() and (got[~live] == 0).all()
+    other = live & ~hit
+    other[3] = False
+    assert (got[other] == float("inf")).all()

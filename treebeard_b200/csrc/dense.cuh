@@ -945,6 +945,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) { // (not a num
   return d;
 }
 
+// What is subtracted from scores whose largest is `top`: nothing where that is infinite (all so far forbidden, their
+// exponentials are 0; or infinite, and the sum with it).
+__device__ __forceinline__ float lse_ref(float top) { return fabsf(top) == INFINITY ? 0.f : top; }
+
 // Sum of a row's exponentials over the tiles of a unit, relative to the largest score of them, in one pass:
 // the sum so far is scaled down whenever a larger score comes.  Scores become powers of two after the largest has
 // been subtracted (an operation more for two scores than scaling them first; 4096 x 100003 scores: 64 columns 151 to
@@ -994,7 +998,7 @@ template <class T, int COLS> struct LseEnd {
       tops[j & 1] = max3(tops[j & 1], x.x, x.y);
       tops[j & 1] = max3(tops[j & 1], y.x, y.y);
     }
-    const float top = fmaxf(tops[0], tops[1]), ref = top == -INFINITY ? 0.f : top; // (all so far forbidden: exponentials are 0)
+    const float top = fmaxf(tops[0], tops[1]), ref = lse_ref(top);
     const Two less(-ref);
     Two sum[2] = {Two(0.f), Two(0.f)};
 #pragma unroll
@@ -1021,7 +1025,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) tb_loss_join_kernel(const flo
   const long long m = (long long)blockIdx.x * 32 + lane;
   float top = -INFINITY, sum = 0.f;
   auto join = [&](float2 q) {
-    const float most = fmaxf(top, q.x), ref = most == -INFINITY ? 0.f : most;
+    const float most = fmaxf(top, q.x), ref = lse_ref(most);
     sum = sum * exp2_fast((top - ref) * kLog2e) + q.y * exp2_fast((q.x - ref) * kLog2e);
     top = most;
   };
