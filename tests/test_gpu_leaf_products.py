@@ -154,3 +154,19 @@ def test_infinite_scores(classes):
     other = live & ~hit
     other[3] = False
     assert (got[other] == float("inf")).all()
+
+
+@pytest.mark.parametrize("name", ["relu", "gelu", "silu"])
+def test_slopes_where_the_kept_value_rounded_to_infinity(name):
+    """In fp16 a value below -65520 is kept as -inf; its slope is 0 and those above 65520 have 1.  NaN stays NaN."""
+    x = torch.tensor([[-300.0], [300.0], [2.0], [float("nan")]], device="cuda").half()
+    w = torch.tensor([[400.0], [1.0]], device="cuda").half()
+    y, pre = lm.linear(x, w, None, name, keep_pre=True)
+    assert pre[0, 0] == float("-inf") and pre[1, 0] == float("inf") and y[0, 0] == 0
+    g = torch.full((4, 2), 0.5, device="cuda").half()
+    dx, dw, db = lm.linear_backward(g[:3], x[:3], w, pre[:3], name)
+    assert torch.isfinite(dw).all() and torch.isfinite(db).all()
+    slopes = torch.tensor([0.0, 1.0], device="cuda").half()
+    assert torch.equal(lm.linear_backward(g[:2, :1], x[:2], torch.ones_like(w[:1]), pre[:2, :1], name)[0][:, 0], 0.5 * slopes)
+    if name != "relu":
+        assert lm.linear_backward(g[3:], x[3:], w, pre[3:], name)[0].isnan().all()

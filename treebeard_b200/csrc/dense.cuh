@@ -492,7 +492,11 @@ template <int ACT> __device__ __forceinline__ float2 act_value(float2 z) {
     return make_float2(z.x * inverse_fast(1.f + exp2_fast(-kLog2e * z.x)), z.y * inverse_fast(1.f + exp2_fast(-kLog2e * z.y)));
   return z;
 }
+// An infinite z, as the rounding of a kept value to fp16 can bring, has the slope of a large one: without this it
+// would be infinity times the 0 of the tail.
+__device__ __forceinline__ float finite(float z) { return fabsf(z) == INFINITY ? copysignf(1e30f, z) : z; }
 template <int ACT> __device__ __forceinline__ float2 act_slope(float2 z) {
+  if constexpr (ACT == kActGelu || ACT == kActSilu) z = make_float2(finite(z.x), finite(z.y));
   if constexpr (ACT == kActRelu) return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
   if constexpr (ACT == kActGelu) { // Phi(z) + z phi(z)
     float2 bell;
