@@ -9,15 +9,17 @@
  * tbk_last_error() has the message.  Matrices are row-major, `ld_*` elements from row to row (columns lie
  * one behind the other).  All device pointers belong to `device`, which need not be the current one; the
  * current device is left as it was.  Calls are ordered by `stream` and may be captured; nothing is
- * allocated and no state is kept between calls.  A call that asks for a workspace takes device memory of
+ * allocated, and nothing is kept between calls but how sizes are cut, which the sizes decide.  A call that asks for a workspace takes device memory of
  * the size that its *_workspace function states, 256-byte aligned, for its own use until its work on the
  * stream is done: calls that may run at the same time need workspaces of their own.
  * `aligned` of these functions: 1 if x and weight begin at 16-byte boundaries and have row strides that are
- * multiples of 8 elements; otherwise a call copies them first, and its workspace has room for that.
+ * multiples of 8 elements; otherwise every call copies them first, as a whole, and its workspace has room for
+ * that (4096 rows of 513 columns, 100003 classes: 442 us, with 512 columns 332).
  * Inputs and outputs of one call must not overlap, except that `out` may be `residual`.
  *
- * Sums are held in fp32 and every output is rounded once from there; the order of all sums is fixed, so
- * equal inputs give equal bits.
+ * Sums are held in fp32 and every output is rounded once from there.  The order of all sums is fixed: equal calls
+ * give equal bits.  It depends on sizes and, in tbk_leaf_sum, on strides and alignment too (a table whose rows do not
+ * lie one behind the other takes another kernel, which joins other parts).
  */
 #ifndef TBK_LEAF_H
 #define TBK_LEAF_H
@@ -73,7 +75,8 @@ TBK_EXPORT int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64
  * rows.  skip [n_rows, inputs] or NULL: what else reaches x's gradient, as where x is the residual too (then
  * skip is grad).
  * pre may be NULL with TBK_ACT_IDENTITY; grad_x, grad_weight, grad_bias may each be NULL (not wanted).
- * dz is rounded to `type` before the two products (grad_bias is summed before that). */
+ * dz is rounded to `type` before the two products (grad_bias is summed before that), without a scale: in fp16
+ * a |dz| above 65504 becomes infinite and one below 6e-5 loses digits, so grad has to come scaled. */
 TBK_EXPORT int tbk_linear_backward_workspace(int64_t n_rows, int64_t inputs, int64_t outputs, int32_t type,
                                                int32_t aligned, int32_t device, uint64_t *bytes);
 TBK_EXPORT int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_t ld_x, const void *weight,
@@ -85,7 +88,8 @@ TBK_EXPORT int tbk_linear_backward(const void *grad, int64_t ld_grad, const void
 /* Softmax cross entropy over `classes` classes without keeping the scores z = x weight^T + bias:
  * lse[n] = log sum_v exp(z[n, v]), loss[n] = lse[n] - z[n, labels[n]], both fp32.  A label outside
  * 0 .. classes-1 leaves its row out: loss 0.  labels: int64 (label_bytes 8) or int32 (4).  A class whose
- * bias is -inf has probability 0; a row of such classes only has lse = -inf. */
+ * bias is -inf has probability 0; a row of such classes only has lse = -inf and, with a label, a loss and
+ * gradients that are not numbers. */
 TBK_EXPORT int tbk_class_loss_workspace(int64_t n_rows, int64_t width, int64_t classes, int32_t type,
                                                int32_t aligned, int32_t device, uint64_t *bytes);
 TBK_EXPORT int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_weight, const void *bias,

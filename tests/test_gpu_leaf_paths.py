@@ -165,3 +165,30 @@ def test_tiles_of_large_layers():
     near(dx, G @ W, 5002 * STEP * (G.abs() @ W.abs()))
     near(dw, G.t() @ X, 9002 * STEP * (G.abs().t() @ X.abs()))
     near(db, G.sum(0), 9002 * STEP * G.abs().sum(0))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_a_model_of_many_rows_with_weights_of_ones(dtype):
+    """What fp16 asks for at training batches: gradients of the sum, whose size the type holds."""
+    n, classes = 20000, 700
+    forest, marg = grown(30, 5)
+    rows = torch.from_numpy(marg.sample_rows(np.random.default_rng(0), n)).cuda()
+    params = dict(table=normal(lm.LeafMap(forest).num_rows, 48, dtype=dtype, scale=30 ** -0.5), w1=normal(96, 48, dtype=dtype, scale=48 ** -0.5, seed=1),
+                  w2=normal(96, 96, dtype=dtype, scale=96 ** -0.5, seed=3), wc=normal(classes, 96, dtype=dtype, scale=96 ** -0.5, seed=4),
+                  bc=normal(classes, dtype=dtype, scale=0.1, seed=5))
+    model = lm.LeafModel(forest, params["table"], [(params["w1"], None, "gelu", False), (params["w2"], None, "silu", True)], params["wc"], params["bc"])
+    labels = torch.arange(n, device="cuda") * 13 % classes
+    loss, grads = model.loss_and_grads(rows, labels, torch.ones(n, device="cuda"))
+    q = {k: v.double().requires_grad_(True) for k, v in params.items()}
+    h = q["table"][table_rows(forest, model.forest.predict_leaf_ids(rows))].sum(1)
+    h = ACT["gelu"][0](h @ q["w1"].t())
+    h = ACT["silu"][0](h @ q["w2"].t()) + h
+    z = h @ q["wc"].t() + q["bc"]
+    want = torch.logsumexp(z, 1) - z.gather(1, labels[:, None])[:, 0]
+    want.sum().backward()
+    # (the roundings of a chain, as in the smaller model's test: 8 half steps in the 2-norm)
+    half = torch.finfo(dtype).eps / 2
+    assert (loss.double() - want).norm() <= 8 * half * want.norm()
+    got = dict(table=grads["table"], w1=grads["layers"][0][0], w2=grads["layers"][1][0], wc=grads["weight"], bc=grads["bias"])
+    for k in q:
+        assert (got[k].double() - q[k].grad).norm() <= 8 * half * q[k].grad.norm(), k

@@ -18,10 +18,10 @@
 //               the tall one's rate; two tiles' accumulators, one taken out while the other is computed.
 //   kDenseOne   one block on 128 x 128 results, for products with few tiles: 128 + 128, half the rate.
 // Plain products, bf16: 8192 x 8192 x 8192 at 1.50 to 1.53 PFLOP/s (cuBLAS 1.60), 32768 x 1024 -> 4096 at 1.35 to 1.39
-// (1.40), in 198 to 205 us; with gelu and the value before it as a second result 284.
-// Those bytes are not all: of 4096 x 512 -> 100003 classes (327 us; the tensor pipe is busy 68 % of the cycles, at 1.65 GHz)
-// a pair that kept A in shared memory for eight tiles, 32 + 64, took 358, one with six stages instead of four as
-// long as this.
+// (1.40), in 198 to 205 us; with gelu and the value before it as a second result 267 to 316.
+// Those bytes are not all: of 4096 x 512 -> 100003 classes (332 to 346 us; the tensor pipe is busy 67 % of the cycles, at
+// 1.62 GHz) a pair that kept A in shared memory for eight tiles, 32 + 64, took 31 us more, one with six stages instead of
+// four as long as this.
 //
 // All waits are bounded: one that gives up ends the launch with a word in tb_dense_status.
 #pragma once
@@ -460,8 +460,10 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
 
 // -Phi(-|z|), Phi the integral of the normal distribution, and exp(-z^2 / 2), of two z.  erfc's shape after Hastings
 // (Approximations for Digital Computers, 1955): Phi(-|z|) = exp(-z^2 / 2) t P(t), t = 1 / (1 + 0.33 |z|);
-// P was fitted here, by reweighted least squares, for the relative error: below 1e-6 for all z.  Without
-// branches, since a warp's values need both sides of any (the library's erff took most of a layer's time).
+// P was fitted here, by reweighted least squares, for the relative error, 1e-6.  In fp32, with the exponential of a
+// rounded square, it is 2e-6 + z^2 2^-24 up to |z| = 13, beyond which the exponential is 0; |z| times it, what gelu takes
+// off max(z, 0), is off by less than 4e-7.  Without branches, since a warp's values need both sides of any (the
+// library's erff took most of a layer's time).
 __device__ __forceinline__ Two normal_tail(float2 z, float2 size, float2 *bell) { // size: |z|, finite
   const Two zz(z), a(size);
   const float2 d = fma2(a, Two(0.33f), Two(1.f)).get();

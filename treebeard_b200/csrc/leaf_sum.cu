@@ -89,7 +89,8 @@ struct LeafSumPlan {
     }
   }
   // Tables of trees are staged where three stages hold the largest and a tile has as many rows as the
-  // largest tree leaves (with fewer, more bytes are copied than read).
+  // largest tree leaves (with fewer, more bytes are copied than read).  A tile's places have room for kLeafMostRows,
+  // which shuts out rows of less than eight lanes: an array's size, no measured border.
   bool staged(int64_t max_rows, int64_t row_bytes) const {
     return !by_row && columns == 1 && threads == 512 && staged_rows <= tb::kLeafMostRows && max_rows <= staged_rows && max_rows * row_bytes + tb::kLeafZeros <= kLeafStagedSmem / 3;
   }

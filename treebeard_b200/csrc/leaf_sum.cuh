@@ -4,8 +4,8 @@
 //   dtable[r,:] = sum of grad[n, :] over the (n, t) with row(t, id[n, t]) = r
 //
 // Both move one table or gradient row per (batch row, tree) between L2 and the multiprocessors and add it up
-// in registers; nothing of that size goes to memory.  Sums are fp32 in an order that the sizes alone decide,
-// rounded once.
+// in registers; nothing of that size goes to memory.  Sums are fp32, rounded once, in an order that sizes decide and, for
+// out, whether the staged kernel takes the call (alignment, table rows one behind the other).
 #pragma once
 #include "element.cuh"
 
@@ -273,9 +273,9 @@ __global__ void __launch_bounds__(512, 1) tb_leaf_sum_kernel(LeafMapView m, cons
 // takes a quarter of a warp at least.  One warp copies the tables of the trees to come into a ring of stages, one
 // bulk copy a tree; three look up, eight trees at a time, where in its stage each batch row's table row will lie;
 // twelve add up, a lane group its eight rows: an address and a read of 30 cycles each, instead of the hundreds of an
-// L1 miss.  A table is copied once for a block's tile of rows.  20011 rows, 1000 trees of 256 leaves, 64 bf16: 221 us
-// with the join (the kernel above: 253); 60 % of shared memory's cycles and 2.1 of 4 instructions a cycle are used, so
-// latency bounds it.  Waits are bounded: one that gives up sets
+// L1 miss.  A table is copied once for a block's tile of rows.  20011 rows, 1000 trees of 256 leaves, 64 bf16: 217 us
+// with the join (the kernel above: 241); 60 % of shared memory's cycles and 2.1 of 4 instructions a cycle are used:
+// neither is the limit, and what is was not found.  Waits are bounded: one that gives up sets
 // tb_leaf_status.
 __device__ int tb_leaf_status;
 constexpr int kLeafAdders = 12, kLeafFinders = 3, kLeafStagedThreads = 32 * (kLeafAdders + kLeafFinders + 1);

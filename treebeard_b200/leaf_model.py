@@ -290,7 +290,9 @@ def linear(x, weight, bias=None, activation: str = "identity", residual=None, ke
 def linear_backward(grad, x, weight, pre=None, activation: str = "identity", bias: bool = True, skip=None):
     """Gradients of linear from grad, the gradient of its result (which is the residual's gradient too):
     (of x, of weight) and, with ``bias``, of the bias.  pre is what linear kept; identity needs none.
-    skip [n, inputs] is added to x's gradient: grad itself, where x was the residual too."""
+    skip [n, inputs] is added to x's gradient: grad itself, where x was the residual too.
+    grad times the activation's slope is rounded to the type before the products: in fp16 it should lie between
+    6e-5 and 65504, so scale the loss."""
     kind = _half(x, "linear_backward")
     dtype = x.dtype
     ld_x = _matrix("x", x, dtype)
@@ -414,7 +416,9 @@ class LeafModel:
 
     def loss_and_grads(self, rows, labels, row_weights=None):
         """(loss [n], gradients of sum(row_weights * loss)); row_weights: fp32 [n], 1/n each if None.
-        Gradients: {"table", "layers": [(weight, bias or None)], "weight", "bias" or None}."""
+        Gradients: {"table", "layers": [(weight, bias or None)], "weight", "bias" or None}, of the parameters' type, as
+        are those between the layers.  fp16 has few digits below 6e-5, where weights of 1/n lead with thousands of rows:
+        pass larger ones (ones, say) and divide in the optimiser.  bf16 needs no scale."""
         kept = []
         h = self.features(rows, kept)
         loss, lse = class_loss(h, self.weight, labels, self.bias)
