@@ -170,3 +170,46 @@ def test_slopes_where_the_kept_value_rounded_to_infinity(name):
     assert torch.equal(lm.linear_backward(g[:2, :1], x[:2], torch.ones_like(w[:1]), pre[:2, :1], name)[0][:, 0], 0.5 * slopes)
     if name != "relu":
         assert lm.linear_backward(g[3:], x[3:], w, pre[3:], name)[0].isnan().all()
+
+
+def test_arguments_that_are_given_up_while_another_stream_reads_them():
+    """A temporary's memory is not handed out again before the call on the other stream has read it."""
+    w = normal(512, 512, dtype=torch.bfloat16)
+    x = normal(2048, 512, dtype=torch.bfloat16)
+    want = lm.linear(x * 2, w)
+    side = torch.cuda.Stream()
+    lm.linear(x, w, stream=side)          # (kernels are loaded, memory is there)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        here = x * 2
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)
+        got = lm.linear(here, w, stream=side)
+        del here
+        foreign = [torch.full_like(x, float("nan")) for _ in range(4)]   # on the current stream, meanwhile
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del foreign
+
+
+def test_a_captured_call_on_a_forked_stream_with_a_temporary():
+    w = normal(512, 512, dtype=torch.bfloat16)
+    x = normal(2048, 512, dtype=torch.bfloat16)
+    want = lm.linear(x * 2, w)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    lm.linear(x, w, stream=side)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        twice = x * 2
+        side.wait_stream(here)
+        got = lm.linear(twice, w, stream=side)
+        del twice
+        foreign = [torch.full_like(x, float("nan")) for _ in range(4)]
+        here.wait_stream(side)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and all(f.isnan().all() for f in foreign)

@@ -7,6 +7,8 @@ activation and residual, ``class_loss`` the softmax cross entropy over as many c
 scores are never stored).  Each has its gradient as a call of its own; the calls take part in no autograd
 graph.  All of them are ordered by the current stream of the tensors' device, or by ``stream``, and can be
 captured into a CUDA graph; a workspace, where one is needed, comes from torch's allocator on that stream.
+With ``stream`` the arguments may be given up right after the call; results belong to that stream, and whoever uses
+them on another waits for it first.
 
 The reference ends at the forest's own prediction and has no counterpart.
 """
@@ -126,11 +128,15 @@ def _on_stream(call):
     def wrapper(*args, stream=None, **kwargs):
         if stream is None:
             return call(*args, **kwargs)
-        for t in (*args, *kwargs.values()):
-            if isinstance(t, torch.Tensor) and t.get_device() != stream.device.index:
+        tensors = [t for t in (*args, *kwargs.values()) if isinstance(t, torch.Tensor)]
+        for t in tensors:
+            if t.get_device() != stream.device.index:
                 _refuse(f"the stream is on {stream.device}, a tensor of the call is not")
         with torch.cuda.stream(stream):
-            return call(*args, **kwargs)
+            result = call(*args, **kwargs)
+        for t in tensors:   # (memory that its owner gives back meanwhile is not handed out before the work is done)
+            t.record_stream(stream)
+        return result
     return wrapper
 
 
