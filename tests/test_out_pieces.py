@@ -5,6 +5,8 @@ import os
 import re
 import subprocess
 
+import pytest
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # every sequence of eight results; p: a part of a sum (both pieces), k: a result and what it was before the activation
 # (both), a, b: the first and second half of a tile with an addend, r: any other result, s: a sum kept without a copy
@@ -65,3 +67,32 @@ def test_only_the_leaf_map_is_read_as_constant():
         code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
         assert "ld.global.nc" not in code and "__restrict__" not in code
         assert not [a for a in re.findall(r"__ldg\(([^;]*)", code) if not re.match(r"(m\.(trees|rows)|words) \+", a)]
+
+
+def test_addresses_between_elements_are_refused():
+    """On the host, before any launch: such a read would end the program."""
+    torch = pytest.importorskip("torch")    # (the binding's)
+    from treebeard_b200 import leaf_model as lm
+    L, p = lm.lib(), 1 << 20
+    names = "x w bias res out pre".split()
+
+    def linear(**odd):
+        a = {n: p + odd.get(n, 0) for n in names}
+        return L.tbk_linear(a["x"], 8, a["w"], 8, a["bias"], 0, a["res"], 4, a["out"], 4, a["pre"], 4, 4, 8, 4, 2, None, 0, 0, None)
+    for name in names:
+        assert linear(**{name: 1}) == 1 and b"multiple" in L.tbk_last_error(), name
+
+    def back(g=0, x=0, w=0, pre=0, skip=0, gx=0, gw=0, gb=0):
+        return L.tbk_linear_backward(p + g, 4, p + x, 8, p + w, 8, p + pre, 4, 2, p + skip, 8, p + gx, 8, p + gw, 8, p + gb, 4, 8, 4, 1, p, 1 << 40, 0, None)
+    for name in "g x w pre skip gx gw gb".split():
+        assert back(**{name: 1}) == 1 and b"multiple" in L.tbk_last_error(), name
+
+    def loss(x=0, w=0, bias=0, labels=0, loss=0, lse=0):
+        return L.tbk_class_loss(p + x, 8, p + w, 8, p + bias, p + labels, 8, p + loss, p + lse, 4, 8, 100, 1, p, 1 << 40, 0, None)
+    for name, by in (("x", 1), ("w", 1), ("bias", 1), ("labels", 4), ("loss", 2), ("lse", 2)):
+        assert loss(**{name: by}) == 1 and b"multiple" in L.tbk_last_error(), name
+
+    def loss_back(g=0, x=0, w=0, bias=0, labels=0, lse=0, gx=0, gw=0, gb=0):
+        return L.tbk_class_loss_backward(p + g, p + x, 8, p + w, 8, p + bias, p + labels, 4, p + lse, p + gx, 8, p + gw, 8, p + gb, 4, 8, 100, 1, p, 1 << 40, 0, None)
+    for name, by in (("g", 2), ("x", 1), ("w", 1), ("bias", 1), ("labels", 2), ("lse", 2), ("gx", 1), ("gw", 1), ("gb", 1)):
+        assert loss_back(**{name: by}) == 1 and b"multiple" in L.tbk_last_error(), name

@@ -54,8 +54,15 @@ int check_sizes(const char *what, int64_t n, int64_t a, int64_t b) {
   return TBK_OK;
 }
 
-int check_matrix(const char *what, const void *p, int64_t ld, int64_t rows, int64_t cols) {
+// size: bytes of an element (the kernels read whole elements, and misaligned ones end a program)
+int check_address(const char *what, const void *p, int size) {
+  if (reinterpret_cast<uintptr_t>(p) % size) return fail(TBK_ERR_INVALID, "%s does not begin at a multiple of its elements' %d bytes", what, size);
+  return TBK_OK;
+}
+
+int check_matrix(const char *what, const void *p, int64_t ld, int64_t rows, int64_t cols, int size) {
   if (!p && rows > 0) return fail(TBK_ERR_INVALID, "%s is null", what);
+  if (const int rc = check_address(what, p, size)) return rc;
   if (ld < cols && rows > 1) return fail(TBK_ERR_INVALID, "%s: %lld elements from row to row are less than its %lld columns", what, (long long)ld, (long long)cols);
   if (ld > ((int64_t)1 << 38)) return fail(TBK_ERR_UNSUPPORTED, "%s: %lld elements from row to row", what, (long long)ld);
   return TBK_OK;

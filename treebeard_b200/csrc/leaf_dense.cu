@@ -395,11 +395,12 @@ int tbk_linear(const void *x, int64_t ld_x, const void *weight, int64_t ld_w, co
   const bool aligned = tma_rows(x, ld_x, n) && tma_rows(weight, ld_w, outputs);
   TRY(tbk_linear_workspace(n, inputs, outputs, type, aligned, device, &need));
   if (act < TBK_ACT_IDENTITY || act > TBK_ACT_SILU) return fail(TBK_ERR_INVALID, "unknown activation %d", act);
-  TRY(check_matrix("x", x, ld_x, n, inputs));
-  TRY(check_matrix("weight", weight, ld_w, outputs, inputs));
-  if (residual) TRY(check_matrix("residual", residual, ld_res, n, outputs));
-  TRY(check_matrix("out", out, ld_out, n, outputs));
-  if (pre) TRY(check_matrix("pre", pre, ld_pre, n, outputs));
+  TRY(check_matrix("x", x, ld_x, n, inputs, 2));
+  TRY(check_matrix("weight", weight, ld_w, outputs, inputs, 2));
+  if (residual) TRY(check_matrix("residual", residual, ld_res, n, outputs, 2));
+  TRY(check_matrix("out", out, ld_out, n, outputs, 2));
+  if (pre) TRY(check_matrix("pre", pre, ld_pre, n, outputs, 2));
+  TRY(check_address("bias", bias, 2));
   if (n == 0) return TBK_OK;
   TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(device);
@@ -448,13 +449,14 @@ int tbk_linear_backward(const void *grad, int64_t ld_grad, const void *x, int64_
   const bool aligned = tma_rows(x, ld_x, n) && tma_rows(weight, ld_w, outputs);
   TRY(tbk_linear_backward_workspace(n, inputs, outputs, type, aligned, device, &need));
   if (act < TBK_ACT_IDENTITY || act > TBK_ACT_SILU) return fail(TBK_ERR_INVALID, "unknown activation %d", act);
-  TRY(check_matrix("grad", grad, ld_grad, n, outputs));
-  TRY(check_matrix("x", x, ld_x, n, inputs));
-  TRY(check_matrix("weight", weight, ld_w, outputs, inputs));
-  if (act != TBK_ACT_IDENTITY) TRY(check_matrix("pre", pre, ld_pre, n, outputs));
-  if (skip) TRY(check_matrix("skip", skip, ld_skip, n, inputs));
-  if (grad_x) TRY(check_matrix("grad_x", grad_x, ld_gx, n, inputs));
-  if (grad_w) TRY(check_matrix("grad_weight", grad_w, ld_gw, outputs, inputs));
+  TRY(check_matrix("grad", grad, ld_grad, n, outputs, 2));
+  TRY(check_matrix("x", x, ld_x, n, inputs, 2));
+  TRY(check_matrix("weight", weight, ld_w, outputs, inputs, 2));
+  if (act != TBK_ACT_IDENTITY) TRY(check_matrix("pre", pre, ld_pre, n, outputs, 2));
+  if (skip) TRY(check_matrix("skip", skip, ld_skip, n, inputs, 2));
+  if (grad_x) TRY(check_matrix("grad_x", grad_x, ld_gx, n, inputs, 2));
+  if (grad_w) TRY(check_matrix("grad_weight", grad_w, ld_gw, outputs, inputs, 2));
+  TRY(check_address("grad_bias", grad_b, 2));
   if (outputs > 1 << 24) return fail(TBK_ERR_UNSUPPORTED, "linear_backward: %lld outputs", (long long)outputs);
   if (n > 0) TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(device);
@@ -511,6 +513,7 @@ int tbk_class_loss_workspace(int64_t n, int64_t width, int64_t classes, int32_t 
 static int check_labels(const void *labels, int32_t label_bytes, int64_t n) {
   if (!labels && n > 0) return fail(TBK_ERR_INVALID, "labels is null");
   if (label_bytes != 4 && label_bytes != 8) return fail(TBK_ERR_INVALID, "labels of %d bytes", label_bytes);
+  TRY(check_address("labels", labels, label_bytes));
   return TBK_OK;
 }
 
@@ -520,10 +523,13 @@ int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, int64_t ld_w
   uint64_t need = 0;
   const bool aligned = tma_rows(x, ld_x, n) && tma_rows(weight, ld_w, classes);
   TRY(tbk_class_loss_workspace(n, width, classes, type, aligned, device, &need));
-  TRY(check_matrix("x", x, ld_x, n, width));
-  TRY(check_matrix("weight", weight, ld_w, classes, width));
+  TRY(check_matrix("x", x, ld_x, n, width, 2));
+  TRY(check_matrix("weight", weight, ld_w, classes, width, 2));
   TRY(check_labels(labels, label_bytes, n));
   if (n > 0 && (!loss || !lse)) return fail(TBK_ERR_INVALID, "null output pointer");
+  TRY(check_address("bias", bias, 2));
+  TRY(check_address("loss", loss, 4));
+  TRY(check_address("lse", lse, 4));
   if (n == 0) return TBK_OK;
   TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(device);
@@ -570,12 +576,16 @@ int tbk_class_loss_backward(const float *grad, const void *x, int64_t ld_x, cons
   uint64_t need = 0;
   const bool aligned = tma_rows(x, ld_x, n) && tma_rows(weight, ld_w, classes);
   TRY(tbk_class_loss_backward_workspace(n, width, classes, type, aligned, device, &need));
-  TRY(check_matrix("x", x, ld_x, n, width));
-  TRY(check_matrix("weight", weight, ld_w, classes, width));
+  TRY(check_matrix("x", x, ld_x, n, width, 2));
+  TRY(check_matrix("weight", weight, ld_w, classes, width, 2));
   TRY(check_labels(labels, label_bytes, n));
   if (n > 0 && (!grad || !lse)) return fail(TBK_ERR_INVALID, "null input pointer");
-  if (grad_x) TRY(check_matrix("grad_x", grad_x, ld_gx, n, width));
-  if (grad_w) TRY(check_matrix("grad_weight", grad_w, ld_gw, classes, width));
+  TRY(check_address("bias", bias, 2));
+  TRY(check_address("grad_bias", grad_b, 2));
+  TRY(check_address("grad_loss", grad, 4));
+  TRY(check_address("lse", lse, 4));
+  if (grad_x) TRY(check_matrix("grad_x", grad_x, ld_gx, n, width, 2));
+  if (grad_w) TRY(check_matrix("grad_weight", grad_w, ld_gw, classes, width, 2));
   if (n > 0) TRY(check_workspace(ws, ws_bytes, need));
   OnDevice on(device);
   CUDA_TRY(on.error);

@@ -184,12 +184,13 @@ static int check_leaf_call(const tbk_leaf_map *map, const int32_t *ids, int64_t 
   TRY(check_sizes("leaf sum", n, width, 1));
   if (type != TBK_TYPE_F32 && type != TBK_TYPE_F16 && type != TBK_TYPE_BF16) return fail(TBK_ERR_INVALID, "unknown element type %d", type);
   if (width > 1 << 20) return fail(TBK_ERR_UNSUPPORTED, "leaf sum: %lld columns", (long long)width);
-  return check_matrix("leaf_ids", ids, ld_ids, n, map->view.num_trees);
+  return check_matrix("leaf_ids", ids, ld_ids, n, map->view.num_trees, 4);
 }
 
+static int element_bytes(int32_t type) { return type == TBK_TYPE_F32 ? 4 : 2; }
 // (the kernels multiply row numbers with 32-bit strides)
 static int check_stride(const char *what, int64_t ld, int32_t type) {
-  if (ld * (type == TBK_TYPE_F32 ? 4 : 2) > 0xffffffffll) return fail(TBK_ERR_UNSUPPORTED, "%s: %lld elements from row to row", what, (long long)ld);
+  if (ld * element_bytes(type) > 0xffffffffll) return fail(TBK_ERR_UNSUPPORTED, "%s: %lld elements from row to row", what, (long long)ld);
   return TBK_OK;
 }
 
@@ -204,8 +205,8 @@ int tbk_leaf_sum_workspace(const tbk_leaf_map *map, int64_t n, int64_t width, in
 int tbk_leaf_sum(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, const void *table, int64_t ld_table,
                  int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream_) {
   TRY(check_leaf_call(map, ids, n, ld_ids, width, type));
-  TRY(check_matrix("table", table, ld_table, map->rows, width));
-  TRY(check_matrix("out", out, ld_out, n, width));
+  TRY(check_matrix("table", table, ld_table, map->rows, width, element_bytes(type)));
+  TRY(check_matrix("out", out, ld_out, n, width, element_bytes(type)));
   TRY(check_stride("table", ld_table, type));
   if (n == 0) return TBK_OK;
   uint64_t need = 0;
@@ -266,15 +267,15 @@ int tbk_leaf_sum_backward_workspace(const tbk_leaf_map *map, int64_t n, int64_t 
 int tbk_leaf_sum_backward(const tbk_leaf_map *map, const int32_t *ids, int64_t n, int64_t ld_ids, const void *grad, int64_t ld_grad,
                           int64_t width, int32_t type, void *out, int64_t ld_out, void *ws, uint64_t ws_bytes, void *stream_) {
   TRY(check_leaf_call(map, ids, n, ld_ids, width, type));
-  TRY(check_matrix("grad", grad, ld_grad, n, width));
-  TRY(check_matrix("out", out, ld_out, map->rows, width));
+  TRY(check_matrix("grad", grad, ld_grad, n, width, element_bytes(type)));
+  TRY(check_matrix("out", out, ld_out, map->rows, width, element_bytes(type)));
   TRY(check_stride("grad", ld_grad, type));
   uint64_t need = 0;
   TRY(tbk_leaf_sum_backward_workspace(map, n, width, type, &need));
   OnDevice on(map->device);
   CUDA_TRY(on.error);
   cudaStream_t stream = (cudaStream_t)stream_;
-  const size_t size = type == TBK_TYPE_F32 ? 4 : 2;
+  const size_t size = element_bytes(type);
   if (n == 0) {
     CUDA_TRY(cudaMemset2DAsync(out, (size_t)ld_out * size, 0, (size_t)width * size, (size_t)map->rows, stream));
     return TBK_OK;
