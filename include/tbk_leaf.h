@@ -99,7 +99,8 @@ TBK_EXPORT int tbk_class_loss(const void *x, int64_t ld_x, const void *weight, i
 
 /* Gradients of sum_n grad_loss[n] * loss[n] (grad_loss fp32): with dz[n, v] = grad_loss[n] * (exp(z[n, v] -
  * lse[n]) - [v = labels[n]]), grad_x = dz weight, grad_weight = dz^T x, grad_bias = sum of dz's rows; each may
- * be NULL (not wanted).  The scores are computed again, a piece of the classes at a time; dz is rounded to
+ * be NULL (not wanted).  A row without a label has zeros for dz, which its x is multiplied with: x has to be finite
+ * there too.  The scores are computed again, a piece of the classes at a time; dz is rounded to
  * `type`, scaled by a power of two so that the largest |grad_loss| of a row with a label lies near the middle of the
  * type's range (grad_bias is summed before that). */
 TBK_EXPORT int tbk_class_loss_backward_workspace(int64_t n_rows, int64_t width, int64_t classes, int32_t type,

@@ -359,7 +359,8 @@ def class_loss(x, weight, labels, bias=None):
 @_on_stream
 def class_loss_backward(grad_loss, x, weight, labels, lse, bias=None):
     """Gradients of sum(grad_loss * loss) with respect to x, weight and, where one is given, bias.
-    grad_loss: fp32 [n], every row's weight in the objective (1/n for the mean); lse: what class_loss gave."""
+    grad_loss: fp32 [n], every row's weight in the objective (1/n for the mean); lse: what class_loss gave.  Rows without
+    a label add nothing, provided that x is finite there (zero times a NaN is one, in weight's gradient)."""
     kind, ld_x, ld_w, n, width, classes = _class_call("class_loss_backward", x, weight, labels, bias)
     _vector("grad_loss", grad_loss, torch.float32, n)
     _vector("lse", lse, torch.float32, n)
